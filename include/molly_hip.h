@@ -407,6 +407,47 @@ int molly_attn_decode_qkv(void* stream, const float* qkv_slabs, int n_slabs, con
                           int kv_len_hint, float* workspace, long workspace_floats);
 
 /* ------------------------------------------------------------------------------------------------
+ * A paged key / value cache for `generate` (the reference keeps HF's DynamicCache, src/model/omics_one.py:220-232: one dense tensor a layer).
+ * A layer's cache is two pools, K and V, [n_pages][n_kv_heads][page_size][head_dim] contiguous, 16-byte aligned; a place (slot) is
+ * page * page_size + offset.  page_size: a power of two in 16..256; head_dim 64 | 128; n_pages * page_size < 2^31.
+ * kscale / vscale NULL: bf16 pools.  Given: e4m3 pools (1 byte a value) and their exponent bytes [n_pages][n_kv_heads][page_size]: a head of a
+ * token holds code * 2^(e - 127), e the smallest with which its largest finite magnitude is at most 448 * 2^(e - 127); infinities and NaN are NaN.
+ *
+ * append: rows of k and v (row strides ldk / ldv) go to slot[row]; a slot outside the pool (-1) skips the row.  With gains (nullable, each by
+ * itself) the heads of q and k get RMSNorm, with cos / sin [n_pos][head_dim / 2] rotary at positions[row] (HF:models/qwen3/
+ * modeling_qwen3.py:225-236); a position outside the tables makes the row's heads NaN.  q rows (nullable) go to q_out (q_out == q allowed).
+ * fp32 throughout, one rounding where a value is stored.  Slots of one call are distinct (two rows with one slot: the pool keeps
+ * values of either).
+ * read: the rows of slot[] back as bf16 (exact for either kind of pool); a slot outside the pool gives a row of zeros. */
+int molly_paged_kv_append(void* stream, const void* k, const void* v, const void* q_or_null, void* q_out_or_null, void* kpool, void* vpool,
+                          void* kscale_or_null, void* vscale_or_null, const int* slot, int n_rows, int n_pages, int page_size, int n_heads,
+                          int n_kv_heads, int head_dim, int ldq, int ldk, int ldv, int ldqo, const void* q_norm_w, const void* k_norm_w,
+                          const float* cos, const float* sin, const int* positions, int n_pos, float eps);
+int molly_paged_kv_read(void* stream, const void* kpool, const void* vpool, const void* kscale_or_null, const void* vscale_or_null,
+                        const int* slot, int n_rows, int n_pages, int page_size, int n_kv_heads, int head_dim, void* k_out, void* v_out,
+                        int ldk, int ldv);
+/* attention of ragged chunks of new tokens over the pages: sequence b has the q rows cu_q[b] .. cu_q[b + 1] - 1 (cu_q int [B + 1], ascending),
+ * kv_len[b] keys in the cache, the new tokens' own among them (they are its last ones), and key j in page block_table[b][j / page_size] (row
+ * stride ld_table).  Row i of the n new ones sees the keys 0 .. kv_len[b] - n + i; a row that sees none comes out as zeros; a row
+ * one of whose keys lies on a page outside 0 .. n_pages - 1, or behind max_pages, comes out as NaN (no memory outside the pools is read); rows
+ * in front of cu_q[0] or behind cu_q[B] are left as they were.  One new token a sequence is the decode step. */
+int molly_attn_paged(void* stream, const void* q, void* out, const void* kpool, const void* vpool, const void* kscale_or_null,
+                     const void* vscale_or_null, const int* block_table, const int* cu_q, const int* kv_len, int n_tokens, int B, int n_pages,
+                     int page_size, int max_pages, int ld_table, int n_heads, int n_kv_heads, int head_dim, int ldq, int ldo, float scale);
+
+/* Logit processors in front of the draw, one pass: logits [rows][ld_logits] (fp32, or bf16 when logits_bf16) -> out fp32 [rows][ld_out]
+ * (out == logits allowed for fp32 with the same stride).  c = occurrences of the token among the first n_generated[row] (NULL: n_history)
+ * entries of generated [rows][ld_generated] (ids outside 0 .. V - 1 are ignored):
+ *   c > 0: s = (s < 0 ? s * repetition : s / repetition) - presence - frequency * c;  s += bias;  s = -inf where the token is not allowed
+ * (HF:generation/logits_process.py RepetitionPenaltyLogitsProcessor, then the additive ones, then the hard ones).  The three penalties: scalars, or
+ * fp32 [rows] where *_rows is given.  bias fp32 [V] (ld_bias 0: one for all rows) or [rows][ld_bias]; allowed: bit v & 31 of word v >> 5 set =
+ * token v allowed, [words] (ld_allowed 0) or [rows][ld_allowed]. */
+int molly_process_logits(void* stream, const void* logits, int logits_bf16, float* out, int rows, int V, long ld_logits, long ld_out,
+                         const int64_t* generated, const int* n_generated_or_null, int n_history, long ld_generated, float repetition,
+                         float presence, float frequency, const float* repetition_rows, const float* presence_rows,
+                         const float* frequency_rows, const float* bias, long ld_bias, const void* allowed, long ld_allowed);
+
+/* ------------------------------------------------------------------------------------------------
  * LoRA branch  y = W x + (alpha/r) * B (A dropout(x))  — PEFT lora.Linear.forward as the reference configures it
  * (src/utils/tools.py:379-389: r = --lora_r, lora_alpha 64, lora_dropout 0.05).  The rank-r contractions are
  * molly_gemm_bf16 calls; these are the HBM-bound parts.

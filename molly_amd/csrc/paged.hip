@@ -1,0 +1,359 @@
+// The paged key / value cache of `generate` and the attention that reads it.
+//   molly_paged_kv_append : rows of k and v (and q) -> q/k-norm, rotary -> the pages of the cache, bf16 or e4m3
+//   molly_paged_kv_read   : the rows of a list of places, back as bf16
+//   molly_attn_paged      : ragged chunks of new tokens attend causally to everything their sequence has in the pages
+// The reference's `generate` keeps HF's DynamicCache (reference src/model/omics_one.py:220-232), one dense tensor a layer that is
+// concatenated to at every step; here a layer's cache is a pool of pages [n_pages][n_kv_heads][page_size][head_dim], and a sequence is a
+// row of page ids.  Head-major: the keys of one (page, head) are contiguous, so what one workgroup of the attention reads are
+// whole lines, page_size * head_dim values at a time.
+//
+// e4m3 pools: a head of a token is held as codes and ONE exponent byte e: value = code * 2^(e - 127).  e is the smallest power of two that
+// brings the head's largest magnitude to 448 (the format's largest value) or less.  With a power of two the division and the product
+// are exact: the only rounding is the code's own (round to nearest even, half a step: 2^-4 of the value), the value read back is
+// a bf16 without rounding, and one conversion instruction (v_cvt_scalef32_pk_bf16_fp8) makes two of them.  What a
+// free scale would gain is nothing above the format's subnormals: a code keeps its 4 significant bits wherever it sits in the 15 octaves.
+#include "common.h"
+#include "molly_hip.h"
+
+namespace {
+
+__device__ __forceinline__ float exp2i(int e) { return __builtin_bit_cast(float, (unsigned)(e + 127) << 23); }      // 2^e, -126 <= e <= 127
+
+// the exponent byte of a head whose largest finite magnitude is amax (448 = 1.75 * 2^8)
+__device__ __forceinline__ int e4m3_exponent(float amax) {
+    const unsigned u = __builtin_bit_cast(unsigned, amax);
+    const int e = (int)(u >> 23) - 8 + ((u & 0x7fffffu) > 0x600000u ? 1 : 0);
+    return min(max(e, 1), 254);
+}
+// four codes; a value that is not finite becomes the format's NaN (e4m3 has no infinity)
+__device__ __forceinline__ unsigned e4m3_pack4(const float* x, float inv) {
+    float y[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) y[i] = fabsf(x[i]) < INFINITY ? x[i] * inv : __builtin_nanf("");
+    int w = __builtin_amdgcn_cvt_pk_fp8_f32(y[0], y[1], 0, false);
+    w = __builtin_amdgcn_cvt_pk_fp8_f32(y[2], y[3], w, true);
+    return (unsigned)w;
+}
+// eight codes -> eight bf16, times the power of two `scale`
+__device__ __forceinline__ u32x4 e4m3_to_bf8(u32x2 c, float scale) {
+    u32x4 r;
+    r[0] = __builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(c[0], scale, false));
+    r[1] = __builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(c[0], scale, true));
+    r[2] = __builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(c[1], scale, false));
+    r[3] = __builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(c[1], scale, true));
+    return r;
+}
+
+struct AppendArgs {
+    const bf16_t* q; const bf16_t* k; const bf16_t* v; bf16_t* q_out;
+    void* kpool; void* vpool; uint8_t* kscale; uint8_t* vscale;
+    const int* slot; const bf16_t* qw; const bf16_t* kw; const float* cos; const float* sin; const int* pos;
+    long n_slots;                                    // pages * page size
+    int n, nq, nkv, ldq, ldk, ldv, ldqo, page_shift, n_pos;
+    float eps;
+};
+
+// One block = a run of tokens x one head: the tokens of a prompt lie next to each other in a page, so the block's stores are one contiguous
+// run of the pool (and of its exponent bytes); the rows it reads are pieces of HD * 2 bytes.  A thread owns 8 + 8 elements of a head,
+// its rotary partners among them; HD / 16 lanes hold a head.  Bound by HBM: every byte is touched once.
+template <int HD, bool FP8>
+__global__ __launch_bounds__(256) void paged_append_kernel(AppendArgs p) {
+    constexpr int LPH = HD / 16, TPB = 256 / LPH, half = HD / 2;
+    const int sub = threadIdx.x % LPH;
+    const int row = blockIdx.x * TPB + threadIdx.x / LPH;
+    const int head = blockIdx.y;                     // q heads, k heads, v heads
+    const bool isq = head < p.nq, isk = !isq && head < p.nq + p.nkv;
+    const int h = isq ? head : isk ? head - p.nq : head - p.nq - p.nkv;
+    const bool live = row < p.n;
+    const int r = live ? row : p.n - 1;              // (the lanes behind the last row stay: the head's sums are taken over lanes)
+    const bf16_t* src = (isq ? p.q + (size_t)r * p.ldq : isk ? p.k + (size_t)r * p.ldk : p.v + (size_t)r * p.ldv) + h * HD + sub * 8;
+    const u32x4 a = *reinterpret_cast<const u32x4*>(src), b = *reinterpret_cast<const u32x4*>(src + half);
+    float x[8], y[8];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+        const unsigned ae = a[e], be = b[e];
+        x[2 * e] = bflo(ae); x[2 * e + 1] = bfhi(ae);
+        y[2 * e] = bflo(be); y[2 * e + 1] = bfhi(be);
+    }
+    const bf16_t* w = isq ? p.qw : isk ? p.kw : nullptr;
+    if (w) {                                         // (block-uniform) fp32 throughout: the row is rounded once, where it is stored
+        float ss = 0.f;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) ss += x[e] * x[e] + y[e] * y[e];
+#pragma unroll
+        for (int o = 1; o < LPH; o <<= 1) ss += __shfl_xor(ss, o, 64);
+        const float rstd = rsqrtf(ss * (1.f / HD) + p.eps);
+        const u32x4 wa = *reinterpret_cast<const u32x4*>(w + sub * 8), wb = *reinterpret_cast<const u32x4*>(w + half + sub * 8);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            const unsigned u = wa[e], v = wb[e];
+            x[2 * e] *= rstd * bflo(u); x[2 * e + 1] *= rstd * bfhi(u);
+            y[2 * e] *= rstd * bflo(v); y[2 * e + 1] *= rstd * bfhi(v);
+        }
+    }
+    if (p.cos && (isq || isk)) {
+        const int pos = p.pos[r];
+        const bool known = pos >= 0 && pos < p.n_pos;                 // a position outside the tables: the head is NaN
+        const size_t at = (size_t)(known ? pos : 0) * half + sub * 8;
+#pragma unroll
+        for (int g = 0; g < 2; ++g) {
+            const f32x4 c = *reinterpret_cast<const f32x4*>(p.cos + at + 4 * g), s = *reinterpret_cast<const f32x4*>(p.sin + at + 4 * g);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const float cc = known ? c[e] : __builtin_nanf(""), x1 = x[4 * g + e], x2 = y[4 * g + e];
+                x[4 * g + e] = x1 * cc - x2 * s[e];
+                y[4 * g + e] = x2 * cc + x1 * s[e];
+            }
+        }
+    }
+    auto pack8 = [](const float* f) { return u32x4{pack_bf2(f[0], f[1]), pack_bf2(f[2], f[3]), pack_bf2(f[4], f[5]), pack_bf2(f[6], f[7])}; };
+    if (isq) {
+        if (!live) return;
+        bf16_t* d = p.q_out + (size_t)row * p.ldqo + h * HD + sub * 8;
+        *reinterpret_cast<u32x4*>(d) = pack8(x);
+        *reinterpret_cast<u32x4*>(d + half) = pack8(y);
+        return;
+    }
+    const long s = live ? p.slot[row] : -1;
+    const bool keep = s >= 0 && s < p.n_slots;       // anything else: a row of padding
+    const size_t key = (((size_t)(s >> p.page_shift) * p.nkv + h) << p.page_shift) + (s & ((1 << p.page_shift) - 1));
+    if constexpr (FP8) {
+        float m = 0.f;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            const float u = fabsf(x[e]), v = fabsf(y[e]);
+            m = fmaxf(m, fmaxf(u < INFINITY ? u : 0.f, v < INFINITY ? v : 0.f));
+        }
+#pragma unroll
+        for (int o = 1; o < LPH; o <<= 1) m = fmaxf(m, __shfl_xor(m, o, 64));
+        if (!keep) return;
+        const int e = e4m3_exponent(m);
+        const float inv = exp2i(127 - e);                              // (e <= 247: m is finite)
+        uint8_t* d = (uint8_t*)(isk ? p.kpool : p.vpool) + key * HD + sub * 8;
+        *reinterpret_cast<u32x2*>(d) = u32x2{e4m3_pack4(x, inv), e4m3_pack4(x + 4, inv)};
+        *reinterpret_cast<u32x2*>(d + half) = u32x2{e4m3_pack4(y, inv), e4m3_pack4(y + 4, inv)};
+        if (sub == 0) (isk ? p.kscale : p.vscale)[key] = (uint8_t)e;
+    } else {
+        if (!keep) return;
+        bf16_t* d = (bf16_t*)(isk ? p.kpool : p.vpool) + key * HD + sub * 8;
+        *reinterpret_cast<u32x4*>(d) = pack8(x);
+        *reinterpret_cast<u32x4*>(d + half) = pack8(y);
+    }
+}
+
+struct ReadArgs {
+    const void* kpool; const void* vpool; const uint8_t* kscale; const uint8_t* vscale;
+    const int* slot; bf16_t* k_out; bf16_t* v_out;
+    long n_slots;
+    int n, nkv, ldk, ldv, page_shift;
+};
+
+// The append's block shape the other way round: a run of places x one head of K or V, 16 elements a thread.
+template <int HD, bool FP8>
+__global__ __launch_bounds__(256) void paged_read_kernel(ReadArgs p) {
+    constexpr int LPH = HD / 16, TPB = 256 / LPH;
+    const int sub = threadIdx.x % LPH;
+    const int row = blockIdx.x * TPB + threadIdx.x / LPH;
+    if (row >= p.n) return;
+    const bool isk = (int)blockIdx.y < p.nkv;
+    const int h = isk ? blockIdx.y : blockIdx.y - p.nkv;
+    const long s = p.slot[row];
+    u32x4 a = {0, 0, 0, 0}, b = {0, 0, 0, 0};        // a place outside the pool holds nothing
+    if (s >= 0 && s < p.n_slots) {
+        const size_t key = (((size_t)(s >> p.page_shift) * p.nkv + h) << p.page_shift) + (s & ((1 << p.page_shift) - 1));
+        if constexpr (FP8) {
+            const u32x4 c = *reinterpret_cast<const u32x4*>((const uint8_t*)(isk ? p.kpool : p.vpool) + key * HD + sub * 16);
+            const float scale = exp2i((int)(isk ? p.kscale : p.vscale)[key] - 127);
+            a = e4m3_to_bf8(u32x2{c[0], c[1]}, scale);
+            b = e4m3_to_bf8(u32x2{c[2], c[3]}, scale);
+        } else {
+            const u32x4* c = reinterpret_cast<const u32x4*>((const bf16_t*)(isk ? p.kpool : p.vpool) + key * HD + sub * 16);
+            a = c[0]; b = c[1];
+        }
+    }
+    u32x4* d = reinterpret_cast<u32x4*>((isk ? p.k_out + (size_t)row * p.ldk : p.v_out + (size_t)row * p.ldv) + h * HD + sub * 16);
+    d[0] = a; d[1] = b;
+}
+
+struct AttnPagedArgs {
+    const bf16_t* q; bf16_t* out;
+    const void* kpool; const void* vpool; const uint8_t* kscale; const uint8_t* vscale;
+    const int* table; const int* cu_q; const int* kv_len;
+    int n_tok, B, n_pages, page_shift, max_pages, ld_table, nh, nkv, ldq, ldo;
+    float qscale;                                    // softmax scale * log2(e)
+};
+
+// the sequence of row `t`: the last b with cu_q[b] <= t (B when t lies behind the last one)
+__device__ __forceinline__ int find_seq(const int* cu, int B, int t) {
+    int lo = 0, hi = B;                              // cu[lo] <= t < cu[hi + 1] ..
+    while (lo < hi) {
+        const int mid = (lo + hi) >> 1;
+        if (cu[mid + 1] <= t) lo = mid + 1; else hi = mid;
+    }
+    return lo;
+}
+
+// one value of a pool
+template <bool FP8>
+__device__ __forceinline__ float pool_value(const void* pool, const uint8_t* scale, size_t key, int HD, int d) {
+    if (FP8) {
+        const unsigned c = ((const uint8_t*)pool)[key * HD + d];
+        const unsigned r = __builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(c, exp2i((int)scale[key] - 127), false));
+        return bflo(r);
+    }
+    return bf2f(((const bf16_t*)pool)[key * HD + d]);
+}
+
+// One wave per (token, head): every lane owns HD / 64 columns, the keys go by one at a time with a running maximum and sum.
+template <int HD, bool FP8>
+__global__ __launch_bounds__(64) void attn_paged_simple_kernel(AttnPagedArgs p) {
+    constexpr int C = HD / 64;
+    const int t = blockIdx.x, head = blockIdx.y, lane = threadIdx.x;
+    const int kvh = head / (p.nh / p.nkv);
+    if (t < p.cu_q[0]) return;
+    const int b = find_seq(p.cu_q, p.B, t);
+    if (b >= p.B) return;                            // behind the last sequence: left as it was
+    const int n = p.cu_q[b + 1] - p.cu_q[b];
+    const int last = p.kv_len[b] - n + (t - p.cu_q[b]);                 // the last key this row sees
+    float qv[C], acc[C], m = -INFINITY, l = 0.f;
+#pragma unroll
+    for (int c = 0; c < C; ++c) { qv[c] = bf2f(p.q[(size_t)t * p.ldq + head * HD + c * 64 + lane]) * p.qscale; acc[c] = 0.f; }
+    for (int key = 0; key <= last; ++key) {
+        const int pi = key >> p.page_shift;
+        const int page = pi < p.max_pages ? p.table[(size_t)b * p.ld_table + pi] : -1;
+        if (page < 0 || page >= p.n_pages) { l = __builtin_nanf(""); break; }
+        const size_t at = (((size_t)page * p.nkv + kvh) << p.page_shift) + (key & ((1 << p.page_shift) - 1));
+        float s = 0.f;
+#pragma unroll
+        for (int c = 0; c < C; ++c) s += qv[c] * pool_value<FP8>(p.kpool, p.kscale, at, HD, c * 64 + lane);
+        s = wave_sum(s);
+        const float mn = fmaxf(m, s), mu = mn == -INFINITY ? 0.f : mn;
+        const float a = __builtin_amdgcn_exp2f(m - mu), e = __builtin_amdgcn_exp2f(s - mu);
+        l = l * a + e;
+#pragma unroll
+        for (int c = 0; c < C; ++c) acc[c] = acc[c] * a + e * pool_value<FP8>(p.vpool, p.vscale, at, HD, c * 64 + lane);
+        m = mn;
+    }
+    const float inv = l == 0.f ? 0.f : 1.f / l;
+#pragma unroll
+    for (int c = 0; c < C; ++c) p.out[(size_t)t * p.ldo + head * HD + c * 64 + lane] = f2bf(acc[c] * inv);
+}
+
+int log2_exact(int x) {
+    for (int s = 0; s < 31; ++s)
+        if (x == 1 << s) return s;
+    return -1;
+}
+bool aligned16(const void* p) { return ((uintptr_t)p % 16) == 0; }
+
+// what the three entry points ask of a cache
+int check_pool(const char* what, const void* kpool, const void* vpool, const void* kscale, const void* vscale, int n_pages, int page_size,
+               int n_kv_heads, int head_dim) {
+    MOLLY_CHECK(head_dim == 64 || head_dim == 128, "%s: head_dim=%d (built for 64 and 128)", what, head_dim);
+    MOLLY_CHECK(n_pages > 0 && n_kv_heads > 0 && page_size >= 16 && page_size <= 256 && log2_exact(page_size) >= 0,
+                "%s: n_pages=%d n_kv_heads=%d page_size=%d (a power of two in 16..256)", what, n_pages, n_kv_heads, page_size);
+    MOLLY_CHECK((long)n_pages * page_size <= 0x7fffffffL, "%s: %d pages of %d places: places are 32-bit", what, n_pages, page_size);
+    MOLLY_CHECK(kpool && vpool && aligned16(kpool) && aligned16(vpool), "%s: the pools must be 16-byte aligned device memory", what);
+    MOLLY_CHECK((kscale == nullptr) == (vscale == nullptr), "%s: e4m3 pools have exponents for K and for V", what);
+    return 0;
+}
+
+}  // namespace
+
+extern "C" int molly_paged_kv_append(void* stream, const void* k, const void* v, const void* q_or_null, void* q_out_or_null, void* kpool,
+                                     void* vpool, void* kscale_or_null, void* vscale_or_null, const int* slot, int n_rows, int n_pages,
+                                     int page_size, int n_heads, int n_kv_heads, int head_dim, int ldq, int ldk, int ldv, int ldqo,
+                                     const void* q_norm_w, const void* k_norm_w, const float* cos, const float* sin, const int* positions,
+                                     int n_pos, float eps) {
+    MOLLY_ENTER();
+    if (int rc = check_pool("paged_kv_append", kpool, vpool, kscale_or_null, vscale_or_null, n_pages, page_size, n_kv_heads, head_dim)) return rc;
+    const int nq = q_or_null ? n_heads : 0;
+    MOLLY_CHECK(n_rows >= 0 && nq >= 0 && k && v && slot, "paged_kv_append: n_rows=%d n_heads=%d; k, v, slot required", n_rows, n_heads);
+    MOLLY_CHECK((q_or_null == nullptr) == (q_out_or_null == nullptr), "paged_kv_append: q and q_out go together");
+    MOLLY_CHECK((cos == nullptr) == (sin == nullptr) && (cos == nullptr || (positions != nullptr && n_pos > 0)),
+                "paged_kv_append: cos, sin and positions go together (n_pos=%d)", n_pos);
+    MOLLY_CHECK((nq + 2L * n_kv_heads) <= 65535, "paged_kv_append: %d + 2 * %d heads", nq, n_kv_heads);
+    MOLLY_CHECK(aligned16(k) && aligned16(v) && ldk % 8 == 0 && ldv % 8 == 0 && ldk >= n_kv_heads * head_dim && ldv >= n_kv_heads * head_dim,
+                "paged_kv_append: k / v rows must be 16-byte aligned and hold n_kv_heads * head_dim values (ldk=%d ldv=%d)", ldk, ldv);
+    MOLLY_CHECK(nq == 0 || (aligned16(q_or_null) && aligned16(q_out_or_null) && ldq % 8 == 0 && ldqo % 8 == 0 && ldq >= nq * head_dim &&
+                            ldqo >= nq * head_dim), "paged_kv_append: q rows must be 16-byte aligned and hold n_heads * head_dim values (ldq=%d ldqo=%d)",
+                ldq, ldqo);
+    MOLLY_CHECK(aligned16(q_norm_w) && aligned16(k_norm_w) && aligned16(cos) && aligned16(sin), "paged_kv_append: gains / tables must be 16-byte aligned");
+    if (n_rows == 0) return 0;
+    AppendArgs p{};
+    p.q = (const bf16_t*)q_or_null; p.k = (const bf16_t*)k; p.v = (const bf16_t*)v; p.q_out = (bf16_t*)q_out_or_null;
+    p.kpool = kpool; p.vpool = vpool; p.kscale = (uint8_t*)kscale_or_null; p.vscale = (uint8_t*)vscale_or_null;
+    p.slot = slot; p.qw = (const bf16_t*)q_norm_w; p.kw = (const bf16_t*)k_norm_w; p.cos = cos; p.sin = sin; p.pos = positions;
+    p.n_slots = (long)n_pages * page_size;
+    p.n = n_rows; p.nq = nq; p.nkv = n_kv_heads; p.ldq = ldq; p.ldk = ldk; p.ldv = ldv; p.ldqo = ldqo;
+    p.page_shift = log2_exact(page_size); p.n_pos = n_pos; p.eps = eps;
+    const dim3 grid(cdiv(n_rows, 256 / (head_dim / 16)), nq + 2 * n_kv_heads);
+    hipStream_t st = (hipStream_t)stream;
+    if (head_dim == 128) {
+        if (kscale_or_null) hipLaunchKernelGGL((paged_append_kernel<128, true>), grid, dim3(256), 0, st, p);
+        else hipLaunchKernelGGL((paged_append_kernel<128, false>), grid, dim3(256), 0, st, p);
+    } else {
+        if (kscale_or_null) hipLaunchKernelGGL((paged_append_kernel<64, true>), grid, dim3(256), 0, st, p);
+        else hipLaunchKernelGGL((paged_append_kernel<64, false>), grid, dim3(256), 0, st, p);
+    }
+    MOLLY_LAUNCH_CHECK();
+    return 0;
+}
+
+extern "C" int molly_paged_kv_read(void* stream, const void* kpool, const void* vpool, const void* kscale_or_null, const void* vscale_or_null,
+                                   const int* slot, int n_rows, int n_pages, int page_size, int n_kv_heads, int head_dim, void* k_out,
+                                   void* v_out, int ldk, int ldv) {
+    MOLLY_ENTER();
+    if (int rc = check_pool("paged_kv_read", kpool, vpool, kscale_or_null, vscale_or_null, n_pages, page_size, n_kv_heads, head_dim)) return rc;
+    MOLLY_CHECK(n_rows >= 0 && slot && k_out && v_out && 2L * n_kv_heads <= 65535, "paged_kv_read: n_rows=%d; slot, k_out, v_out required", n_rows);
+    MOLLY_CHECK(aligned16(k_out) && aligned16(v_out) && ldk % 8 == 0 && ldv % 8 == 0 && ldk >= n_kv_heads * head_dim && ldv >= n_kv_heads * head_dim,
+                "paged_kv_read: output rows must be 16-byte aligned and hold n_kv_heads * head_dim values (ldk=%d ldv=%d)", ldk, ldv);
+    if (n_rows == 0) return 0;
+    ReadArgs p{};
+    p.kpool = kpool; p.vpool = vpool; p.kscale = (const uint8_t*)kscale_or_null; p.vscale = (const uint8_t*)vscale_or_null;
+    p.slot = slot; p.k_out = (bf16_t*)k_out; p.v_out = (bf16_t*)v_out;
+    p.n_slots = (long)n_pages * page_size; p.n = n_rows; p.nkv = n_kv_heads; p.ldk = ldk; p.ldv = ldv; p.page_shift = log2_exact(page_size);
+    const dim3 grid(cdiv(n_rows, 256 / (head_dim / 16)), 2 * n_kv_heads);
+    hipStream_t st = (hipStream_t)stream;
+    if (head_dim == 128) {
+        if (kscale_or_null) hipLaunchKernelGGL((paged_read_kernel<128, true>), grid, dim3(256), 0, st, p);
+        else hipLaunchKernelGGL((paged_read_kernel<128, false>), grid, dim3(256), 0, st, p);
+    } else {
+        if (kscale_or_null) hipLaunchKernelGGL((paged_read_kernel<64, true>), grid, dim3(256), 0, st, p);
+        else hipLaunchKernelGGL((paged_read_kernel<64, false>), grid, dim3(256), 0, st, p);
+    }
+    MOLLY_LAUNCH_CHECK();
+    return 0;
+}
+
+extern "C" int molly_attn_paged(void* stream, const void* q, void* out, const void* kpool, const void* vpool, const void* kscale_or_null,
+                                const void* vscale_or_null, const int* block_table, const int* cu_q, const int* kv_len, int n_tokens, int B,
+                                int n_pages, int page_size, int max_pages, int ld_table, int n_heads, int n_kv_heads, int head_dim, int ldq,
+                                int ldo, float scale) {
+    MOLLY_ENTER();
+    if (int rc = check_pool("attn_paged", kpool, vpool, kscale_or_null, vscale_or_null, n_pages, page_size, n_kv_heads, head_dim)) return rc;
+    MOLLY_CHECK(n_tokens >= 0 && B >= 0 && max_pages >= 0 && ld_table >= max_pages, "attn_paged: n_tokens=%d B=%d max_pages=%d ld_table=%d", n_tokens, B,
+                max_pages, ld_table);
+    MOLLY_CHECK(n_heads > 0 && n_heads % n_kv_heads == 0 && n_heads <= 65535, "attn_paged: n_heads=%d not a multiple of n_kv_heads=%d", n_heads, n_kv_heads);
+    if (n_tokens == 0 || B == 0) return 0;
+    MOLLY_CHECK(q && out && block_table && cu_q && kv_len, "attn_paged: q, out, block_table, cu_q, kv_len required");
+    MOLLY_CHECK(aligned16(q) && aligned16(out) && ldq % 8 == 0 && ldo % 8 == 0 && ldq >= n_heads * head_dim && ldo >= n_heads * head_dim,
+                "attn_paged: q / out rows must be 16-byte aligned and hold n_heads * head_dim values (ldq=%d ldo=%d)", ldq, ldo);
+    AttnPagedArgs p{};
+    p.q = (const bf16_t*)q; p.out = (bf16_t*)out; p.kpool = kpool; p.vpool = vpool;
+    p.kscale = (const uint8_t*)kscale_or_null; p.vscale = (const uint8_t*)vscale_or_null;
+    p.table = block_table; p.cu_q = cu_q; p.kv_len = kv_len; p.n_tok = n_tokens; p.B = B;
+    p.n_pages = n_pages; p.page_shift = log2_exact(page_size); p.max_pages = max_pages; p.ld_table = ld_table;
+    p.nh = n_heads; p.nkv = n_kv_heads; p.ldq = ldq; p.ldo = ldo; p.qscale = scale * 1.44269504088896341f;
+    const dim3 grid(n_tokens, n_heads);
+    hipStream_t st = (hipStream_t)stream;
+    if (head_dim == 128) {
+        if (kscale_or_null) hipLaunchKernelGGL((attn_paged_simple_kernel<128, true>), grid, dim3(64), 0, st, p);
+        else hipLaunchKernelGGL((attn_paged_simple_kernel<128, false>), grid, dim3(64), 0, st, p);
+    } else {
+        if (kscale_or_null) hipLaunchKernelGGL((attn_paged_simple_kernel<64, true>), grid, dim3(64), 0, st, p);
+        else hipLaunchKernelGGL((attn_paged_simple_kernel<64, false>), grid, dim3(64), 0, st, p);
+    }
+    MOLLY_LAUNCH_CHECK();
+    return 0;
+}

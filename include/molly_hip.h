@@ -430,10 +430,16 @@ int molly_paged_kv_read(void* stream, const void* kpool, const void* vpool, cons
  * kv_len[b] keys in the cache, the new tokens' own among them (they are its last ones), and key j in page block_table[b][j / page_size] (row
  * stride ld_table).  Row i of the n new ones sees the keys 0 .. kv_len[b] - n + i; a row that sees none comes out as zeros; a row
  * one of whose keys lies on a page outside 0 .. n_pages - 1, or behind max_pages, comes out as NaN (no memory outside the pools is read); rows
- * in front of cu_q[0] or behind cu_q[B] are left as they were.  One new token a sequence is the decode step. */
+ * in front of cu_q[0] or behind cu_q[B] are left as they were.  One new token a sequence is the decode step.  scale > 0.
+ * max_q / max_kv: the most new tokens / keys of any sequence, as far as the caller knows (0: no idea); they choose how the work is cut, never the
+ * result's meaning.  workspace: molly_attn_paged_workspace(the same arguments) floats for the parts of cut key axes (0: none is wanted; NULL or
+ * too small: the key axes stay whole); calls that may run at the same time need one each. */
+int molly_attn_paged_workspace(int n_tokens, int B, int n_heads, int n_kv_heads, int head_dim, int page_size, int max_pages, int e4m3,
+                               int max_q, int max_kv);
 int molly_attn_paged(void* stream, const void* q, void* out, const void* kpool, const void* vpool, const void* kscale_or_null,
                      const void* vscale_or_null, const int* block_table, const int* cu_q, const int* kv_len, int n_tokens, int B, int n_pages,
-                     int page_size, int max_pages, int ld_table, int n_heads, int n_kv_heads, int head_dim, int ldq, int ldo, float scale);
+                     int page_size, int max_pages, int ld_table, int n_heads, int n_kv_heads, int head_dim, int ldq, int ldo, float scale,
+                     int max_q, int max_kv, float* workspace, long workspace_floats);
 
 /* Logit processors in front of the draw, one pass: logits [rows][ld_logits] (fp32, or bf16 when logits_bf16) -> out fp32 [rows][ld_out]
  * (out == logits allowed for fp32 with the same stride).  c = occurrences of the token among the first n_generated[row] (NULL: n_history)

@@ -1,0 +1,729 @@
+// Attention of ragged chunks of new tokens over the paged cache (layout: paged.h).
+//   out[t, h] = sum_j softmax_j(scale q . k_j) v_j   over the keys j <= kv_len - n + i  of the sequence that row t, its i-th of n new ones, is in
+// replaces the attention of HF's generate over a DynamicCache (reference src/model/omics_one.py:220-232; HF:models/qwen3/
+// modeling_qwen3.py:185-208) for prompts taken in pieces, continued sequences and batches that mix both with decode steps.
+//
+// The query heads of a kv head are packed into the rows of one tile (row = token * G + head of the group), so K and V are read once for all of
+// them whatever G is; the arithmetic is that of attention.hip: S^T = K Q^T and O^T = V^T P^T by 32x32x16 MFMA, online softmax in the exp2
+// domain in fp32, P rounded to bf16 (2^-8 of a term) for the second product.  Two kernels:
+//   attn_paged_rows_kernel : up to 32 rows a tile (decode, short chunks).  The four waves of a block take every fourth step of 32 keys, each with
+//                            K / V images of its own in LDS: no workgroup barrier in the loop, the waves meet at the end.  Bound by HBM.
+//   attn_paged_tile_kernel : 128 rows a tile (prompt chunks, mixed batches).  The waves own 32 rows each and share K / V tiles of 64
+//                            keys, double-buffered.  Bound by the matrix pipes where the chunk is long.
+// Either cuts the key axis over blocks where there are too few tiles to fill the chip; attn_paged_merge_kernel joins the parts.
+// A bf16 step's rows go straight to LDS by DMA (16 keys lie within one page, so one page id serves a wave's piece); e4m3 codes pass through registers,
+// are turned into bf16 there (exact) and stored into the same image: one set of fragment reads serves both.
+#include <stdlib.h>
+
+#include "attn_frag.h"
+#include "common.h"
+#include "molly_hip.h"
+#include "paged.h"
+
+namespace {
+
+constexpr int TROWS = 128, RROWS = 32;               // rows of a tile in the two kernels
+constexpr int MIN_KEYS_ROWS = 256, MIN_KEYS_TILE = 512;      // fewest keys that a part of a cut key axis gets
+constexpr int MAX_PARTS = 64;
+
+struct AttnPagedArgs {
+    const bf16_t* q; bf16_t* out;
+    const char* kpool; const char* vpool; const uint8_t* kscale; const uint8_t* vscale;
+    const int* table; const int* cu_q; const int* kv_len;
+    float* part;                                     // [tile][kv head][parts]: ROWS * HD un-normalised outputs, ROWS * 2 (max, sum)
+    int n_tok, B, n_pages, page_shift, max_pages, ld_table, nh, nkv, G, ldq, ldo;
+    int tps;                                         // rows kernel: tiles per sequence; tile kernel: bound of the tiles of all of them
+    int parts;                                       // most parts of a tile's key axis
+    float scale_log2;                                // softmax scale * log2(e), > 0
+};
+
+// what a tile of query rows is: R0 .. R0 + rows - 1 of the n * G rows of its sequence
+struct Tile {
+    int b, tok0, n, row0, rows;                      // sequence, its first row in q, its new tokens, first packed row, packed rows
+    int first;                                       // key that row 0 of the sequence sees last (kv_len - n)
+    int n_vis;                                       // keys that the tile's last row sees (<= 0: none)
+};
+template <int ROWS>
+__device__ __forceinline__ Tile make_tile(const AttnPagedArgs& p, int b, int ti) {
+    Tile t;
+    t.b = b;
+    const int s = min(max(p.cu_q[b], 0), p.n_tok), e = min(max(p.cu_q[b + 1], s), p.n_tok);
+    t.tok0 = s; t.n = e - s;
+    t.row0 = ti * ROWS;
+    t.rows = min(ROWS, t.n * p.G - t.row0);
+    t.first = p.kv_len[b] - t.n;
+    t.n_vis = t.rows > 0 ? t.first + (t.row0 + t.rows - 1) / p.G + 1 : 0;
+    return t;
+}
+// parts that a tile's key axis is cut into, and a part's keys (whole steps of ALIGN)
+__device__ __forceinline__ int parts_of(int n_keys, int parts, int min_keys) { return min(parts, max(n_keys / min_keys, 1)); }
+template <int ALIGN> __device__ __forceinline__ int part_keys(int n_keys, int parts) { return ((n_keys + parts - 1) / parts + ALIGN - 1) / ALIGN * ALIGN; }
+
+// ---- K / V steps ------------------------------------------------------------------------------------------------------------------------
+struct KvSource {
+    const int* row;                                  // the sequence's page ids
+    int n_pages, shift, nkv, kvh;
+    // index (in keys of the pool) of the 16 keys that hold `key`, with the page id already loaded; a page that is none reads page 0 (the rows that see
+    // it are made NaN at the end)
+    __device__ __forceinline__ size_t group(int key, int page) const {
+        const unsigned pg = (unsigned)page < (unsigned)n_pages ? (unsigned)page : 0u;
+        return (((size_t)pg * nkv + kvh) << shift) + (key & ((1 << shift) - 1) & ~15);
+    }
+};
+
+// one 16-key group (rows 16 g .. of a tile image) by LDS-DMA: NPG pieces of 1 KiB per matrix.  `off`: the lane's byte offsets (group_offsets).
+template <int HD> constexpr int NPG = HD / 32;
+template <int HD> __device__ __forceinline__ void piece_row_col(int i, int lane, int& row, int& col) {
+    constexpr int NCB = HD / 16;
+    const int blk = lane >> 3, cin = lane & 7, rbl = i * (8 / NCB) + blk / NCB, b0 = rbl & 1, b1 = (rbl >> 1) & 1;
+    row = rbl * 4 + (cin >> 1);
+    col = (((blk % NCB) ^ b0) << 4) + (((cin & 1) ^ b1) << 3);
+}
+__device__ __forceinline__ void dma16(unsigned off, const char* base, unsigned lds) {
+    // (from asm, as in attention.hip: with the builtin hipcc waits for every pending LDS-DMA in front of the next transposed read)
+    asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(off), "s"(base), "s"(lds) : "memory", "m0");
+}
+template <int HD>
+__device__ __forceinline__ void dma_group(const char* base, unsigned lds, const unsigned (&off)[NPG<HD>]) {
+#pragma unroll
+    for (int i = 0; i < NPG<HD>; ++i) dma16(off[i], base, __builtin_amdgcn_readfirstlane(lds + i * 1024));
+}
+// the same for the group that the last key is in (or lies in front of): rows behind it repeat it, so that nothing behind a sequence's end — stale
+// pages may hold NaN — gets into the tile
+template <int HD>
+__device__ __forceinline__ void dma_group_clamped(const char* base, unsigned lds, int lim, int lane) {
+#pragma unroll
+    for (int i = 0; i < NPG<HD>; ++i) {
+        int row, col;
+        piece_row_col<HD>(i, lane, row, col);
+        dma16((unsigned)((min(row, lim) * HD + col) * 2), base, __builtin_amdgcn_readfirstlane(lds + i * 1024));
+    }
+}
+
+// one 16-key group of e4m3 codes through registers: NL loads of 16 codes a lane and matrix
+template <int HD> constexpr int NL = HD / 64;
+template <int HD> struct Codes {
+    u32x4 k[NL<HD>], v[NL<HD>];
+    uint8_t ke[NL<HD>], ve[NL<HD>];
+};
+template <int HD>
+__device__ __forceinline__ void codes_load(Codes<HD>& c, const AttnPagedArgs& p, size_t at, int lim, int lane) {
+    constexpr int NCB = HD / 16, LRB = NCB * 4;      // lanes of a 4-row block: 4 rows on the low lane bits (conflict-free LDS stores), 16 codes each
+#pragma unroll
+    for (int j = 0; j < NL<HD>; ++j) {
+        const int row = min((j * (64 / LRB) + lane / LRB) * 4 + (lane & 3), lim), cb = (lane >> 2) & (NCB - 1);
+        const size_t key = at + row;
+        c.k[j] = *reinterpret_cast<const u32x4*>(p.kpool + key * HD + cb * 16);
+        c.v[j] = *reinterpret_cast<const u32x4*>(p.vpool + key * HD + cb * 16);
+        c.ke[j] = p.kscale[key];
+        c.ve[j] = p.vscale[key];
+    }
+}
+template <int HD>
+__device__ __forceinline__ void codes_store(const Codes<HD>& c, bf16_t* imgk, bf16_t* imgv, int lane) {      // images of the group's 16 rows
+    constexpr int NCB = HD / 16, LRB = NCB * 4;
+#pragma unroll
+    for (int j = 0; j < NL<HD>; ++j) {
+        const int rbl = j * (64 / LRB) + lane / LRB, cb = (lane >> 2) & (NCB - 1), q = lane & 3, b0 = rbl & 1, b1 = (rbl >> 1) & 1;
+        const int o = (rbl * NCB + (cb ^ b0)) * 64 + q * 16;
+        const float ks = exp2i((int)c.ke[j] - 127), vs = exp2i((int)c.ve[j] - 127);
+        *reinterpret_cast<u32x4*>(imgk + o + b1 * 8) = e4m3_to_bf8(u32x2{c.k[j][0], c.k[j][1]}, ks);
+        *reinterpret_cast<u32x4*>(imgk + o + (b1 ^ 1) * 8) = e4m3_to_bf8(u32x2{c.k[j][2], c.k[j][3]}, ks);
+        *reinterpret_cast<u32x4*>(imgv + o + b1 * 8) = e4m3_to_bf8(u32x2{c.v[j][0], c.v[j][1]}, vs);
+        *reinterpret_cast<u32x4*>(imgv + o + (b1 ^ 1) * 8) = e4m3_to_bf8(u32x2{c.v[j][2], c.v[j][3]}, vs);
+    }
+}
+
+// ---- 32 query rows of a wave ---------------------------------------------------------------------------------------------------------------
+template <int HD> struct Rows {
+    bf16x8 qf[HD / 16];                              // B operand of S^T: lane (r, h) holds q[row r][16 s + 8 h .. +7]
+    f32x16 o[HD / 32];                               // O^T: lane = row, registers = columns
+    float m, l;                                      // running maximum (log2 domain, scaled) and this half-wave's part of the sum
+    int qi;                                          // last key the lane's row sees
+    int qmin, qmax;                                  // over the wave's rows (uniform)
+    bool odd;                                        // add_odd has something to do (uniform)
+};
+template <int HD>
+__device__ __forceinline__ void rows_init(Rows<HD>& st, const AttnPagedArgs& p, const Tile& t, int kvh, int wave_row, int lane) {
+    const int r = lane & 31, h = lane >> 5;
+    const int R = t.row0 + min(wave_row + r, t.rows - 1);          // (lanes behind the tile's last row repeat it)
+    const int tok = R / p.G, g = R - tok * p.G;
+    const bf16_t* qp = p.q + (size_t)(t.tok0 + tok) * p.ldq + (kvh * p.G + g) * HD + 8 * h;
+#pragma unroll
+    for (int s = 0; s < HD / 16; ++s) st.qf[s] = *reinterpret_cast<const bf16x8*>(qp + 16 * s);
+#pragma unroll
+    for (int d = 0; d < HD / 32; ++d)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) st.o[d][e] = 0.f;
+    st.m = -INFINITY; st.l = 0.f; st.odd = false;
+    st.qi = t.first + tok;
+    st.qmin = t.first + (t.row0 + min(wave_row, t.rows - 1)) / p.G;
+    st.qmax = t.first + (t.row0 + min(wave_row + 31, t.rows - 1)) / p.G;
+}
+
+// V values that are not finite, in a step that some row does not see all of: P is 0 there, and 0 * NaN would be NaN.  attend32 takes them out of such
+// a step (clear_odd) and this adds them to the rows that do see them, at the end.  step0, step0 + stride ..: the wave's steps below k1.
+template <int HD, bool FP8>
+__device__ __forceinline__ void add_odd(Rows<HD>& st, const AttnPagedArgs& p, const KvSource& src, int step0, int stride, int k1, int lane) {
+    const int h = lane >> 5;
+#pragma unroll 1
+    for (int kb = step0; kb < k1; kb += stride) {
+        if (kb + 31 <= st.qmin) continue;
+#pragma unroll 1
+        for (int key = kb; key < min(kb + 32, k1); ++key) {
+            const size_t at = src.group(key, src.row[key >> src.shift]) + (key & 15);
+            const float scale = FP8 ? exp2i((int)p.vscale[at] - 127) : 1.f;
+#pragma unroll
+            for (int d = 0; d < HD / 32; ++d)
+#pragma unroll
+                for (int g4 = 0; g4 < 4; ++g4) {
+                    const int col = 32 * d + 8 * g4 + 4 * h;
+                    u32x2 w;
+                    if constexpr (FP8) {
+                        const u32x4 x = e4m3_to_bf8(u32x2{*reinterpret_cast<const unsigned*>(p.vpool + at * HD + col), 0u}, scale);
+                        w = u32x2{x[0], x[1]};
+                    } else {
+                        w = *reinterpret_cast<const u32x2*>(p.vpool + (at * HD + col) * 2);
+                    }
+                    const float x[4] = {bflo(w[0]), bfhi(w[0]), bflo(w[1]), bfhi(w[1])};
+#pragma unroll
+                    for (int e = 0; e < 4; ++e)
+                        st.o[d][4 * g4 + e] += key <= st.qi && !(fabsf(x[e]) < INFINITY) ? x[e] : 0.f;
+                }
+        }
+    }
+}
+// values whose exponent field is all ones -> 0; true if there was one in any lane
+template <int ND>
+__device__ __forceinline__ bool clear_odd(bf16x8 (&vf)[2][ND]) {
+    typedef __attribute__((ext_vector_type(2))) unsigned short u16x2;
+    const u16x2 limit = {0x7f7f, 0x7f7f}, one = {1, 1};
+    u16x2 top = {0, 0};
+#pragma unroll
+    for (int sp = 0; sp < 2; ++sp)
+#pragma unroll
+        for (int d = 0; d < ND; ++d) {
+            const u32x4 w = __builtin_bit_cast(u32x4, vf[sp][d]);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const unsigned x = w[j] & 0x7f807f80u;
+                top = __builtin_elementwise_max(top, __builtin_bit_cast(u16x2, x));
+            }
+        }
+    if (!__any(top[0] == 0x7f80 || top[1] == 0x7f80)) return false;
+#pragma unroll
+    for (int sp = 0; sp < 2; ++sp)
+#pragma unroll
+        for (int d = 0; d < ND; ++d) {
+            u32x4 w = __builtin_bit_cast(u32x4, vf[sp][d]);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const unsigned x = w[j] & 0x7f807f80u;
+                const u16x2 odd = __builtin_elementwise_sub_sat(__builtin_bit_cast(u16x2, x), limit);       // 1: not finite
+                w[j] &= __builtin_bit_cast(unsigned, (u16x2)(odd - one));
+            }
+            vf[sp][d] = __builtin_bit_cast(bf16x8, w);
+        }
+    return true;
+}
+
+// one step of 32 keys: rows `sub` * 32 .. of the images, keys kbase ..
+template <int HD>
+__device__ __forceinline__ void attend32(Rows<HD>& st, const bf16_t* sK, const bf16_t* sV, int sub, int kbase, float scale_log2, int lane) {
+    constexpr int NS = HD / 16, ND = HD / 32;
+    const int r = lane & 31, h = lane >> 5;
+    bf16x8 kf[NS];
+#pragma unroll
+    for (int s = 0; s < NS; ++s) kf[s] = row_frag<HD>(sK, 32 * sub + r, s, h);
+    __builtin_amdgcn_sched_barrier(0);               // every read in flight before the first MFMA
+    f32x16 sc;
+#pragma unroll
+    for (int e = 0; e < 16; ++e) sc[e] = 0.f;
+#pragma unroll
+    for (int s = 0; s < NS; ++s) sc = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kf[s], st.qf[s], sc, 0, 0, 0);
+    bf16x8 vf[2][ND];
+#pragma unroll
+    for (int sp = 0; sp < 2; ++sp)
+#pragma unroll
+        for (int d = 0; d < ND; ++d) vf[sp][d] = tr_frag<HD>(sV, 32 * sub, sp, d, lane);
+    const bool edge = kbase + 31 > st.qmin;          // (uniform) some row does not see all of the step
+    float mx = -INFINITY;
+    if (edge) {
+#pragma unroll
+        for (int e = 0; e < 16; ++e) {
+            const int key = kbase + (e & 3) + 8 * (e >> 2) + 4 * h;
+            sc[e] = key <= st.qi ? sc[e] : -INFINITY;
+        }
+    }
+#pragma unroll
+    for (int e = 0; e < 16; ++e) mx = fmaxf(mx, sc[e]);
+    mx = xhalf_max(mx) * scale_log2;
+    if (!__all(mx - st.m <= RESCALE_THR)) {          // the reference maximum follows only where it has grown by more than 2^8
+        const float m_new = fmaxf(st.m, mx);
+        const float alpha = fast_exp2(st.m - (m_new == -INFINITY ? 0.f : m_new));
+        st.l *= alpha;
+        st.m = m_new;
+#pragma unroll
+        for (int d = 0; d < ND; ++d)
+#pragma unroll
+            for (int e = 0; e < 16; ++e) st.o[d][e] *= alpha;
+    }
+    const float m_ref = st.m == -INFINITY ? 0.f : st.m;
+#pragma unroll
+    for (int e = 0; e < 16; ++e) sc[e] = fast_exp2(sc[e] * scale_log2 - m_ref);
+    float rs[4];
+#pragma unroll
+    for (int g = 0; g < 4; ++g) rs[g] = (sc[4 * g] + sc[4 * g + 1]) + (sc[4 * g + 2] + sc[4 * g + 3]);
+    st.l += (rs[0] + rs[1]) + (rs[2] + rs[3]);
+    const bf16x8 pf[2] = {acc_to_frag(sc, 0), acc_to_frag(sc, 8)};
+    if (edge && clear_odd<ND>(vf)) st.odd = true;
+#pragma unroll
+    for (int d = 0; d < ND; ++d) {
+        st.o[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vf[0][d], pf[0], st.o[d], 0, 0, 0);
+        st.o[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vf[1][d], pf[1], st.o[d], 0, 0, 0);
+    }
+}
+
+// the first of the keys k0 .. k1 - 1 that lies on a page that is none, by all threads of the block (0x7fffffff: all pages are); *sh is set
+// behind the next barrier
+__device__ __forceinline__ void scan_pages(const AttnPagedArgs& p, const int* row, int k0, int k1, int* sh) {
+    const int last = k1 > k0 ? (k1 - 1) >> p.page_shift : -1;
+    for (int i = (k0 >> p.page_shift) + threadIdx.x; i <= last; i += 256)
+        if ((unsigned)row[i] >= (unsigned)p.n_pages) atomicMin(sh, i << p.page_shift);
+}
+
+// ---- short chunks: one tile of up to 32 rows a block, its waves take every fourth step --------------------------------------------------------
+template <int HD, bool FP8>
+__global__ __launch_bounds__(256, (HD == 128 && !FP8) ? 1 : 2) void attn_paged_rows_kernel(AttnPagedArgs p) {
+    extern __shared__ __attribute__((aligned(16))) char smem[];
+    __shared__ int s_bad;
+    __shared__ float s_ml[4][RROWS][2];
+    constexpr int IMG = 32 * HD;                     // elements of a step's K (or V) image
+    constexpr int NBUF = FP8 ? 1 : 2;
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    int bid = blockIdx.x;
+    const int s = bid % p.parts; bid /= p.parts;
+    const int kvh = bid % p.nkv; bid /= p.nkv;
+    const int b = bid / p.tps;
+    bf16_t* img = reinterpret_cast<bf16_t*>(smem) + wave * NBUF * 2 * IMG;            // [buffer][K | V]
+    const unsigned img_lds = __builtin_amdgcn_readfirstlane((unsigned)(uintptr_t)LDS_PTR(img));
+    unsigned off[NPG<HD>];
+#pragma unroll
+    for (int i = 0; i < NPG<HD>; ++i) {
+        int row, col;
+        piece_row_col<HD>(i, lane, row, col);
+        off[i] = (unsigned)((row * HD + col) * 2);
+    }
+    for (int ti = bid % p.tps;; ti += p.tps) {       // (a sequence has more tiles than p.tps only where the caller's max_q was too small)
+        const Tile t = make_tile<RROWS>(p, b, ti);
+        if (t.rows <= 0) return;
+        const int kmax = p.max_pages << p.page_shift;
+        const int n_keys = min(t.n_vis, kmax);
+        const int parts = ti < p.tps ? parts_of(n_keys, p.parts, MIN_KEYS_ROWS) : 1;
+        if (s >= parts) continue;
+        const int chunk = part_keys<128>(n_keys, parts);
+        const int k0 = s * chunk, k1 = min(n_keys, k0 + chunk), last = k1 - 1;
+        const KvSource src{p.table + (size_t)b * p.ld_table, p.n_pages, p.page_shift, p.nkv, kvh};
+        if (tid == 0) s_bad = t.n_vis > kmax ? kmax : 0x7fffffff;
+        Rows<HD> st;
+        rows_init<HD>(st, p, t, kvh, 0, lane);
+        const int key0 = k0 + 32 * wave;
+        // page ids of the wave's next 32 steps, two groups each: lane 2 i + g.  Waited for here, once in 4,096 keys: a wait inside the steps would be a wait
+        // for the DMA in flight.
+        int pages = 0;
+        auto look = [&](int key) {
+            const int i = (key - key0) >> 7;
+            if ((i & 31) == 0) {
+                pages = src.row[min(key + (lane >> 1) * 128 + (lane & 1) * 16, last) >> p.page_shift];
+                arrived(pages);
+            }
+            return i & 31;
+        };
+        auto dma_step = [&](int key, int buf) {
+            const int i = look(key);
+#pragma unroll
+            for (int g = 0; g < 2; ++g) {
+                const int kb = key + 16 * g, kc = min(kb, last & ~15);
+                const size_t at = src.group(kc, __builtin_amdgcn_readlane(pages, 2 * i + g)) * (HD * 2);
+                const unsigned dst = img_lds + (buf * 2 * IMG + g * 16 * HD) * 2;
+                if (kb + 15 <= last) {
+                    dma_group<HD>(p.kpool + at, dst, off);
+                    dma_group<HD>(p.vpool + at, dst + IMG * 2, off);
+                } else {
+                    const int lim = kb > last ? 0 : last - kc;              // (a group behind the last key: 16 copies of a key that is there)
+                    dma_group_clamped<HD>(p.kpool + at, dst, lim, lane);
+                    dma_group_clamped<HD>(p.vpool + at, dst + IMG * 2, lim, lane);
+                }
+            }
+        };
+        if constexpr (FP8) {
+            Codes<HD> c[2];
+            auto load_step = [&](int key) {
+                const int i = look(key);
+#pragma unroll
+                for (int g = 0; g < 2; ++g) {
+                    const int kb = key + 16 * g, kc = min(kb, last & ~15);
+                    codes_load<HD>(c[g], p, src.group(kc, __builtin_amdgcn_readlane(pages, 2 * i + g)), kb > last ? 0 : min(last - kc, 15), lane);
+                }
+            };
+            if (key0 < k1) load_step(key0);
+#pragma unroll 1
+            for (int key = key0; key < k1; key += 128) {
+#pragma unroll
+                for (int g = 0; g < 2; ++g) codes_store<HD>(c[g], img + g * 16 * HD, img + IMG + g * 16 * HD, lane);
+                if (key + 128 < k1) load_step(key + 128);
+                attend32<HD>(st, img, img + IMG, 0, key, p.scale_log2, lane);
+            }
+        } else {
+            int buf = 0;
+#pragma unroll
+            for (int i = 0; i < HD / 16; ++i) arrived(st.qf[i]);
+            if (key0 < k1) dma_step(key0, 0);
+#pragma unroll 1
+            for (int key = key0; key < k1; key += 128) {
+                if (key + 128 < k1) {
+                    dma_step(key + 128, buf ^ 1);
+                    // this step's pieces have landed when only the next one's are still out
+                    if (HD == 128) asm volatile("s_waitcnt vmcnt(16)" ::: "memory");
+                    else asm volatile("s_waitcnt vmcnt(8)" ::: "memory");
+                } else {
+                    dma_wait();
+                }
+                attend32<HD>(st, img + buf * 2 * IMG, img + buf * 2 * IMG + IMG, 0, key, p.scale_log2, lane);
+                buf ^= 1;
+            }
+        }
+        if (st.odd) add_odd<HD, FP8>(st, p, src, k0 + 32 * wave, 128, k1, lane);
+        __syncthreads();                             // the images are dead; s_bad is set
+        scan_pages(p, src.row, k0, k1, &s_bad);
+        // the four waves' rows, un-normalised, through LDS
+        const int r = lane & 31, h = lane >> 5;
+        const float l = st.l + __shfl_xor(st.l, 32, 64);
+        if (h == 0) { s_ml[wave][r][0] = st.m; s_ml[wave][r][1] = l; }
+        float* acc = reinterpret_cast<float*>(smem) + (size_t)wave * RROWS * HD;
+        if (r < t.rows)
+#pragma unroll
+            for (int d = 0; d < HD / 32; ++d)
+#pragma unroll
+                for (int g4 = 0; g4 < 4; ++g4)
+                    *reinterpret_cast<f32x4*>(acc + r * HD + 32 * d + 8 * g4 + 4 * h) =
+                        f32x4{st.o[d][4 * g4], st.o[d][4 * g4 + 1], st.o[d][4 * g4 + 2], st.o[d][4 * g4 + 3]};
+        __syncthreads();
+        const int bad = s_bad;
+        float* part = parts > 1 ? p.part + ((size_t)((b * p.tps + ti) * p.nkv + kvh) * p.parts + s) * (RROWS * (HD + 2)) : nullptr;
+        for (int i = tid; i < t.rows * (HD / 4); i += 256) {
+            const int row = i / (HD / 4), c4 = (i % (HD / 4)) * 4;
+            float m = -INFINITY;
+#pragma unroll
+            for (int w = 0; w < 4; ++w) m = fmaxf(m, s_ml[w][row][0]);
+            const float mu = m == -INFINITY ? 0.f : m;
+            f32x4 a = {0.f, 0.f, 0.f, 0.f};
+            float ls = 0.f;
+#pragma unroll
+            for (int w = 0; w < 4; ++w) {
+                const float f = fast_exp2(s_ml[w][row][0] - mu);
+                const f32x4 x = *reinterpret_cast<const f32x4*>(reinterpret_cast<const float*>(smem) + ((size_t)w * RROWS + row) * HD + c4);
+                ls += s_ml[w][row][1] * f;
+#pragma unroll
+                for (int e = 0; e < 4; ++e) a[e] += f == 0.f ? 0.f : x[e] * f;            // (a wave without keys has zeros: never 0 * inf)
+            }
+            const int R = t.row0 + row, tok = R / p.G;
+            if (t.first + tok >= bad) ls = __builtin_nanf("");
+            if (part) {
+                *reinterpret_cast<f32x4*>(part + row * HD + c4) = a;
+                if (c4 == 0) { part[RROWS * HD + row * 2] = m; part[RROWS * HD + row * 2 + 1] = ls; }
+            } else {
+                const float inv = ls == 0.f ? 0.f : 1.f / ls;
+                bf16_t* d = p.out + (size_t)(t.tok0 + tok) * p.ldo + (kvh * p.G + R - tok * p.G) * HD + c4;
+                *reinterpret_cast<u32x2*>(d) = u32x2{pack_bf2(a[0] * inv, a[1] * inv), pack_bf2(a[2] * inv, a[3] * inv)};
+            }
+        }
+        __syncthreads();                             // (the next tile's images and s_bad)
+    }
+}
+
+// ---- long chunks: 128 rows a block -----------------------------------------------------------------------------------------------------------
+// tile f of the sequences' tiles in reverse order (within a sequence the longest causal range first); -1: there are fewer
+__device__ __forceinline__ int find_tile(const AttnPagedArgs& p, int f, int lane, int* ti) {
+    auto tiles = [&](int b) {
+        if (b >= p.B) return 0;
+        const int s = min(max(p.cu_q[b], 0), p.n_tok), e = min(max(p.cu_q[b + 1], s), p.n_tok);
+        return ((e - s) * p.G + TROWS - 1) / TROWS;
+    };
+    int total = 0;
+    for (int b0 = 0; b0 < p.B; b0 += 64) total += (int)wave_sum((float)tiles(b0 + lane));      // (exact: below 2^24 tiles, checked by the host)
+    f = total - 1 - f;
+    if (f < 0) return -1;
+    for (int b0 = 0, base = 0; b0 < p.B; b0 += 64) {
+        const int n = tiles(b0 + lane);
+        int inc = n;
+#pragma unroll
+        for (int o = 1; o < 64; o <<= 1) {
+            const int x = __shfl_up(inc, o, 64);
+            inc += lane >= o ? x : 0;
+        }
+        const unsigned long long hit = __ballot(base + inc > f);
+        if (hit) {
+            const int who = __ffsll((long long)hit) - 1;
+            *ti = f - base - (__builtin_amdgcn_readlane(inc, who) - __builtin_amdgcn_readlane(n, who));
+            return b0 + who;
+        }
+        base += __builtin_amdgcn_readlane(inc, 63);
+    }
+    return -1;
+}
+
+template <int HD, bool FP8>
+__global__ __launch_bounds__(256, 2) void attn_paged_tile_kernel(AttnPagedArgs p) {
+    extern __shared__ __attribute__((aligned(16))) char smem_raw[];
+    __shared__ int s_bad;
+    bf16_t* smem = reinterpret_cast<bf16_t*>(smem_raw);            // [2 stages][K tile | V tile]
+    constexpr int TILE = 64 * HD;
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    // the workgroups of one XCD (every eighth) take a contiguous run of the order (kv head, part, tile): they share a head's keys in its L2
+    const int q8 = gridDim.x >> 3, r8 = gridDim.x & 7, xcd = blockIdx.x & 7;
+    int v = (xcd < r8 ? xcd * (q8 + 1) : r8 * (q8 + 1) + (xcd - r8) * q8) + (blockIdx.x >> 3);
+    const int f = v % p.tps; v /= p.tps;
+    const int s = v % p.parts, kvh = v / p.parts;
+    int ti = 0;
+    const int b = __builtin_amdgcn_readfirstlane(find_tile(p, f, lane, &ti));
+    if (b < 0) return;
+    ti = __builtin_amdgcn_readfirstlane(ti);
+    const Tile t = make_tile<TROWS>(p, b, ti);
+    const int kmax = p.max_pages << p.page_shift;
+    const int n_keys = min(t.n_vis, kmax);
+    const int parts = parts_of(n_keys, p.parts, MIN_KEYS_TILE);
+    if (s >= parts) return;
+    const int chunk = part_keys<64>(n_keys, parts);
+    const int k0 = s * chunk, k1 = min(n_keys, k0 + chunk), last = k1 - 1;
+    const KvSource src{p.table + (size_t)b * p.ld_table, p.n_pages, p.page_shift, p.nkv, kvh};
+    if (tid == 0) s_bad = t.n_vis > kmax ? kmax : 0x7fffffff;
+    const bool active = wave * 32 < t.rows;
+    Rows<HD> st;
+    rows_init<HD>(st, p, t, kvh, wave * 32, lane);
+#pragma unroll
+    for (int i = 0; i < HD / 16; ++i) arrived(st.qf[i]);
+    unsigned off[NPG<HD>];
+#pragma unroll
+    for (int i = 0; i < NPG<HD>; ++i) {
+        int row, col;
+        piece_row_col<HD>(i, lane, row, col);
+        off[i] = (unsigned)((row * HD + col) * 2);
+    }
+    const unsigned smem_lds = __builtin_amdgcn_readfirstlane((unsigned)(uintptr_t)LDS_PTR(smem));
+    int pages = 0;                                   // page ids of this wave's 16 keys of the next 64 tiles (waited for once in 4,096 keys)
+    Codes<HD> c;
+    auto issue = [&](int k, int stg) {               // keys k .. k + 63; this wave's are k + 16 * wave ..
+        const int i = ((k - k0) >> 6) & 63;
+        if (i == 0) {
+            pages = src.row[min(k + 64 * lane + 16 * wave, last) >> p.page_shift];
+            arrived(pages);
+        }
+        const int kb = k + 16 * wave, kc = min(kb, last & ~15);
+        const size_t at = src.group(kc, __builtin_amdgcn_readlane(pages, i));
+        if constexpr (FP8) {
+            codes_load<HD>(c, p, at, kb > last ? 0 : min(last - kc, 15), lane);
+        } else {
+            const unsigned dst = smem_lds + (stg * 2 * TILE + wave * 16 * HD) * 2;
+            if (kb + 15 <= last) {
+                dma_group<HD>(p.kpool + at * (HD * 2), dst, off);
+                dma_group<HD>(p.vpool + at * (HD * 2), dst + TILE * 2, off);
+            } else {
+                const int lim = kb > last ? 0 : last - kc;
+                dma_group_clamped<HD>(p.kpool + at * (HD * 2), dst, lim, lane);
+                dma_group_clamped<HD>(p.vpool + at * (HD * 2), dst + TILE * 2, lim, lane);
+            }
+        }
+    };
+    auto land = [&](int stg) {
+        if constexpr (FP8) codes_store<HD>(c, smem + stg * 2 * TILE + wave * 16 * HD, smem + stg * 2 * TILE + TILE + wave * 16 * HD, lane);
+        else dma_wait();
+    };
+    if (k0 < k1) {
+        issue(k0, 0);
+        land(0);
+    }
+    __syncthreads();
+    scan_pages(p, src.row, k0, k1, &s_bad);
+    int cur = 0;
+#pragma unroll 1
+    for (int k = k0; k < k1; k += 64) {
+        const bf16_t* sK = smem + cur * 2 * TILE;
+        if (k + 64 < k1) issue(k + 64, cur ^ 1);
+        if (active) {
+#pragma unroll
+            for (int sub = 0; sub < 2; ++sub)
+                if (k + 32 * sub <= st.qmax) attend32<HD>(st, sK, sK + TILE, sub, k + 32 * sub, p.scale_log2, lane);
+        }
+        if (k + 64 < k1) land(cur ^ 1);
+        __syncthreads();
+        cur ^= 1;
+    }
+    if (k0 >= k1) __syncthreads();                   // (s_bad)
+    // ---- epilogue: this wave's 32 rows
+    if (!active) return;
+    if (st.odd) add_odd<HD, FP8>(st, p, src, k0, 32, min(k1, st.qmax + 1), lane);
+    const int r = lane & 31, h = lane >> 5;
+    float l = st.l + __shfl_xor(st.l, 32, 64);
+    if (st.qi >= s_bad) l = __builtin_nanf("");
+    const int rows = min(32, t.rows - wave * 32);
+    if (parts > 1) {
+        float* part = p.part + ((size_t)(f * p.nkv + kvh) * p.parts + s) * (TROWS * (HD + 2));
+        if (r < rows) {
+            float* d = part + (size_t)(wave * 32 + r) * HD;
+#pragma unroll
+            for (int dd = 0; dd < HD / 32; ++dd)
+#pragma unroll
+                for (int g4 = 0; g4 < 4; ++g4)
+                    *reinterpret_cast<f32x4*>(d + 32 * dd + 8 * g4 + 4 * h) =
+                        f32x4{st.o[dd][4 * g4], st.o[dd][4 * g4 + 1], st.o[dd][4 * g4 + 2], st.o[dd][4 * g4 + 3]};
+            if (h == 0) { part[TROWS * HD + (wave * 32 + r) * 2] = st.m; part[TROWS * HD + (wave * 32 + r) * 2 + 1] = l; }
+        }
+        return;
+    }
+    const float inv = l == 0.f ? 0.f : 1.f / l;
+    // rows through a slab of the wave's own in the dead stages: whole rows leave, 16 bytes a lane
+    constexpr int PITCH = HD + 8, LPR = HD / 8, RPI = 64 / LPR;
+    bf16_t* slab = smem + wave * 32 * PITCH;
+#pragma unroll
+    for (int d = 0; d < HD / 32; ++d)
+#pragma unroll
+        for (int g4 = 0; g4 < 4; ++g4)
+            *reinterpret_cast<u32x2*>(slab + r * PITCH + 32 * d + 8 * g4 + 4 * h) =
+                u32x2{pack_bf2(st.o[d][4 * g4] * inv, st.o[d][4 * g4 + 1] * inv), pack_bf2(st.o[d][4 * g4 + 2] * inv, st.o[d][4 * g4 + 3] * inv)};
+    const int lr = lane / LPR, lc = (lane % LPR) * 8;
+#pragma unroll
+    for (int it = 0; it < 32 / RPI; ++it) {
+        const int row = it * RPI + lr;
+        const u32x4 x = *reinterpret_cast<const u32x4*>(slab + row * PITCH + lc);
+        const int R = t.row0 + wave * 32 + row, tok = R / p.G;
+        if (row < rows) *reinterpret_cast<u32x4*>(p.out + (size_t)(t.tok0 + tok) * p.ldo + (kvh * p.G + R - tok * p.G) * HD + lc) = x;
+    }
+}
+
+// ---- the parts of a tile's rows: out = sum_s 2^(m_s - m) o_s / sum_s 2^(m_s - m) l_s; one wave a row
+template <int HD, bool TILEK>
+__global__ __launch_bounds__(256) void attn_paged_merge_kernel(AttnPagedArgs p) {
+    constexpr int ROWS = TILEK ? TROWS : RROWS, C = HD / 64;
+    const int lane = threadIdx.x & 63, row = blockIdx.y * 4 + (threadIdx.x >> 6);
+    const int tile = blockIdx.x / p.nkv, kvh = blockIdx.x % p.nkv;
+    int b, ti = 0;
+    if (TILEK) b = find_tile(p, tile, lane, &ti);
+    else { b = tile / p.tps; ti = tile % p.tps; }
+    if (b < 0) return;
+    const Tile t = make_tile<ROWS>(p, b, ti);
+    if (row >= t.rows) return;
+    const int parts = parts_of(min(t.n_vis, p.max_pages << p.page_shift), p.parts, TILEK ? MIN_KEYS_TILE : MIN_KEYS_ROWS);
+    if (parts == 1) return;                          // written by the attention itself
+    const float* base = p.part + (size_t)(tile * p.nkv + kvh) * p.parts * (ROWS * (HD + 2));
+    float m = -INFINITY;
+    for (int s = 0; s < parts; ++s) m = fmaxf(m, base[(size_t)s * (ROWS * (HD + 2)) + ROWS * HD + row * 2]);
+    const float mu = m == -INFINITY ? 0.f : m;
+    float l = 0.f, a[C];
+#pragma unroll
+    for (int c = 0; c < C; ++c) a[c] = 0.f;
+    for (int s = 0; s < parts; ++s) {
+        const float* ps = base + (size_t)s * (ROWS * (HD + 2));
+        const float f = fast_exp2(ps[ROWS * HD + row * 2] - mu);
+        l += ps[ROWS * HD + row * 2 + 1] * f;
+#pragma unroll
+        for (int c = 0; c < C; ++c) a[c] += f == 0.f ? 0.f : ps[row * HD + lane * C + c] * f;
+    }
+    const float inv = l == 0.f ? 0.f : 1.f / l;
+    const int R = t.row0 + row, tok = R / p.G;
+    bf16_t* d = p.out + (size_t)(t.tok0 + tok) * p.ldo + (kvh * p.G + R - tok * p.G) * HD + lane * C;
+    if (C == 2) *reinterpret_cast<unsigned*>(d) = pack_bf2(a[0] * inv, a[C - 1] * inv);
+    else d[0] = f2bf(a[0] * inv);
+}
+
+// ---- host: which kernel, and how many parts
+struct Shape { bool tile; int tps, parts; long part_floats; };
+Shape pick_shape(int n_tok, int B, int nkv, int G, int HD, bool fp8, long max_keys, int max_q, int max_kv) {
+    Shape sh{};
+    const long mq = max_q > 0 && max_q < n_tok ? max_q : n_tok;
+    const long keys = max_kv > 0 && max_kv < max_keys ? max_kv : max_keys;
+    sh.tile = mq * G > RROWS;
+    const int rows = sh.tile ? TROWS : RROWS;
+    const long tps = sh.tile ? (long)n_tok * G / TROWS + B : (mq * G + RROWS - 1) / RROWS;
+    sh.tps = (int)tps;
+    const long units = (sh.tile ? tps : tps * B) * nkv;
+    // resident blocks: 2 a CU, 1 for the rows kernel with 128 KB of images
+    const long want = sh.tile ? 512 : (HD == 128 && !fp8 ? 512 : 1024);
+    long parts = want / (units > 0 ? units : 1);
+    const long most = keys / (sh.tile ? MIN_KEYS_TILE : MIN_KEYS_ROWS);
+    if (parts > most) parts = most;
+    if (parts > MAX_PARTS) parts = MAX_PARTS;
+    sh.parts = parts < 1 ? 1 : (int)parts;
+    sh.part_floats = sh.parts > 1 ? units * sh.parts * rows * (HD + 2) : 0;
+    return sh;
+}
+
+template <int HD, bool FP8>
+void launch(hipStream_t st, const AttnPagedArgs& p, const Shape& sh) {
+    if (sh.tile) {
+        const size_t lds = 2 * 2 * 64 * HD * 2;
+        static const hipError_t once = hipFuncSetAttribute((const void*)attn_paged_tile_kernel<HD, FP8>, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
+        (void)once;
+        hipLaunchKernelGGL((attn_paged_tile_kernel<HD, FP8>), dim3(sh.tps * p.nkv * sh.parts), dim3(256), lds, st, p);
+        if (sh.parts > 1) hipLaunchKernelGGL((attn_paged_merge_kernel<HD, true>), dim3(sh.tps * p.nkv, TROWS / 4), dim3(256), 0, st, p);
+    } else {
+        const size_t lds = 4 * RROWS * HD * 4 * (FP8 ? 1 : 2);        // images (e4m3: one buffer of 32 rows K | V in bf16), at the end the four waves' rows in fp32
+        static const hipError_t once = hipFuncSetAttribute((const void*)attn_paged_rows_kernel<HD, FP8>, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
+        (void)once;
+        hipLaunchKernelGGL((attn_paged_rows_kernel<HD, FP8>), dim3(p.B * sh.tps * p.nkv * sh.parts), dim3(256), lds, st, p);
+        if (sh.parts > 1) hipLaunchKernelGGL((attn_paged_merge_kernel<HD, false>), dim3(p.B * sh.tps * p.nkv, RROWS / 4), dim3(256), 0, st, p);
+    }
+}
+
+int check_sizes(int n_tokens, int B, int n_heads, int n_kv_heads, int max_pages, int page_size) {
+    MOLLY_CHECK(n_tokens >= 0 && B >= 0 && max_pages >= 0, "attn_paged: n_tokens=%d B=%d max_pages=%d", n_tokens, B, max_pages);
+    MOLLY_CHECK(n_heads > 0 && n_kv_heads > 0 && n_heads % n_kv_heads == 0, "attn_paged: n_heads=%d not a multiple of n_kv_heads=%d", n_heads, n_kv_heads);
+    MOLLY_CHECK((long)max_pages * page_size <= 0x7ffffe00L, "attn_paged: %d pages of %d keys a sequence: keys are 32-bit", max_pages, page_size);
+    MOLLY_CHECK((long)n_tokens * n_heads / n_kv_heads <= 0x1fffffffL && ((long)n_tokens * n_heads / 32 + 2L * B * n_kv_heads) * MAX_PARTS <= 0x7fffffffL,
+                "attn_paged: n_tokens=%d x n_heads=%d, B=%d: more tiles than one call takes", n_tokens, n_heads, B);
+    return 0;
+}
+
+}  // namespace
+
+extern "C" int molly_attn_paged_workspace(int n_tokens, int B, int n_heads, int n_kv_heads, int head_dim, int page_size, int max_pages, int e4m3,
+                                          int max_q, int max_kv) {
+    if (n_tokens <= 0 || B <= 0 || page_size <= 0 || check_sizes(n_tokens, B, n_heads, n_kv_heads, max_pages, page_size)) return 0;
+    const Shape sh = pick_shape(n_tokens, B, n_kv_heads, n_heads / n_kv_heads, head_dim, e4m3 != 0, (long)max_pages * page_size, max_q, max_kv);
+    return sh.part_floats <= 0x7fffffffL ? (int)sh.part_floats : 0;
+}
+
+extern "C" int molly_attn_paged(void* stream, const void* q, void* out, const void* kpool, const void* vpool, const void* kscale_or_null,
+                                const void* vscale_or_null, const int* block_table, const int* cu_q, const int* kv_len, int n_tokens, int B,
+                                int n_pages, int page_size, int max_pages, int ld_table, int n_heads, int n_kv_heads, int head_dim, int ldq,
+                                int ldo, float scale, int max_q, int max_kv, float* workspace, long workspace_floats) {
+    MOLLY_ENTER();
+    if (int rc = check_pool("attn_paged", kpool, vpool, kscale_or_null, vscale_or_null, n_pages, page_size, n_kv_heads, head_dim)) return rc;
+    if (int rc = check_sizes(n_tokens, B, n_heads, n_kv_heads, max_pages, page_size)) return rc;
+    MOLLY_CHECK(ld_table >= max_pages, "attn_paged: ld_table=%d for max_pages=%d", ld_table, max_pages);
+    MOLLY_CHECK(scale > 0.f && scale < INFINITY, "attn_paged: scale=%g must be positive", (double)scale);
+    if (n_tokens == 0 || B == 0) return 0;
+    MOLLY_CHECK(q && out && cu_q && kv_len && (block_table || max_pages == 0), "attn_paged: q, out, block_table, cu_q, kv_len required");
+    MOLLY_CHECK(aligned16(q) && aligned16(out) && ldq % 8 == 0 && ldo % 8 == 0 && ldq >= n_heads * head_dim && ldo >= n_heads * head_dim,
+                "attn_paged: q / out rows must be 16-byte aligned and hold n_heads * head_dim values (ldq=%d ldo=%d)", ldq, ldo);
+    MOLLY_CHECK(aligned16(workspace), "attn_paged: the workspace must be 16-byte aligned");
+    AttnPagedArgs p{};
+    p.q = (const bf16_t*)q; p.out = (bf16_t*)out; p.kpool = (const char*)kpool; p.vpool = (const char*)vpool;
+    p.kscale = (const uint8_t*)kscale_or_null; p.vscale = (const uint8_t*)vscale_or_null;
+    p.table = block_table; p.cu_q = cu_q; p.kv_len = kv_len; p.n_tok = n_tokens; p.B = B;
+    p.n_pages = n_pages; p.page_shift = log2_exact(page_size); p.max_pages = max_pages; p.ld_table = ld_table;
+    p.nh = n_heads; p.nkv = n_kv_heads; p.G = n_heads / n_kv_heads; p.ldq = ldq; p.ldo = ldo; p.scale_log2 = scale * LOG2E;
+    Shape sh = pick_shape(n_tokens, B, n_kv_heads, p.G, head_dim, kscale_or_null != nullptr, (long)max_pages * page_size, max_q, max_kv);
+    if (sh.parts > 1 && (!workspace || workspace_floats < sh.part_floats)) sh.parts = 1;
+    p.part = workspace; p.tps = sh.tps; p.parts = sh.parts;
+    hipStream_t st = (hipStream_t)stream;
+    if (head_dim == 128) {
+        if (kscale_or_null) launch<128, true>(st, p, sh);
+        else launch<128, false>(st, p, sh);
+    } else {
+        if (kscale_or_null) launch<64, true>(st, p, sh);
+        else launch<64, false>(st, p, sh);
+    }
+    MOLLY_LAUNCH_CHECK();
+    return 0;
+}

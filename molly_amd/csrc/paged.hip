@@ -1,23 +1,11 @@
-// The paged key / value cache of `generate` and the attention that reads it.
+// Rows into the paged key / value cache and back (the layout and the e4m3 form: paged.h).
 //   molly_paged_kv_append : rows of k and v (and q) -> q/k-norm, rotary -> the pages of the cache, bf16 or e4m3
 //   molly_paged_kv_read   : the rows of a list of places, back as bf16
-//   molly_attn_paged      : ragged chunks of new tokens attend causally to everything their sequence has in the pages
-// The reference's `generate` keeps HF's DynamicCache (reference src/model/omics_one.py:220-232), one dense tensor a layer that is
-// concatenated to at every step; here a layer's cache is a pool of pages [n_pages][n_kv_heads][page_size][head_dim], and a sequence is a
-// row of page ids.  Head-major: the keys of one (page, head) are contiguous, so what one workgroup of the attention reads are
-// whole lines, page_size * head_dim values at a time.
-//
-// e4m3 pools: a head of a token is held as codes and ONE exponent byte e: value = code * 2^(e - 127).  e is the smallest power of two that
-// brings the head's largest magnitude to 448 (the format's largest value) or less.  With a power of two the division and the product
-// are exact: the only rounding is the code's own (round to nearest even, half a step: 2^-4 of the value), the value read back is
-// a bf16 without rounding, and one conversion instruction (v_cvt_scalef32_pk_bf16_fp8) makes two of them.  What a
-// free scale would gain is nothing above the format's subnormals: a code keeps its 4 significant bits wherever it sits in the 15 octaves.
 #include "common.h"
 #include "molly_hip.h"
+#include "paged.h"
 
 namespace {
-
-__device__ __forceinline__ float exp2i(int e) { return __builtin_bit_cast(float, (unsigned)(e + 127) << 23); }      // 2^e, -126 <= e <= 127
 
 // the exponent byte of a head whose largest finite magnitude is amax (448 = 1.75 * 2^8)
 __device__ __forceinline__ int e4m3_exponent(float amax) {
@@ -34,16 +22,6 @@ __device__ __forceinline__ unsigned e4m3_pack4(const float* x, float inv) {
     w = __builtin_amdgcn_cvt_pk_fp8_f32(y[2], y[3], w, true);
     return (unsigned)w;
 }
-// eight codes -> eight bf16, times the power of two `scale`
-__device__ __forceinline__ u32x4 e4m3_to_bf8(u32x2 c, float scale) {
-    u32x4 r;
-    r[0] = __builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(c[0], scale, false));
-    r[1] = __builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(c[0], scale, true));
-    r[2] = __builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(c[1], scale, false));
-    r[3] = __builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(c[1], scale, true));
-    return r;
-}
-
 struct AppendArgs {
     const bf16_t* q; const bf16_t* k; const bf16_t* v; bf16_t* q_out;
     void* kpool; void* vpool; uint8_t* kscale; uint8_t* vscale;
@@ -175,89 +153,6 @@ __global__ __launch_bounds__(256) void paged_read_kernel(ReadArgs p) {
     d[0] = a; d[1] = b;
 }
 
-struct AttnPagedArgs {
-    const bf16_t* q; bf16_t* out;
-    const void* kpool; const void* vpool; const uint8_t* kscale; const uint8_t* vscale;
-    const int* table; const int* cu_q; const int* kv_len;
-    int n_tok, B, n_pages, page_shift, max_pages, ld_table, nh, nkv, ldq, ldo;
-    float qscale;                                    // softmax scale * log2(e)
-};
-
-// the sequence of row `t`: the last b with cu_q[b] <= t (B when t lies behind the last one)
-__device__ __forceinline__ int find_seq(const int* cu, int B, int t) {
-    int lo = 0, hi = B;                              // cu[lo] <= t < cu[hi + 1] ..
-    while (lo < hi) {
-        const int mid = (lo + hi) >> 1;
-        if (cu[mid + 1] <= t) lo = mid + 1; else hi = mid;
-    }
-    return lo;
-}
-
-// one value of a pool
-template <bool FP8>
-__device__ __forceinline__ float pool_value(const void* pool, const uint8_t* scale, size_t key, int HD, int d) {
-    if (FP8) {
-        const unsigned c = ((const uint8_t*)pool)[key * HD + d];
-        const unsigned r = __builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(c, exp2i((int)scale[key] - 127), false));
-        return bflo(r);
-    }
-    return bf2f(((const bf16_t*)pool)[key * HD + d]);
-}
-
-// One wave per (token, head): every lane owns HD / 64 columns, the keys go by one at a time with a running maximum and sum.
-template <int HD, bool FP8>
-__global__ __launch_bounds__(64) void attn_paged_simple_kernel(AttnPagedArgs p) {
-    constexpr int C = HD / 64;
-    const int t = blockIdx.x, head = blockIdx.y, lane = threadIdx.x;
-    const int kvh = head / (p.nh / p.nkv);
-    if (t < p.cu_q[0]) return;
-    const int b = find_seq(p.cu_q, p.B, t);
-    if (b >= p.B) return;                            // behind the last sequence: left as it was
-    const int n = p.cu_q[b + 1] - p.cu_q[b];
-    const int last = p.kv_len[b] - n + (t - p.cu_q[b]);                 // the last key this row sees
-    float qv[C], acc[C], m = -INFINITY, l = 0.f;
-#pragma unroll
-    for (int c = 0; c < C; ++c) { qv[c] = bf2f(p.q[(size_t)t * p.ldq + head * HD + c * 64 + lane]) * p.qscale; acc[c] = 0.f; }
-    for (int key = 0; key <= last; ++key) {
-        const int pi = key >> p.page_shift;
-        const int page = pi < p.max_pages ? p.table[(size_t)b * p.ld_table + pi] : -1;
-        if (page < 0 || page >= p.n_pages) { l = __builtin_nanf(""); break; }
-        const size_t at = (((size_t)page * p.nkv + kvh) << p.page_shift) + (key & ((1 << p.page_shift) - 1));
-        float s = 0.f;
-#pragma unroll
-        for (int c = 0; c < C; ++c) s += qv[c] * pool_value<FP8>(p.kpool, p.kscale, at, HD, c * 64 + lane);
-        s = wave_sum(s);
-        const float mn = fmaxf(m, s), mu = mn == -INFINITY ? 0.f : mn;
-        const float a = __builtin_amdgcn_exp2f(m - mu), e = __builtin_amdgcn_exp2f(s - mu);
-        l = l * a + e;
-#pragma unroll
-        for (int c = 0; c < C; ++c) acc[c] = acc[c] * a + e * pool_value<FP8>(p.vpool, p.vscale, at, HD, c * 64 + lane);
-        m = mn;
-    }
-    const float inv = l == 0.f ? 0.f : 1.f / l;
-#pragma unroll
-    for (int c = 0; c < C; ++c) p.out[(size_t)t * p.ldo + head * HD + c * 64 + lane] = f2bf(acc[c] * inv);
-}
-
-int log2_exact(int x) {
-    for (int s = 0; s < 31; ++s)
-        if (x == 1 << s) return s;
-    return -1;
-}
-bool aligned16(const void* p) { return ((uintptr_t)p % 16) == 0; }
-
-// what the three entry points ask of a cache
-int check_pool(const char* what, const void* kpool, const void* vpool, const void* kscale, const void* vscale, int n_pages, int page_size,
-               int n_kv_heads, int head_dim) {
-    MOLLY_CHECK(head_dim == 64 || head_dim == 128, "%s: head_dim=%d (built for 64 and 128)", what, head_dim);
-    MOLLY_CHECK(n_pages > 0 && n_kv_heads > 0 && page_size >= 16 && page_size <= 256 && log2_exact(page_size) >= 0,
-                "%s: n_pages=%d n_kv_heads=%d page_size=%d (a power of two in 16..256)", what, n_pages, n_kv_heads, page_size);
-    MOLLY_CHECK((long)n_pages * page_size <= 0x7fffffffL, "%s: %d pages of %d places: places are 32-bit", what, n_pages, page_size);
-    MOLLY_CHECK(kpool && vpool && aligned16(kpool) && aligned16(vpool), "%s: the pools must be 16-byte aligned device memory", what);
-    MOLLY_CHECK((kscale == nullptr) == (vscale == nullptr), "%s: e4m3 pools have exponents for K and for V", what);
-    return 0;
-}
-
 }  // namespace
 
 extern "C" int molly_paged_kv_append(void* stream, const void* k, const void* v, const void* q_or_null, void* q_out_or_null, void* kpool,
@@ -321,38 +216,6 @@ extern "C" int molly_paged_kv_read(void* stream, const void* kpool, const void* 
     } else {
         if (kscale_or_null) hipLaunchKernelGGL((paged_read_kernel<64, true>), grid, dim3(256), 0, st, p);
         else hipLaunchKernelGGL((paged_read_kernel<64, false>), grid, dim3(256), 0, st, p);
-    }
-    MOLLY_LAUNCH_CHECK();
-    return 0;
-}
-
-extern "C" int molly_attn_paged(void* stream, const void* q, void* out, const void* kpool, const void* vpool, const void* kscale_or_null,
-                                const void* vscale_or_null, const int* block_table, const int* cu_q, const int* kv_len, int n_tokens, int B,
-                                int n_pages, int page_size, int max_pages, int ld_table, int n_heads, int n_kv_heads, int head_dim, int ldq,
-                                int ldo, float scale) {
-    MOLLY_ENTER();
-    if (int rc = check_pool("attn_paged", kpool, vpool, kscale_or_null, vscale_or_null, n_pages, page_size, n_kv_heads, head_dim)) return rc;
-    MOLLY_CHECK(n_tokens >= 0 && B >= 0 && max_pages >= 0 && ld_table >= max_pages, "attn_paged: n_tokens=%d B=%d max_pages=%d ld_table=%d", n_tokens, B,
-                max_pages, ld_table);
-    MOLLY_CHECK(n_heads > 0 && n_heads % n_kv_heads == 0 && n_heads <= 65535, "attn_paged: n_heads=%d not a multiple of n_kv_heads=%d", n_heads, n_kv_heads);
-    if (n_tokens == 0 || B == 0) return 0;
-    MOLLY_CHECK(q && out && block_table && cu_q && kv_len, "attn_paged: q, out, block_table, cu_q, kv_len required");
-    MOLLY_CHECK(aligned16(q) && aligned16(out) && ldq % 8 == 0 && ldo % 8 == 0 && ldq >= n_heads * head_dim && ldo >= n_heads * head_dim,
-                "attn_paged: q / out rows must be 16-byte aligned and hold n_heads * head_dim values (ldq=%d ldo=%d)", ldq, ldo);
-    AttnPagedArgs p{};
-    p.q = (const bf16_t*)q; p.out = (bf16_t*)out; p.kpool = kpool; p.vpool = vpool;
-    p.kscale = (const uint8_t*)kscale_or_null; p.vscale = (const uint8_t*)vscale_or_null;
-    p.table = block_table; p.cu_q = cu_q; p.kv_len = kv_len; p.n_tok = n_tokens; p.B = B;
-    p.n_pages = n_pages; p.page_shift = log2_exact(page_size); p.max_pages = max_pages; p.ld_table = ld_table;
-    p.nh = n_heads; p.nkv = n_kv_heads; p.ldq = ldq; p.ldo = ldo; p.qscale = scale * 1.44269504088896341f;
-    const dim3 grid(n_tokens, n_heads);
-    hipStream_t st = (hipStream_t)stream;
-    if (head_dim == 128) {
-        if (kscale_or_null) hipLaunchKernelGGL((attn_paged_simple_kernel<128, true>), grid, dim3(64), 0, st, p);
-        else hipLaunchKernelGGL((attn_paged_simple_kernel<128, false>), grid, dim3(64), 0, st, p);
-    } else {
-        if (kscale_or_null) hipLaunchKernelGGL((attn_paged_simple_kernel<64, true>), grid, dim3(64), 0, st, p);
-        else hipLaunchKernelGGL((attn_paged_simple_kernel<64, false>), grid, dim3(64), 0, st, p);
     }
     MOLLY_LAUNCH_CHECK();
     return 0;

@@ -872,11 +872,18 @@ def paged_kv_read(kpool, vpool, slot, kscale=None, vscale=None, k_out=None, v_ou
     return k_out, v_out
 
 
-def attn_paged(q, kpool, vpool, block_table, cu_q, kv_len, n_heads, scale=None, kscale=None, vscale=None, max_q=0, max_kv=0, out=None):
+def attn_paged_workspace(n_tokens, B, n_heads, n_kv_heads, head_dim, page_size, max_pages, e4m3, max_q=0, max_kv=0) -> int:
+    """fp32 elements of scratch that an attn_paged of these sizes can use (0: none)"""
+    return lib().query("molly_attn_paged_workspace", n_tokens, B, n_heads, n_kv_heads, head_dim, page_size, max_pages, int(e4m3), max_q, max_kv)
+
+
+def attn_paged(q, kpool, vpool, block_table, cu_q, kv_len, n_heads, scale=None, kscale=None, vscale=None, max_q=0, max_kv=0, out=None,
+               workspace=None):
     """Causal attention of ragged chunks of new tokens over a paged cache (molly_attn_paged).  q [n_tokens, n_heads * dim]: sequence b's new tokens
     are the rows cu_q[b] .. cu_q[b + 1] - 1 (int32 [B + 1]), kv_len (int32 [B]) its keys in the cache, the new tokens' among them,
     block_table (int32 [B, max_pages]) its pages.  scale: dim ** -0.5 by default.  max_q / max_kv: the most new tokens / keys of any sequence, as
-    far as the caller knows; they only choose how the work is cut (0: n_tokens / what the table can hold).  -> out [n_tokens, n_heads * dim]"""
+    far as the caller knows; they only choose how the work is cut (0: n_tokens / what the table can hold).  workspace: float32 scratch of
+    attn_paged_workspace(..) elements (None: the call takes its own).  -> out [n_tokens, n_heads * dim]"""
     what = "attn_paged"
     P, nkv, page, hd = _pools(kpool, vpool, kscale, vscale, what)
     n_heads = int(n_heads)
@@ -894,10 +901,16 @@ def attn_paged(q, kpool, vpool, block_table, cu_q, kv_len, n_heads, scale=None, 
     _rows(out, what, "out", n_heads * hd)
     if out.shape[0] != n:
         raise ValueError(f"{what}: {n} rows of q and {out.shape[0]} of out")
-    _same_device(what, dev, q, vpool, kscale, vscale, block_table, cu_q, kv_len, out)
+    if workspace is None:
+        floats = attn_paged_workspace(n, B, n_heads, nkv, hd, page, max_pages, kscale is not None, max_q, max_kv)
+        workspace = torch.empty(floats, dtype=torch.float32, device=q.device) if floats else None
+    elif workspace.dtype != torch.float32 or not workspace.is_contiguous():
+        raise ValueError(f"{what}: workspace must be contiguous float32")
+    _same_device(what, dev, q, vpool, kscale, vscale, block_table, cu_q, kv_len, out, workspace)
     with torch.cuda.device(dev):
         lib().call("molly_attn_paged", _stream(), q, out, kpool, vpool, kscale, vscale, block_table, cu_q, kv_len, n, B, P, page, max_pages,
-                   block_table.stride(0) if B > 1 else max_pages, n_heads, nkv, hd, _ld(q), _ld(out), float(hd ** -0.5 if scale is None else scale))
+                   block_table.stride(0) if B > 1 else max_pages, n_heads, nkv, hd, _ld(q), _ld(out), float(hd ** -0.5 if scale is None else scale),
+                   max_q, max_kv, workspace, workspace.numel() if workspace is not None else 0)
     return out
 
 

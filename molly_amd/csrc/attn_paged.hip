@@ -22,7 +22,7 @@
 
 namespace {
 
-constexpr int TROWS = 128, RROWS = 32;               // rows of a tile in the two kernels
+constexpr int RROWS = 32;                            // rows of a tile in the rows kernel; the tile kernel has 128 * RB
 constexpr int MIN_KEYS_ROWS = 256, MIN_KEYS_TILE = 512;      // fewest keys that a part of a cut key axis gets
 constexpr int MAX_PARTS = 64;
 
@@ -164,11 +164,11 @@ __device__ __forceinline__ void rows_init(Rows<HD>& st, const AttnPagedArgs& p, 
 // V values that are not finite, in a step that some row does not see all of: P is 0 there, and 0 * NaN would be NaN.  attend32 takes them out of such
 // a step (clear_odd) and this adds them to the rows that do see them, at the end.  step0, step0 + stride ..: the wave's steps below k1.
 template <int HD, bool FP8>
-__device__ __forceinline__ void add_odd(Rows<HD>& st, const AttnPagedArgs& p, const KvSource& src, int step0, int stride, int k1, int lane) {
+__device__ __forceinline__ void add_odd(Rows<HD>& st, int qmin, const AttnPagedArgs& p, const KvSource& src, int step0, int stride, int k1, int lane) {
     const int h = lane >> 5;
 #pragma unroll 1
     for (int kb = step0; kb < k1; kb += stride) {
-        if (kb + 31 <= st.qmin) continue;
+        if (kb + 31 <= qmin) continue;                // (every row saw these: they went through the product)
 #pragma unroll 1
         for (int key = kb; key < min(kb + 32, k1); ++key) {
             const size_t at = src.group(key, src.row[key >> src.shift]) + (key & 15);
@@ -227,60 +227,68 @@ __device__ __forceinline__ bool clear_odd(bf16x8 (&vf)[2][ND]) {
     return true;
 }
 
-// one step of 32 keys: rows `sub` * 32 .. of the images, keys kbase ..
-template <int HD>
-__device__ __forceinline__ void attend32(Rows<HD>& st, const bf16_t* sK, const bf16_t* sV, int sub, int kbase, float scale_log2, int lane) {
+// one step of 32 keys: rows `sub` * 32 .. of the images, keys kbase ..  RB blocks of 32 query rows share the K and V fragments.
+template <int HD, int RB>
+__device__ __forceinline__ void attend32(Rows<HD> (&st)[RB], const bf16_t* sK, const bf16_t* sV, int sub, int kbase, float scale_log2, int lane) {
     constexpr int NS = HD / 16, ND = HD / 32;
     const int r = lane & 31, h = lane >> 5;
     bf16x8 kf[NS];
 #pragma unroll
     for (int s = 0; s < NS; ++s) kf[s] = row_frag<HD>(sK, 32 * sub + r, s, h);
     __builtin_amdgcn_sched_barrier(0);               // every read in flight before the first MFMA
-    f32x16 sc;
+    f32x16 sc[RB];
 #pragma unroll
-    for (int e = 0; e < 16; ++e) sc[e] = 0.f;
+    for (int b = 0; b < RB; ++b) {
 #pragma unroll
-    for (int s = 0; s < NS; ++s) sc = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kf[s], st.qf[s], sc, 0, 0, 0);
+        for (int e = 0; e < 16; ++e) sc[b][e] = 0.f;
+#pragma unroll
+        for (int s = 0; s < NS; ++s) sc[b] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kf[s], st[b].qf[s], sc[b], 0, 0, 0);
+    }
     bf16x8 vf[2][ND];
 #pragma unroll
     for (int sp = 0; sp < 2; ++sp)
 #pragma unroll
         for (int d = 0; d < ND; ++d) vf[sp][d] = tr_frag<HD>(sV, 32 * sub, sp, d, lane);
-    const bool edge = kbase + 31 > st.qmin;          // (uniform) some row does not see all of the step
-    float mx = -INFINITY;
+    const bool edge = kbase + 31 > st[0].qmin;       // (uniform) some row does not see all of the step
     if (edge) {
 #pragma unroll
-        for (int e = 0; e < 16; ++e) {
-            const int key = kbase + (e & 3) + 8 * (e >> 2) + 4 * h;
-            sc[e] = key <= st.qi ? sc[e] : -INFINITY;
+        for (int b = 0; b < RB; ++b)
+#pragma unroll
+            for (int e = 0; e < 16; ++e) {
+                const int key = kbase + (e & 3) + 8 * (e >> 2) + 4 * h;
+                sc[b][e] = key <= st[b].qi ? sc[b][e] : -INFINITY;
+            }
+        if (clear_odd<ND>(vf)) st[0].odd = true;
+    }
+#pragma unroll
+    for (int b = 0; b < RB; ++b) {
+        float mx = -INFINITY;
+#pragma unroll
+        for (int e = 0; e < 16; ++e) mx = fmaxf(mx, sc[b][e]);
+        mx = xhalf_max(mx) * scale_log2;
+        if (!__all(mx - st[b].m <= RESCALE_THR)) {   // the reference maximum follows only where it has grown by more than 2^8
+            const float m_new = fmaxf(st[b].m, mx);
+            const float alpha = fast_exp2(st[b].m - (m_new == -INFINITY ? 0.f : m_new));
+            st[b].l *= alpha;
+            st[b].m = m_new;
+#pragma unroll
+            for (int d = 0; d < ND; ++d)
+#pragma unroll
+                for (int e = 0; e < 16; ++e) st[b].o[d][e] *= alpha;
         }
-    }
+        const float m_ref = st[b].m == -INFINITY ? 0.f : st[b].m;
 #pragma unroll
-    for (int e = 0; e < 16; ++e) mx = fmaxf(mx, sc[e]);
-    mx = xhalf_max(mx) * scale_log2;
-    if (!__all(mx - st.m <= RESCALE_THR)) {          // the reference maximum follows only where it has grown by more than 2^8
-        const float m_new = fmaxf(st.m, mx);
-        const float alpha = fast_exp2(st.m - (m_new == -INFINITY ? 0.f : m_new));
-        st.l *= alpha;
-        st.m = m_new;
+        for (int e = 0; e < 16; ++e) sc[b][e] = fast_exp2(sc[b][e] * scale_log2 - m_ref);
+        float rs[4];
 #pragma unroll
-        for (int d = 0; d < ND; ++d)
+        for (int g = 0; g < 4; ++g) rs[g] = (sc[b][4 * g] + sc[b][4 * g + 1]) + (sc[b][4 * g + 2] + sc[b][4 * g + 3]);
+        st[b].l += (rs[0] + rs[1]) + (rs[2] + rs[3]);
+        const bf16x8 pf[2] = {acc_to_frag(sc[b], 0), acc_to_frag(sc[b], 8)};
 #pragma unroll
-            for (int e = 0; e < 16; ++e) st.o[d][e] *= alpha;
-    }
-    const float m_ref = st.m == -INFINITY ? 0.f : st.m;
-#pragma unroll
-    for (int e = 0; e < 16; ++e) sc[e] = fast_exp2(sc[e] * scale_log2 - m_ref);
-    float rs[4];
-#pragma unroll
-    for (int g = 0; g < 4; ++g) rs[g] = (sc[4 * g] + sc[4 * g + 1]) + (sc[4 * g + 2] + sc[4 * g + 3]);
-    st.l += (rs[0] + rs[1]) + (rs[2] + rs[3]);
-    const bf16x8 pf[2] = {acc_to_frag(sc, 0), acc_to_frag(sc, 8)};
-    if (edge && clear_odd<ND>(vf)) st.odd = true;
-#pragma unroll
-    for (int d = 0; d < ND; ++d) {
-        st.o[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vf[0][d], pf[0], st.o[d], 0, 0, 0);
-        st.o[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vf[1][d], pf[1], st.o[d], 0, 0, 0);
+        for (int d = 0; d < ND; ++d) {
+            st[b].o[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vf[0][d], pf[0], st[b].o[d], 0, 0, 0);
+            st[b].o[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vf[1][d], pf[1], st[b].o[d], 0, 0, 0);
+        }
     }
 }
 
@@ -325,7 +333,8 @@ __global__ __launch_bounds__(256, (HD == 128 && !FP8) ? 1 : 2) void attn_paged_r
         const int k0 = s * chunk, k1 = min(n_keys, k0 + chunk), last = k1 - 1;
         const KvSource src{p.table + (size_t)b * p.ld_table, p.n_pages, p.page_shift, p.nkv, kvh};
         if (tid == 0) s_bad = t.n_vis > kmax ? kmax : 0x7fffffff;
-        Rows<HD> st;
+        Rows<HD> rows[1];
+        Rows<HD>& st = rows[0];
         rows_init<HD>(st, p, t, kvh, 0, lane);
         const int key0 = k0 + 32 * wave;
         // page ids of the wave's next 32 steps, two groups each: lane 2 i + g.  Waited for here, once in 4,096 keys: a wait inside the steps would be a wait
@@ -372,7 +381,7 @@ __global__ __launch_bounds__(256, (HD == 128 && !FP8) ? 1 : 2) void attn_paged_r
 #pragma unroll
                 for (int g = 0; g < 2; ++g) codes_store<HD>(c[g], img + g * 16 * HD, img + IMG + g * 16 * HD, lane);
                 if (key + 128 < k1) load_step(key + 128);
-                attend32<HD>(st, img, img + IMG, 0, key, p.scale_log2, lane);
+                attend32<HD, 1>(rows, img, img + IMG, 0, key, p.scale_log2, lane);
             }
         } else {
             int buf = 0;
@@ -389,11 +398,11 @@ __global__ __launch_bounds__(256, (HD == 128 && !FP8) ? 1 : 2) void attn_paged_r
                 } else {
                     dma_wait();
                 }
-                attend32<HD>(st, img + buf * 2 * IMG, img + buf * 2 * IMG + IMG, 0, key, p.scale_log2, lane);
+                attend32<HD, 1>(rows, img + buf * 2 * IMG, img + buf * 2 * IMG + IMG, 0, key, p.scale_log2, lane);
                 buf ^= 1;
             }
         }
-        if (st.odd) add_odd<HD, FP8>(st, p, src, k0 + 32 * wave, 128, k1, lane);
+        if (st.odd) add_odd<HD, FP8>(st, st.qmin, p, src, k0 + 32 * wave, 128, k1, lane);
         __syncthreads();                             // the images are dead; s_bad is set
         scan_pages(p, src.row, k0, k1, &s_bad);
         // the four waves' rows, un-normalised, through LDS
@@ -442,9 +451,9 @@ __global__ __launch_bounds__(256, (HD == 128 && !FP8) ? 1 : 2) void attn_paged_r
     }
 }
 
-// ---- long chunks: 128 rows a block -----------------------------------------------------------------------------------------------------------
+// ---- long chunks: 128 * RB rows a block -----------------------------------------------------------------------------------------------------------
 // tile f of the sequences' tiles in reverse order (within a sequence the longest causal range first); -1: there are fewer
-__device__ __forceinline__ int find_tile(const AttnPagedArgs& p, int f, int lane, int* ti) {
+template <int TROWS> __device__ __forceinline__ int find_tile(const AttnPagedArgs& p, int f, int lane, int* ti) {
     auto tiles = [&](int b) {
         if (b >= p.B) return 0;
         const int s = min(max(p.cu_q[b], 0), p.n_tok), e = min(max(p.cu_q[b + 1], s), p.n_tok);
@@ -473,12 +482,12 @@ __device__ __forceinline__ int find_tile(const AttnPagedArgs& p, int f, int lane
     return -1;
 }
 
-template <int HD, bool FP8>
-__global__ __launch_bounds__(256, 2) void attn_paged_tile_kernel(AttnPagedArgs p) {
+template <int HD, bool FP8, int RB>
+__global__ __launch_bounds__(256, RB == 1 ? 2 : 1) void attn_paged_tile_kernel(AttnPagedArgs p) {
     extern __shared__ __attribute__((aligned(16))) char smem_raw[];
     __shared__ int s_bad;
     bf16_t* smem = reinterpret_cast<bf16_t*>(smem_raw);            // [2 stages][K tile | V tile]
-    constexpr int TILE = 64 * HD;
+    constexpr int TILE = 64 * HD, TROWS = 128 * RB, WROWS = 32 * RB;
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     // the workgroups of one XCD (every eighth) take a contiguous run of the order (kv head, part, tile): they share a head's keys in its L2
     const int q8 = gridDim.x >> 3, r8 = gridDim.x & 7, xcd = blockIdx.x & 7;
@@ -486,7 +495,7 @@ __global__ __launch_bounds__(256, 2) void attn_paged_tile_kernel(AttnPagedArgs p
     const int f = v % p.tps; v /= p.tps;
     const int s = v % p.parts, kvh = v / p.parts;
     int ti = 0;
-    const int b = __builtin_amdgcn_readfirstlane(find_tile(p, f, lane, &ti));
+    const int b = __builtin_amdgcn_readfirstlane(find_tile<TROWS>(p, f, lane, &ti));
     if (b < 0) return;
     ti = __builtin_amdgcn_readfirstlane(ti);
     const Tile t = make_tile<TROWS>(p, b, ti);
@@ -498,11 +507,15 @@ __global__ __launch_bounds__(256, 2) void attn_paged_tile_kernel(AttnPagedArgs p
     const int k0 = s * chunk, k1 = min(n_keys, k0 + chunk), last = k1 - 1;
     const KvSource src{p.table + (size_t)b * p.ld_table, p.n_pages, p.page_shift, p.nkv, kvh};
     if (tid == 0) s_bad = t.n_vis > kmax ? kmax : 0x7fffffff;
-    const bool active = wave * 32 < t.rows;
-    Rows<HD> st;
-    rows_init<HD>(st, p, t, kvh, wave * 32, lane);
+    const bool active = wave * WROWS < t.rows;
+    Rows<HD> st[RB];
 #pragma unroll
-    for (int i = 0; i < HD / 16; ++i) arrived(st.qf[i]);
+    for (int rb = 0; rb < RB; ++rb) rows_init<HD>(st[rb], p, t, kvh, wave * WROWS + 32 * rb, lane);
+#pragma unroll
+    for (int rb = 0; rb < RB; ++rb)
+#pragma unroll
+        for (int i = 0; i < HD / 16; ++i) arrived(st[rb].qf[i]);
+    const int qmax = st[RB - 1].qmax;
     unsigned off[NPG<HD>];
 #pragma unroll
     for (int i = 0; i < NPG<HD>; ++i) {
@@ -553,104 +566,126 @@ __global__ __launch_bounds__(256, 2) void attn_paged_tile_kernel(AttnPagedArgs p
         if (active) {
 #pragma unroll
             for (int sub = 0; sub < 2; ++sub)
-                if (k + 32 * sub <= st.qmax) attend32<HD>(st, sK, sK + TILE, sub, k + 32 * sub, p.scale_log2, lane);
+                if (k + 32 * sub <= qmax) attend32<HD, RB>(st, sK, sK + TILE, sub, k + 32 * sub, p.scale_log2, lane);
         }
         if (k + 64 < k1) land(cur ^ 1);
         __syncthreads();
         cur ^= 1;
     }
     if (k0 >= k1) __syncthreads();                   // (s_bad)
-    // ---- epilogue: this wave's 32 rows
+    // ---- epilogue: this wave's rows, 32 at a time
     if (!active) return;
-    if (st.odd) add_odd<HD, FP8>(st, p, src, k0, 32, min(k1, st.qmax + 1), lane);
     const int r = lane & 31, h = lane >> 5;
-    float l = st.l + __shfl_xor(st.l, 32, 64);
-    if (st.qi >= s_bad) l = __builtin_nanf("");
-    const int rows = min(32, t.rows - wave * 32);
-    if (parts > 1) {
-        float* part = p.part + ((size_t)(f * p.nkv + kvh) * p.parts + s) * (TROWS * (HD + 2));
-        if (r < rows) {
-            float* d = part + (size_t)(wave * 32 + r) * HD;
 #pragma unroll
-            for (int dd = 0; dd < HD / 32; ++dd)
+    for (int rb = 0; rb < RB; ++rb) {
+        const int wrow = wave * WROWS + 32 * rb, rows = min(32, t.rows - wrow);
+        if (rows <= 0) return;
+        if (st[0].odd) add_odd<HD, FP8>(st[rb], st[0].qmin, p, src, k0, 32, min(k1, qmax + 1), lane);
+        float l = st[rb].l + __shfl_xor(st[rb].l, 32, 64);
+        if (st[rb].qi >= s_bad) l = __builtin_nanf("");
+        if (parts > 1) {
+            float* part = p.part + ((size_t)(f * p.nkv + kvh) * p.parts + s) * (TROWS * (HD + 2));
+            if (r < rows) {
+                float* d = part + (size_t)(wrow + r) * HD;
 #pragma unroll
-                for (int g4 = 0; g4 < 4; ++g4)
-                    *reinterpret_cast<f32x4*>(d + 32 * dd + 8 * g4 + 4 * h) =
-                        f32x4{st.o[dd][4 * g4], st.o[dd][4 * g4 + 1], st.o[dd][4 * g4 + 2], st.o[dd][4 * g4 + 3]};
-            if (h == 0) { part[TROWS * HD + (wave * 32 + r) * 2] = st.m; part[TROWS * HD + (wave * 32 + r) * 2 + 1] = l; }
+                for (int dd = 0; dd < HD / 32; ++dd)
+#pragma unroll
+                    for (int g4 = 0; g4 < 4; ++g4)
+                        *reinterpret_cast<f32x4*>(d + 32 * dd + 8 * g4 + 4 * h) = f32x4{st[rb].o[dd][4 * g4], st[rb].o[dd][4 * g4 + 1],
+                                                                                       st[rb].o[dd][4 * g4 + 2], st[rb].o[dd][4 * g4 + 3]};
+                if (h == 0) *reinterpret_cast<f32x2*>(part + TROWS * HD + (wrow + r) * 2) = f32x2{st[rb].m, l};
+            }
+            continue;
         }
-        return;
-    }
-    const float inv = l == 0.f ? 0.f : 1.f / l;
-    // rows through a slab of the wave's own in the dead stages: whole rows leave, 16 bytes a lane
-    constexpr int PITCH = HD + 8, LPR = HD / 8, RPI = 64 / LPR;
-    bf16_t* slab = smem + wave * 32 * PITCH;
+        const float inv = l == 0.f ? 0.f : 1.f / l;
+        // rows through a slab of the wave's own in the dead stages: whole rows leave, 16 bytes a lane
+        constexpr int PITCH = HD + 8, LPR = HD / 8, RPI = 64 / LPR;
+        bf16_t* slab = smem + wave * 32 * PITCH;
 #pragma unroll
-    for (int d = 0; d < HD / 32; ++d)
+        for (int d = 0; d < HD / 32; ++d)
 #pragma unroll
-        for (int g4 = 0; g4 < 4; ++g4)
-            *reinterpret_cast<u32x2*>(slab + r * PITCH + 32 * d + 8 * g4 + 4 * h) =
-                u32x2{pack_bf2(st.o[d][4 * g4] * inv, st.o[d][4 * g4 + 1] * inv), pack_bf2(st.o[d][4 * g4 + 2] * inv, st.o[d][4 * g4 + 3] * inv)};
-    const int lr = lane / LPR, lc = (lane % LPR) * 8;
+            for (int g4 = 0; g4 < 4; ++g4)
+                *reinterpret_cast<u32x2*>(slab + r * PITCH + 32 * d + 8 * g4 + 4 * h) =
+                    u32x2{pack_bf2(st[rb].o[d][4 * g4] * inv, st[rb].o[d][4 * g4 + 1] * inv),
+                          pack_bf2(st[rb].o[d][4 * g4 + 2] * inv, st[rb].o[d][4 * g4 + 3] * inv)};
+        const int lr = lane / LPR, lc = (lane % LPR) * 8;
 #pragma unroll
-    for (int it = 0; it < 32 / RPI; ++it) {
-        const int row = it * RPI + lr;
-        const u32x4 x = *reinterpret_cast<const u32x4*>(slab + row * PITCH + lc);
-        const int R = t.row0 + wave * 32 + row, tok = R / p.G;
-        if (row < rows) *reinterpret_cast<u32x4*>(p.out + (size_t)(t.tok0 + tok) * p.ldo + (kvh * p.G + R - tok * p.G) * HD + lc) = x;
+        for (int it = 0; it < 32 / RPI; ++it) {
+            const int row = it * RPI + lr;
+            const u32x4 x = *reinterpret_cast<const u32x4*>(slab + row * PITCH + lc);
+            const int R = t.row0 + wrow + row, tok = R / p.G;
+            if (row < rows) *reinterpret_cast<u32x4*>(p.out + (size_t)(t.tok0 + tok) * p.ldo + (kvh * p.G + R - tok * p.G) * HD + lc) = x;
+        }
     }
 }
 
-// ---- the parts of a tile's rows: out = sum_s 2^(m_s - m) o_s / sum_s 2^(m_s - m) l_s; one wave a row
-template <int HD, bool TILEK>
+// ---- the parts of a tile's rows: out = sum_s 2^(m_s - m) o_s / sum_s 2^(m_s - m) l_s; one wave a row, lane s holding part s's maximum and sum
+template <int HD, int ROWS>
 __global__ __launch_bounds__(256) void attn_paged_merge_kernel(AttnPagedArgs p) {
-    constexpr int ROWS = TILEK ? TROWS : RROWS, C = HD / 64;
-    const int lane = threadIdx.x & 63, row = blockIdx.y * 4 + (threadIdx.x >> 6);
+    constexpr bool TILEK = ROWS != RROWS;
+    constexpr int C = HD / 64, STRIDE = ROWS * (HD + 2);
+    const int lane = threadIdx.x & 63;
     const int tile = blockIdx.x / p.nkv, kvh = blockIdx.x % p.nkv;
     int b, ti = 0;
-    if (TILEK) b = find_tile(p, tile, lane, &ti);
+    if constexpr (TILEK) b = find_tile<ROWS>(p, tile, lane, &ti);
     else { b = tile / p.tps; ti = tile % p.tps; }
     if (b < 0) return;
     const Tile t = make_tile<ROWS>(p, b, ti);
-    if (row >= t.rows) return;
     const int parts = parts_of(min(t.n_vis, p.max_pages << p.page_shift), p.parts, TILEK ? MIN_KEYS_TILE : MIN_KEYS_ROWS);
     if (parts == 1) return;                          // written by the attention itself
-    const float* base = p.part + (size_t)(tile * p.nkv + kvh) * p.parts * (ROWS * (HD + 2));
-    float m = -INFINITY;
-    for (int s = 0; s < parts; ++s) m = fmaxf(m, base[(size_t)s * (ROWS * (HD + 2)) + ROWS * HD + row * 2]);
-    const float mu = m == -INFINITY ? 0.f : m;
-    float l = 0.f, a[C];
+    const float* base = p.part + (size_t)(tile * p.nkv + kvh) * p.parts * STRIDE;
+    for (int row = blockIdx.y * 4 + (threadIdx.x >> 6); row < t.rows; row += gridDim.y * 4) {
+        float ms = -INFINITY, ls = 0.f;
+        if (lane < parts) {
+            const f32x2 ml = *reinterpret_cast<const f32x2*>(base + (size_t)lane * STRIDE + ROWS * HD + row * 2);
+            ms = ml[0]; ls = ml[1];
+        }
+        const float m = wave_max(ms), f = fast_exp2(ms - (m == -INFINITY ? 0.f : m));
+        const float l = wave_sum(lane < parts ? ls * f : 0.f);
+        float a[C];
 #pragma unroll
-    for (int c = 0; c < C; ++c) a[c] = 0.f;
-    for (int s = 0; s < parts; ++s) {
-        const float* ps = base + (size_t)s * (ROWS * (HD + 2));
-        const float f = fast_exp2(ps[ROWS * HD + row * 2] - mu);
-        l += ps[ROWS * HD + row * 2 + 1] * f;
+        for (int c = 0; c < C; ++c) a[c] = 0.f;
+        const float* po = base + row * HD + lane * C;
+        for (int s0 = 0; s0 < parts; s0 += 8) {      // eight parts' loads in flight
+            float x[8][C];
 #pragma unroll
-        for (int c = 0; c < C; ++c) a[c] += f == 0.f ? 0.f : ps[row * HD + lane * C + c] * f;
+            for (int i = 0; i < 8; ++i)
+#pragma unroll
+                for (int c = 0; c < C; ++c) x[i][c] = po[(size_t)min(s0 + i, parts - 1) * STRIDE + c];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {            // (lanes behind the last part weigh 0; a part that weighs nothing adds nothing: never 0 * inf)
+                const float fs = s0 + i < parts ? __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, f), (s0 + i) & 63)) : 0.f;
+#pragma unroll
+                for (int c = 0; c < C; ++c) a[c] += fs == 0.f ? 0.f : x[i][c] * fs;
+            }
+        }
+        const float inv = l == 0.f ? 0.f : 1.f / l;
+        const int R = t.row0 + row, tok = R / p.G;
+        bf16_t* d = p.out + (size_t)(t.tok0 + tok) * p.ldo + (kvh * p.G + R - tok * p.G) * HD + lane * C;
+        if (C == 2) *reinterpret_cast<unsigned*>(d) = pack_bf2(a[0] * inv, a[C - 1] * inv);
+        else d[0] = f2bf(a[0] * inv);
     }
-    const float inv = l == 0.f ? 0.f : 1.f / l;
-    const int R = t.row0 + row, tok = R / p.G;
-    bf16_t* d = p.out + (size_t)(t.tok0 + tok) * p.ldo + (kvh * p.G + R - tok * p.G) * HD + lane * C;
-    if (C == 2) *reinterpret_cast<unsigned*>(d) = pack_bf2(a[0] * inv, a[C - 1] * inv);
-    else d[0] = f2bf(a[0] * inv);
 }
 
 // ---- host: which kernel, and how many parts
-struct Shape { bool tile; int tps, parts; long part_floats; };
+struct Shape { int rb, tps, parts, rows; long part_floats; };
 Shape pick_shape(int n_tok, int B, int nkv, int G, int HD, bool fp8, long max_keys, int max_q, int max_kv) {
     Shape sh{};
     const long mq = max_q > 0 && max_q < n_tok ? max_q : n_tok;
     const long keys = max_kv > 0 && max_kv < max_keys ? max_kv : max_keys;
-    sh.tile = mq * G > RROWS;
-    const int rows = sh.tile ? TROWS : RROWS;
-    const long tps = sh.tile ? (long)n_tok * G / TROWS + B : (mq * G + RROWS - 1) / RROWS;
+    // 256-row tiles (one block a CU) where they still give every CU one; 128-row ones (two a CU) below that; the rows kernel for single steps
+    static const int force = [] { const char* e = getenv("MOLLY_PAGED_RB"); return e ? atoi(e) : -1; }();
+    sh.rb = mq * G <= RROWS ? 0 : ((long)n_tok * G / 256) * nkv >= 256 ? 2 : 1;
+    if (force > 0 && sh.rb) sh.rb = force;
+    const int rows = sh.rb ? 128 * sh.rb : RROWS;
+    const long tps = sh.rb ? (long)n_tok * G / rows + B : (mq * G + RROWS - 1) / RROWS;
     sh.tps = (int)tps;
-    const long units = (sh.tile ? tps : tps * B) * nkv;
+    sh.rows = (int)(mq * G < rows ? mq * G : rows);      // rows of a tile, as far as the caller knows
+    const long units = (sh.rb ? tps : tps * B) * nkv;
     // resident blocks: 2 a CU, 1 for the rows kernel with 128 KB of images
-    const long want = sh.tile ? 512 : (HD == 128 && !fp8 ? 512 : 1024);
+    const long want = sh.rb ? 512 / sh.rb : (HD == 128 && !fp8 ? 512 : 1024);
     long parts = want / (units > 0 ? units : 1);
-    const long most = keys / (sh.tile ? MIN_KEYS_TILE : MIN_KEYS_ROWS);
+    const long most = keys / (sh.rb ? MIN_KEYS_TILE : MIN_KEYS_ROWS);
     if (parts > most) parts = most;
     if (parts > MAX_PARTS) parts = MAX_PARTS;
     sh.parts = parts < 1 ? 1 : (int)parts;
@@ -658,21 +693,23 @@ Shape pick_shape(int n_tok, int B, int nkv, int G, int HD, bool fp8, long max_ke
     return sh;
 }
 
+template <int HD, bool FP8, int RB>
+void launch_tile(hipStream_t st, const AttnPagedArgs& p, const Shape& sh) {
+    const size_t lds = 2 * 2 * 64 * HD * 2;
+    static const hipError_t once = hipFuncSetAttribute((const void*)attn_paged_tile_kernel<HD, FP8, RB>, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
+    (void)once;
+    hipLaunchKernelGGL((attn_paged_tile_kernel<HD, FP8, RB>), dim3(sh.tps * p.nkv * sh.parts), dim3(256), lds, st, p);
+    if (sh.parts > 1) hipLaunchKernelGGL((attn_paged_merge_kernel<HD, 128 * RB>), dim3(sh.tps * p.nkv, 32 * RB), dim3(256), 0, st, p);
+}
 template <int HD, bool FP8>
 void launch(hipStream_t st, const AttnPagedArgs& p, const Shape& sh) {
-    if (sh.tile) {
-        const size_t lds = 2 * 2 * 64 * HD * 2;
-        static const hipError_t once = hipFuncSetAttribute((const void*)attn_paged_tile_kernel<HD, FP8>, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
-        (void)once;
-        hipLaunchKernelGGL((attn_paged_tile_kernel<HD, FP8>), dim3(sh.tps * p.nkv * sh.parts), dim3(256), lds, st, p);
-        if (sh.parts > 1) hipLaunchKernelGGL((attn_paged_merge_kernel<HD, true>), dim3(sh.tps * p.nkv, TROWS / 4), dim3(256), 0, st, p);
-    } else {
-        const size_t lds = 4 * RROWS * HD * 4 * (FP8 ? 1 : 2);        // images (e4m3: one buffer of 32 rows K | V in bf16), at the end the four waves' rows in fp32
-        static const hipError_t once = hipFuncSetAttribute((const void*)attn_paged_rows_kernel<HD, FP8>, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
-        (void)once;
-        hipLaunchKernelGGL((attn_paged_rows_kernel<HD, FP8>), dim3(p.B * sh.tps * p.nkv * sh.parts), dim3(256), lds, st, p);
-        if (sh.parts > 1) hipLaunchKernelGGL((attn_paged_merge_kernel<HD, false>), dim3(p.B * sh.tps * p.nkv, RROWS / 4), dim3(256), 0, st, p);
-    }
+    if (sh.rb == 2) return launch_tile<HD, FP8, 2>(st, p, sh);
+    if (sh.rb == 1) return launch_tile<HD, FP8, 1>(st, p, sh);
+    const size_t lds = 4 * RROWS * HD * 4 * (FP8 ? 1 : 2);            // images (e4m3: one buffer of 32 rows K | V in bf16), at the end the four waves' rows in fp32
+    static const hipError_t once = hipFuncSetAttribute((const void*)attn_paged_rows_kernel<HD, FP8>, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
+    (void)once;
+    hipLaunchKernelGGL((attn_paged_rows_kernel<HD, FP8>), dim3(p.B * sh.tps * p.nkv * sh.parts), dim3(256), lds, st, p);
+    if (sh.parts > 1) hipLaunchKernelGGL((attn_paged_merge_kernel<HD, RROWS>), dim3(p.B * sh.tps * p.nkv, cdiv(sh.rows, 4)), dim3(256), 0, st, p);
 }
 
 int check_sizes(int n_tokens, int B, int n_heads, int n_kv_heads, int max_pages, int page_size) {

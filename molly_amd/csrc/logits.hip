@@ -11,6 +11,8 @@
 
 namespace {
 
+constexpr int LONG_HISTORY = 4096;
+
 struct LogitArgs {
     const void* x; float* out;
     const long* gen; const int* n_gen;
@@ -21,30 +23,102 @@ struct LogitArgs {
     long ldx, ldo, ldg, ldb, ldm;                     // ldb / ldm 0: one row for all
 };
 
-template <int SLICE, bool BF16>
-__global__ __launch_bounds__(256) void logits_kernel(LogitArgs p) {
-    __shared__ unsigned cnt[SLICE];
-    const int row = blockIdx.y, v0 = blockIdx.x * SLICE, v1 = min(v0 + SLICE, p.V), t = threadIdx.x;
-    const int n = p.gen ? min(max(p.n_gen ? p.n_gen[row] : p.n_hist, 0), p.n_hist) : 0;
-    if (n > 0) {                                      // (block-uniform)
-        for (int i = t; i < SLICE; i += 256) cnt[i] = 0u;
+// THREADS * 16 tokens a workgroup, four groups of four a thread: 16-byte loads and stores at whatever token the row's first aligned address falls on
+// (`shift` tokens of the first group lie in front of the row).  The logits are asked for in front of the history's pass.
+template <int THREADS, bool BF16, bool HIST>
+__global__ __launch_bounds__(THREADS) void logits_kernel(LogitArgs p) {
+    constexpr int SLICE = THREADS * 16;
+    __shared__ unsigned cnt[HIST ? SLICE : 1];
+    const int row = blockIdx.y, t = threadIdx.x;
+    const size_t x0 = (size_t)row * p.ldx, o0 = (size_t)row * p.ldo;
+    // tokens in front of the row in its first aligned group; -1: the two rows are aligned differently, one token at a time
+    const int sx = (int)((((uintptr_t)p.x >> (BF16 ? 1 : 2)) + x0) & 3), so = (int)((((uintptr_t)p.out >> 2) + o0) & 3);
+    const int shift = sx == so ? sx : 0;
+    const bool vec = sx == so;
+    const int v0 = blockIdx.x * SLICE - shift;       // token of the slice's first place
+    if (v0 >= p.V) return;
+    float x[4][4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        const int v = v0 + (j * THREADS + t) * 4;
+        if (vec && v >= 0 && v + 4 <= p.V) {
+            if constexpr (BF16) {
+                const u32x2 w = *reinterpret_cast<const u32x2*>((const bf16_t*)p.x + x0 + v);
+                x[j][0] = bflo(w[0]); x[j][1] = bfhi(w[0]); x[j][2] = bflo(w[1]); x[j][3] = bfhi(w[1]);
+            } else {
+                const f32x4 w = *reinterpret_cast<const f32x4*>((const float*)p.x + x0 + v);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) x[j][e] = w[e];
+            }
+        } else {
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+                x[j][e] = v + e < 0 || v + e >= p.V ? 0.f : BF16 ? bf2f(((const bf16_t*)p.x)[x0 + v + e]) : ((const float*)p.x)[x0 + v + e];
+        }
+    }
+    if constexpr (HIST) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) *reinterpret_cast<u32x4*>(cnt + (j * THREADS + t) * 4) = u32x4{0, 0, 0, 0};
+        const int n = min(max(p.n_gen ? p.n_gen[row] : p.n_hist, 0), p.n_hist);
         __syncthreads();
         const long* g = p.gen + (size_t)row * p.ldg;
-        for (int i = t; i < n; i += 256) {
-            const long id = g[i];
-            if (id >= v0 && id < v1) atomicAdd(&cnt[(int)(id - v0)], 1u);
+#pragma unroll 4
+        for (int i = t; i < n; i += THREADS) {
+            const long at = g[i] - v0;
+            if (at >= 0 && at < SLICE && g[i] < p.V && g[i] >= 0) atomicAdd(&cnt[(int)at], 1u);
         }
         __syncthreads();
     }
     const float rep = p.rep_v ? p.rep_v[row] : p.rep, pres = p.pres_v ? p.pres_v[row] : p.pres, freq = p.freq_v ? p.freq_v[row] : p.freq;
-    for (int v = v0 + t; v < v1; v += 256) {
-        float s = BF16 ? bf2f(((const bf16_t*)p.x)[(size_t)row * p.ldx + v]) : ((const float*)p.x)[(size_t)row * p.ldx + v];
-        const unsigned c = n > 0 ? cnt[v - v0] : 0u;
-        if (c) s = (s < 0.f ? s * rep : s / rep) - pres - freq * (float)c;
-        if (p.bias) s += p.bias[(size_t)row * p.ldb + v];
-        if (p.mask && !((p.mask[(size_t)row * p.ldm + (v >> 5)] >> (v & 31)) & 1u)) s = -INFINITY;
-        p.out[(size_t)row * p.ldo + v] = s;
+    const unsigned* m = p.mask ? p.mask + (size_t)row * p.ldm : nullptr;
+    const float* bias = p.bias ? p.bias + (size_t)row * p.ldb : nullptr;
+    const bool bias_vec = bias && ((uintptr_t)(bias + v0) & 15) == 0;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        const int v = v0 + (j * THREADS + t) * 4;
+        if (v + 4 <= 0 || v >= p.V) continue;
+        const bool whole = v >= 0 && v + 4 <= p.V;
+        if constexpr (HIST) {
+            const u32x4 c = *reinterpret_cast<const u32x4*>(cnt + (j * THREADS + t) * 4);
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+                if (c[e]) x[j][e] = (x[j][e] < 0.f ? x[j][e] * rep : x[j][e] / rep) - pres - freq * (float)c[e];
+        }
+        if (bias) {
+            if (whole && bias_vec) {
+                const f32x4 b = *reinterpret_cast<const f32x4*>(bias + v);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) x[j][e] += b[e];
+            } else {
+#pragma unroll
+                for (int e = 0; e < 4; ++e) x[j][e] += v + e >= 0 && v + e < p.V ? bias[v + e] : 0.f;
+            }
+        }
+        if (m) {
+            const int first = max(v, 0), last = min(v + 3, p.V - 1);
+            const unsigned wa = m[first >> 5], wb = (last >> 5) != (first >> 5) ? m[last >> 5] : wa;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const unsigned w = ((v + e) >> 5) == (first >> 5) ? wa : wb;
+                if (!((w >> ((v + e) & 31)) & 1u)) x[j][e] = -INFINITY;
+            }
+        }
+        float* o = p.out + o0 + v;
+        if (vec && whole) {
+            *reinterpret_cast<f32x4*>(o) = f32x4{x[j][0], x[j][1], x[j][2], x[j][3]};
+        } else {
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+                if (v + e >= 0 && v + e < p.V) o[e] = x[j][e];
+        }
     }
+}
+
+template <int THREADS, bool HIST>
+void launch(hipStream_t st, const LogitArgs& p, int rows, bool bf16) {
+    const dim3 grid(cdiv(p.V + 3L, THREADS * 16), rows);              // (+ 3: a row may start in the middle of its first group)
+    if (bf16) hipLaunchKernelGGL((logits_kernel<THREADS, true, HIST>), grid, dim3(THREADS), 0, st, p);
+    else hipLaunchKernelGGL((logits_kernel<THREADS, false, HIST>), grid, dim3(THREADS), 0, st, p);
 }
 
 }  // namespace
@@ -69,10 +143,11 @@ extern "C" int molly_process_logits(void* stream, const void* logits, int logits
     p.rep_v = repetition_rows; p.pres_v = presence_rows; p.freq_v = frequency_rows; p.bias = bias; p.mask = (const unsigned*)allowed;
     p.rep = repetition; p.pres = presence; p.freq = frequency; p.V = V; p.n_hist = n_history;
     p.ldx = ld_logits; p.ldo = ld_out; p.ldg = ld_generated; p.ldb = ld_bias; p.ldm = ld_allowed;
-    constexpr int SLICE = 4096;
-    const dim3 grid(cdiv(V, SLICE), rows);
-    if (logits_bf16) hipLaunchKernelGGL((logits_kernel<SLICE, true>), grid, dim3(256), 0, (hipStream_t)stream, p);
-    else hipLaunchKernelGGL((logits_kernel<SLICE, false>), grid, dim3(256), 0, (hipStream_t)stream, p);
+    // every workgroup reads the row's whole history: long ones are read by fewer, larger workgroups
+    hipStream_t st = (hipStream_t)stream;
+    if (n_history == 0) launch<256, false>(st, p, rows, logits_bf16 != 0);
+    else if (n_history <= LONG_HISTORY) launch<256, true>(st, p, rows, logits_bf16 != 0);
+    else launch<1024, true>(st, p, rows, logits_bf16 != 0);
     MOLLY_LAUNCH_CHECK();
     return 0;
 }

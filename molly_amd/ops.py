@@ -760,52 +760,74 @@ def scale_(x, s: float):
 
 # ---- the paged key / value cache (include/molly_hip.h: molly_paged_kv_*, molly_attn_paged) and the logit processors -----------------------
 # Pools: [n_pages, n_kv_heads, page_size, head_dim] bf16, or float8_e4m3fn with exponent bytes [n_pages, n_kv_heads, page_size] (uint8).
-# These wrappers launch on the current stream of the tensors' own device.
+# These wrappers launch on the current stream of the tensors' own device.  A decode step calls them once a layer for a few microseconds of GPU
+# work each, so the checks read a tensor's shape once and the library is called without a conversion loop.
 E4M3 = torch.float8_e4m3fn
 
 
+def _launch(name, dev, *args):
+    """An entry point on device `dev`'s current stream; pointers as integers or None."""
+    L = lib()
+    if dev == torch.cuda.current_device():
+        rc = L.fn[name](torch._C._cuda_getCurrentRawStream(dev), *args)
+    else:
+        with torch.cuda.device(dev):
+            rc = L.fn[name](torch._C._cuda_getCurrentRawStream(dev), *args)
+    if rc != 0:
+        raise RuntimeError(f"{name} failed (rc={rc}): {L.last_error()}")
+
+
+def _on(t, dev, what, name):
+    """The address of a tensor on device `dev` (None: NULL)."""
+    if t is None:
+        return None
+    if t.get_device() != dev:
+        raise ValueError(f"{what}: {name} is on {t.device}, the others on cuda:{dev}")
+    return t.data_ptr()
+
+
 def _pools(kpool, vpool, kscale, vscale, what):
-    """-> (n_pages, n_kv_heads, page_size, head_dim) of a checked pair of pools."""
-    if not kpool.is_cuda:
+    """-> (device, (n_pages, n_kv_heads, page_size, head_dim), addresses of the four) of a checked pair of pools."""
+    dev, shape, dtype = kpool.get_device(), kpool.shape, kpool.dtype
+    if dev < 0:
         raise RuntimeError(f"molly_amd: {what}: the pools must live on the GPU (no CPU path exists)")
-    if kpool.dim() != 4 or kpool.shape != vpool.shape or kpool.dtype != vpool.dtype:
-        raise ValueError(f"{what}: kpool {tuple(kpool.shape)} {kpool.dtype} and vpool {tuple(vpool.shape)} {vpool.dtype} must be alike, [pages, kv heads, page, dim]")
+    if len(shape) != 4 or shape != vpool.shape or dtype != vpool.dtype:
+        raise ValueError(f"{what}: kpool {tuple(shape)} {dtype} and vpool {tuple(vpool.shape)} {vpool.dtype} must be alike, [pages, kv heads, page, dim]")
     if not (kpool.is_contiguous() and vpool.is_contiguous()):
         raise ValueError(f"{what}: the pools must be contiguous")
-    if kpool.dtype == E4M3:
+    if dtype == E4M3:
         for s in (kscale, vscale):
-            if s is None or s.dtype != torch.uint8 or s.shape != kpool.shape[:3] or not s.is_contiguous():
-                raise ValueError(f"{what}: e4m3 pools need contiguous uint8 exponents of shape {tuple(kpool.shape[:3])} for K and V")
-    elif kpool.dtype != BF16:
-        raise TypeError(f"{what}: pools must be bfloat16 or float8_e4m3fn, got {kpool.dtype}")
+            if s is None or s.dtype != torch.uint8 or s.shape != shape[:3] or not s.is_contiguous():
+                raise ValueError(f"{what}: e4m3 pools need contiguous uint8 exponents of shape {tuple(shape[:3])} for K and V")
+    elif dtype != BF16:
+        raise TypeError(f"{what}: pools must be bfloat16 or float8_e4m3fn, got {dtype}")
     elif kscale is not None or vscale is not None:
         raise ValueError(f"{what}: bf16 pools have no exponents")
-    return kpool.shape
+    return dev, shape, (kpool.data_ptr(), _on(vpool, dev, what, "vpool"), _on(kscale, dev, what, "kscale"), _on(vscale, dev, what, "vscale"))
 
 
-def _same_device(what, dev, *tensors):
-    for t in tensors:
-        if t is not None and t.get_device() != dev:
-            raise ValueError(f"{what}: tensors on different devices ({t.device} and cuda:{dev})")
-
-
-def _rows(t, what, name, width=None):
+def _rows(t, dev, what, name, n, width):
+    """-> (address, row stride) of bf16 rows [n, width]; n None: any number."""
+    shape = t.shape
     if t.dtype != BF16:
         raise TypeError(f"{what}: {name} must be bfloat16, got {t.dtype}")
-    if t.dim() != 2 or (t.stride(1) != 1 and t.shape[1] != 1) or (width is not None and t.shape[1] != width):
-        raise ValueError(f"{what}: {name} must be rows of {width if width is not None else 'heads'} contiguous values, got {tuple(t.shape)} with strides {t.stride()}")
-    if t.stride(0) > 0x7fffffff:
-        raise ValueError(f"{what}: {name} has a row stride of {t.stride(0)} values (32 bits)")
+    if len(shape) != 2 or shape[1] != width or (n is not None and shape[0] != n):
+        raise ValueError(f"{what}: {name} must be [{'n' if n is None else n}, {width}], got {tuple(shape)}")
+    ld, one = t.stride()
+    if one != 1 and width != 1:
+        raise ValueError(f"{what}: the rows of {name} must be contiguous, got strides {t.stride()}")
+    if shape[0] <= 1:
+        ld = (width + 7) // 8 * 8                                 # (one row has no stride, whatever torch says)
+    elif ld > 0x7fffffff:
+        raise ValueError(f"{what}: {name} has a row stride of {ld} values (32 bits)")
+    return _on(t, dev, what, name), ld
 
 
-def _ints(t, what, name, shape=None):
-    if t.dtype != torch.int32 or not t.is_contiguous() or (shape is not None and tuple(t.shape) != shape):
-        raise ValueError(f"{what}: {name} must be contiguous int32{'' if shape is None else ' of shape ' + str(shape)}, got {t.dtype} {tuple(t.shape)}")
-
-
-def _ld(t):
-    """row stride of a 2-D tensor (one row: its width, whatever torch says)"""
-    return t.stride(0) if t.shape[0] > 1 else (t.shape[1] + 7) // 8 * 8
+def _ints(t, dev, what, name, shape):
+    """-> address of a contiguous int32 tensor"""
+    if t.dtype != torch.int32 or t.shape != shape or not t.is_contiguous():
+        raise ValueError(f"{what}: {name} must be contiguous int32 {shape}, got {t.dtype} {tuple(t.shape)}")
+    return _on(t, dev, what, name)
 
 
 def paged_kv_append(k, v, kpool, vpool, slot, kscale=None, vscale=None, q=None, q_out=None, qw=None, kw=None, cos=None, sin=None,
@@ -814,39 +836,37 @@ def paged_kv_append(k, v, kpool, vpool, slot, kscale=None, vscale=None, q=None, 
     q/k-norm (gains qw / kw [dim]) and rotary (cos / sin fp32 [n_pos, dim / 2], positions int32 [n]) of k, and of q [n, heads * dim], in the same
     pass where they are given (molly_paged_kv_append).  Row strides are free.  -> q's rows after both (q_out; q_out may be q), or None."""
     what = "paged_kv_append"
-    P, nkv, page, hd = _pools(kpool, vpool, kscale, vscale, what)
-    n, dev = k.shape[0], kpool.get_device()
-    _rows(k, what, "k", nkv * hd); _rows(v, what, "v", nkv * hd); _ints(slot, what, "slot", (n,))
-    if v.shape[0] != n:
-        raise ValueError(f"{what}: {n} rows of k and {v.shape[0]} of v")
-    nq = 0
+    dev, (P, nkv, page, hd), (kp, vp, ks, vs) = _pools(kpool, vpool, kscale, vscale, what)
+    n = k.shape[0]
+    k_at, ldk = _rows(k, dev, what, "k", None, nkv * hd)
+    v_at, ldv = _rows(v, dev, what, "v", n, nkv * hd)
+    slot_at = _ints(slot, dev, what, "slot", (n,))
+    q_at = qo_at = cos_at = sin_at = pos_at = None
+    nq = ldq = ldqo = n_pos = 0
     if q is not None:
-        _rows(q, what, "q")
-        nq = q.shape[1] // hd
-        if q.shape[0] != n or q.shape[1] % hd or nq == 0:
+        width = q.shape[-1]
+        nq = width // hd
+        if width % hd or nq == 0:
             raise ValueError(f"{what}: q must be [{n}, heads * {hd}], got {tuple(q.shape)}")
+        q_at, ldq = _rows(q, dev, what, "q", n, width)
         if q_out is None:
-            q_out = torch.empty((n, nq * hd), dtype=BF16, device=q.device)
-        _rows(q_out, what, "q_out", nq * hd)
-        if q_out.shape[0] != n:
-            raise ValueError(f"{what}: {n} rows of q and {q_out.shape[0]} of q_out")
+            q_out = torch.empty((n, width), dtype=BF16, device=q.device)
+        qo_at, ldqo = _rows(q_out, dev, what, "q_out", n, width)
     elif q_out is not None or qw is not None:
         raise ValueError(f"{what}: q_out / qw without q")
     for w in (qw, kw):
-        if w is not None and (w.dtype != BF16 or tuple(w.shape) != (hd,) or not w.is_contiguous()):
+        if w is not None and (w.dtype != BF16 or w.shape != (hd,) or not w.is_contiguous()):
             raise ValueError(f"{what}: gains must be contiguous bfloat16 [{hd}]")
-    if (cos is None) != (sin is None) or (cos is None) != (positions is None):
-        raise ValueError(f"{what}: cos, sin and positions go together")
-    if cos is not None:
+    if cos is not None and sin is not None and positions is not None:
         for c in (cos, sin):
             if c.dtype != torch.float32 or c.dim() != 2 or c.shape != cos.shape or c.shape[1] != hd // 2 or not c.is_contiguous():
                 raise ValueError(f"{what}: cos / sin must be contiguous float32 [n_pos, {hd // 2}]")
-        _ints(positions, what, "positions", (n,))
-    _same_device(what, dev, k, v, vpool, slot, kscale, vscale, q, q_out, qw, kw, cos, sin, positions)
-    with torch.cuda.device(dev):
-        lib().call("molly_paged_kv_append", _stream(), k, v, q, q_out, kpool, vpool, kscale, vscale, slot, n, P, page, nq, nkv, hd,
-                   _ld(q) if nq else 0, _ld(k), _ld(v), _ld(q_out) if nq else 0, qw, kw, cos, sin, positions, cos.shape[0] if cos is not None else 0,
-                   float(eps))
+        pos_at = _ints(positions, dev, what, "positions", (n,))
+        cos_at, sin_at, n_pos = _on(cos, dev, what, "cos"), _on(sin, dev, what, "sin"), cos.shape[0]
+    elif not (cos is None and sin is None and positions is None):
+        raise ValueError(f"{what}: cos, sin and positions go together")
+    _launch("molly_paged_kv_append", dev, k_at, v_at, q_at, qo_at, kp, vp, ks, vs, slot_at, n, P, page, nq, nkv, hd, ldq, ldk, ldv, ldqo,
+            _on(qw, dev, what, "qw"), _on(kw, dev, what, "kw"), cos_at, sin_at, pos_at, n_pos, eps)
     return q_out
 
 
@@ -854,27 +874,22 @@ def paged_kv_read(kpool, vpool, slot, kscale=None, vscale=None, k_out=None, v_ou
     """The rows of the places slot (int32 [n]) back as bf16 [n, kv heads * dim] each (molly_paged_kv_read); a slot outside the pool: zeros.
     -> (k, v)"""
     what = "paged_kv_read"
-    P, nkv, page, hd = _pools(kpool, vpool, kscale, vscale, what)
-    _ints(slot, what, "slot")
-    if slot.dim() != 1:
-        raise ValueError(f"{what}: slot must be [n], got {tuple(slot.shape)}")
-    n, dev = slot.shape[0], kpool.get_device()
+    dev, (P, nkv, page, hd), (kp, vp, ks, vs) = _pools(kpool, vpool, kscale, vscale, what)
+    n = slot.shape[0] if slot.dim() == 1 else -1
+    slot_at = _ints(slot, dev, what, "slot", (n,))
     if k_out is None:
         k_out = torch.empty((n, nkv * hd), dtype=BF16, device=kpool.device)
     if v_out is None:
         v_out = torch.empty((n, nkv * hd), dtype=BF16, device=kpool.device)
-    _rows(k_out, what, "k_out", nkv * hd); _rows(v_out, what, "v_out", nkv * hd)
-    if k_out.shape[0] != n or v_out.shape[0] != n:
-        raise ValueError(f"{what}: {n} slots, {k_out.shape[0]} / {v_out.shape[0]} output rows")
-    _same_device(what, dev, vpool, slot, kscale, vscale, k_out, v_out)
-    with torch.cuda.device(dev):
-        lib().call("molly_paged_kv_read", _stream(), kpool, vpool, kscale, vscale, slot, n, P, page, nkv, hd, k_out, v_out, _ld(k_out), _ld(v_out))
+    k_at, ldk = _rows(k_out, dev, what, "k_out", n, nkv * hd)
+    v_at, ldv = _rows(v_out, dev, what, "v_out", n, nkv * hd)
+    _launch("molly_paged_kv_read", dev, kp, vp, ks, vs, slot_at, n, P, page, nkv, hd, k_at, v_at, ldk, ldv)
     return k_out, v_out
 
 
 def attn_paged_workspace(n_tokens, B, n_heads, n_kv_heads, head_dim, page_size, max_pages, e4m3, max_q=0, max_kv=0) -> int:
     """fp32 elements of scratch that an attn_paged of these sizes can use (0: none)"""
-    return lib().query("molly_attn_paged_workspace", n_tokens, B, n_heads, n_kv_heads, head_dim, page_size, max_pages, int(e4m3), max_q, max_kv)
+    return lib().fn["molly_attn_paged_workspace"](n_tokens, B, n_heads, n_kv_heads, head_dim, page_size, max_pages, int(e4m3), max_q, max_kv)
 
 
 def attn_paged(q, kpool, vpool, block_table, cu_q, kv_len, n_heads, scale=None, kscale=None, vscale=None, max_q=0, max_kv=0, out=None,
@@ -885,33 +900,38 @@ def attn_paged(q, kpool, vpool, block_table, cu_q, kv_len, n_heads, scale=None, 
     far as the caller knows; they only choose how the work is cut (0: n_tokens / what the table can hold).  workspace: float32 scratch of
     attn_paged_workspace(..) elements (None: the call takes its own).  -> out [n_tokens, n_heads * dim]"""
     what = "attn_paged"
-    P, nkv, page, hd = _pools(kpool, vpool, kscale, vscale, what)
-    n_heads = int(n_heads)
-    dev = kpool.get_device()
+    dev, (P, nkv, page, hd), (kp, vp, ks, vs) = _pools(kpool, vpool, kscale, vscale, what)
     if n_heads <= 0 or n_heads % nkv:
         raise ValueError(f"{what}: {n_heads} heads are not a multiple of {nkv} kv heads")
-    _rows(q, what, "q", n_heads * hd)
-    if block_table.dim() != 2 or block_table.dtype != torch.int32 or (block_table.stride(1) != 1 and block_table.shape[1] != 1):
+    q_at, ldq = _rows(q, dev, what, "q", None, n_heads * hd)
+    n = q.shape[0]
+    if block_table.dtype != torch.int32 or block_table.dim() != 2 or (block_table.shape[1] > 1 and block_table.stride(1) != 1):
         raise ValueError(f"{what}: block_table must be int32 [B, max_pages] with contiguous rows, got {block_table.dtype} {tuple(block_table.shape)}")
     B, max_pages = block_table.shape
-    _ints(cu_q, what, "cu_q", (B + 1,)); _ints(kv_len, what, "kv_len", (B,))
-    n = q.shape[0]
+    cu_at, len_at, table_at = _ints(cu_q, dev, what, "cu_q", (B + 1,)), _ints(kv_len, dev, what, "kv_len", (B,)), _on(block_table, dev, what, "block_table")
     if out is None:
         out = torch.empty((n, n_heads * hd), dtype=BF16, device=q.device)
-    _rows(out, what, "out", n_heads * hd)
-    if out.shape[0] != n:
-        raise ValueError(f"{what}: {n} rows of q and {out.shape[0]} of out")
+    out_at, ldo = _rows(out, dev, what, "out", n, n_heads * hd)
     if workspace is None:
-        floats = attn_paged_workspace(n, B, n_heads, nkv, hd, page, max_pages, kscale is not None, max_q, max_kv)
-        workspace = torch.empty(floats, dtype=torch.float32, device=q.device) if floats else None
-    elif workspace.dtype != torch.float32 or not workspace.is_contiguous():
-        raise ValueError(f"{what}: workspace must be contiguous float32")
-    _same_device(what, dev, q, vpool, kscale, vscale, block_table, cu_q, kv_len, out, workspace)
-    with torch.cuda.device(dev):
-        lib().call("molly_attn_paged", _stream(), q, out, kpool, vpool, kscale, vscale, block_table, cu_q, kv_len, n, B, P, page, max_pages,
-                   block_table.stride(0) if B > 1 else max_pages, n_heads, nkv, hd, _ld(q), _ld(out), float(hd ** -0.5 if scale is None else scale),
-                   max_q, max_kv, workspace, workspace.numel() if workspace is not None else 0)
+        floats = attn_paged_workspace(n, B, n_heads, nkv, hd, page, max_pages, ks is not None, max_q, max_kv)
+        ws = torch.empty(floats, dtype=torch.float32, device=q.device) if floats else None
+    else:
+        ws, floats = workspace, workspace.numel()
+        if ws.dtype != torch.float32 or not ws.is_contiguous():
+            raise ValueError(f"{what}: workspace must be contiguous float32")
+    _launch("molly_attn_paged", dev, q_at, out_at, kp, vp, ks, vs, table_at, cu_at, len_at, n, B, P, page, max_pages,
+            block_table.stride(0) if B > 1 else max_pages, n_heads, nkv, hd, ldq, ldo, hd ** -0.5 if scale is None else scale, max_q, max_kv,
+            _on(ws, dev, what, "workspace"), floats)
     return out
+
+
+def _vocab_rows(t, dev, what, name, dtype, rows, width):
+    """-> (address, row stride) of [width] (stride 0: one row for all) or [rows, width]; None: (NULL, 0)."""
+    if t is None:
+        return None, 0
+    if t.dtype != dtype or t.shape not in ((width,), (rows, width)) or (t.stride(-1) != 1 and width != 1):
+        raise ValueError(f"{what}: {name} must be {dtype} [{width}] or [{rows}, {width}] with contiguous rows, got {t.dtype} {tuple(t.shape)}")
+    return _on(t, dev, what, name), t.stride(0) if t.dim() == 2 and rows > 1 else 0
 
 
 def process_logits(logits, generated=None, n_generated=None, repetition_penalty=1.0, presence_penalty=0.0, frequency_penalty=0.0, bias=None,
@@ -922,43 +942,42 @@ def process_logits(logits, generated=None, n_generated=None, repetition_penalty=
     (fp32 [V] or [rows, V]); then -inf where a token is not allowed (`allowed`: int32 bits [ceil(V / 32)] or [rows, ceil(V / 32)], bit v % 32 of
     word v // 32).  The penalties: numbers, or fp32 [rows]."""
     what = "process_logits"
-    if not logits.is_cuda:
+    dev, dtype = logits.get_device(), logits.dtype
+    if dev < 0:
         raise RuntimeError(f"molly_amd: {what}: logits must live on the GPU (no CPU path exists)")
-    if logits.dim() != 2 or logits.dtype not in (torch.float32, BF16) or (logits.stride(1) != 1 and logits.shape[1] != 1):
-        raise ValueError(f"{what}: logits must be float32 or bfloat16 [rows, V] with contiguous rows, got {logits.dtype} {tuple(logits.shape)}")
+    if logits.dim() != 2 or dtype not in (torch.float32, BF16) or (logits.stride(1) != 1 and logits.shape[1] != 1):
+        raise ValueError(f"{what}: logits must be float32 or bfloat16 [rows, V] with contiguous rows, got {dtype} {tuple(logits.shape)}")
     rows, V = logits.shape
-    dev = logits.get_device()
     if out is None:
         out = torch.empty((rows, V), dtype=torch.float32, device=logits.device)
-    if out.dtype != torch.float32 or out.shape != logits.shape or (out.stride(1) != 1 and V != 1):
+    elif out.dtype != torch.float32 or out.shape != logits.shape or (out.stride(1) != 1 and V != 1):
         raise ValueError(f"{what}: out must be float32 {tuple(logits.shape)} with contiguous rows")
-    if rows > 1 and (logits.stride(0) < V or out.stride(0) < V):
-        raise ValueError(f"{what}: rows of logits / out overlap (strides {logits.stride(0)} / {out.stride(0)}, {V} tokens)")
-    n_hist = 0
+    ldx, ldo = (logits.stride(0), out.stride(0)) if rows > 1 else (V, V)
+    if ldx < V or ldo < V:
+        raise ValueError(f"{what}: rows of logits / out overlap (strides {ldx} / {ldo}, {V} tokens)")
+    gen_at = n_at = None
+    n_hist = ldg = 0
     if generated is not None:
-        if generated.dtype != torch.int64 or generated.dim() != 2 or generated.shape[0] != rows or (generated.stride(1) != 1 and generated.shape[1] > 1):
+        if generated.dtype != torch.int64 or generated.dim() != 2 or generated.shape[0] != rows or (generated.shape[1] > 1 and generated.stride(1) != 1):
             raise ValueError(f"{what}: generated must be int64 [{rows}, n] with contiguous rows")
         n_hist = generated.shape[1]
         if n_generated is not None:
-            _ints(n_generated, what, "n_generated", (rows,))
+            n_at = _ints(n_generated, dev, what, "n_generated", (rows,))
+        gen_at, ldg = _on(generated, dev, what, "generated"), generated.stride(0) if rows > 1 else n_hist
     elif n_generated is not None:
         raise ValueError(f"{what}: n_generated without generated")
-    pen, pen_rows = [], []
+    pen, pen_at = [], []
     for name, x in (("repetition_penalty", repetition_penalty), ("presence_penalty", presence_penalty), ("frequency_penalty", frequency_penalty)):
-        if torch.is_tensor(x):
-            if x.dtype != torch.float32 or tuple(x.shape) != (rows,) or not x.is_contiguous():
+        if isinstance(x, torch.Tensor):
+            if x.dtype != torch.float32 or x.shape != (rows,) or not x.is_contiguous():
                 raise ValueError(f"{what}: {name} must be a number or contiguous float32 [{rows}]")
-            pen.append(1.0); pen_rows.append(x)
+            pen.append(1.0)
+            pen_at.append(_on(x, dev, what, name))
         else:
-            pen.append(float(x)); pen_rows.append(None)
-    for name, x, dt, w in (("bias", bias, torch.float32, V), ("allowed", allowed, torch.int32, (V + 31) // 32)):
-        if x is not None and (x.dtype != dt or tuple(x.shape) not in ((w,), (rows, w)) or (x.stride(-1) != 1 and w != 1)):
-            raise ValueError(f"{what}: {name} must be {dt} [{w}] or [{rows}, {w}] with contiguous rows, got {x.dtype} {tuple(x.shape)}")
-    _same_device(what, dev, out, generated, n_generated, bias, allowed, *pen_rows)
-    one = lambda t: t.stride(0) if t is not None and t.dim() == 2 and t.shape[0] > 1 else 0  # noqa: E731
-    with torch.cuda.device(dev):
-        lib().call("molly_process_logits", _stream(), logits, int(logits.dtype == BF16), out, rows, V, logits.stride(0) if rows > 1 else V,
-                   out.stride(0) if rows > 1 else V, generated if n_hist else None, n_generated if n_hist else None, n_hist,
-                   (generated.stride(0) if rows > 1 else n_hist) if n_hist else 0, pen[0], pen[1], pen[2], *pen_rows, bias, one(bias), allowed,
-                   one(allowed))
+            pen.append(x)
+            pen_at.append(None)
+    bias_at, ldb = _vocab_rows(bias, dev, what, "bias", torch.float32, rows, V)
+    allowed_at, ldm = _vocab_rows(allowed, dev, what, "allowed", torch.int32, rows, (V + 31) // 32)
+    _launch("molly_process_logits", dev, logits.data_ptr(), dtype == BF16, _on(out, dev, what, "out"), rows, V, ldx, ldo, gen_at, n_at, n_hist, ldg,
+            *pen, *pen_at, bias_at, ldb, allowed_at, ldm)
     return out

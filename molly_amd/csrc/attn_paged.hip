@@ -13,8 +13,6 @@
 // Either cuts the key axis over blocks where there are too few tiles to fill the chip; attn_paged_merge_kernel joins the parts.
 // A bf16 step's rows go straight to LDS by DMA (16 keys lie within one page, so one page id serves a wave's piece); e4m3 codes pass through registers,
 // are turned into bf16 there (exact) and stored into the same image: one set of fragment reads serves both.
-#include <stdlib.h>
-
 #include "attn_frag.h"
 #include "common.h"
 #include "molly_hip.h"
@@ -22,8 +20,8 @@
 
 namespace {
 
-constexpr int RROWS = 32;                            // rows of a tile in the rows kernel; the tile kernel has 128 * RB
-constexpr int MIN_KEYS_ROWS = 256, MIN_KEYS_TILE = 512;      // fewest keys that a part of a cut key axis gets
+constexpr int RROWS = 32;                            // rows of a tile in the rows kernel; the tile kernel has 32 a wave
+constexpr int MIN_KEYS = 512;                        // fewest keys that a part of a cut key axis gets
 constexpr int MAX_PARTS = 64;
 
 struct AttnPagedArgs {
@@ -56,7 +54,7 @@ __device__ __forceinline__ Tile make_tile(const AttnPagedArgs& p, int b, int ti)
     return t;
 }
 // parts that a tile's key axis is cut into, and a part's keys (whole steps of ALIGN)
-__device__ __forceinline__ int parts_of(int n_keys, int parts, int min_keys) { return min(parts, max(n_keys / min_keys, 1)); }
+__device__ __forceinline__ int parts_of(int n_keys, int parts) { return min(parts, max(n_keys / MIN_KEYS, 1)); }
 template <int ALIGN> __device__ __forceinline__ int part_keys(int n_keys, int parts) { return ((n_keys + parts - 1) / parts + ALIGN - 1) / ALIGN * ALIGN; }
 
 // ---- K / V steps ------------------------------------------------------------------------------------------------------------------------
@@ -71,9 +69,10 @@ struct KvSource {
     }
 };
 
-// one 16-key group (rows 16 g .. of a tile image) by LDS-DMA: NPG pieces of 1 KiB per matrix.  `off`: the lane's byte offsets (group_offsets).
-template <int HD> constexpr int NPG = HD / 32;
-template <int HD> __device__ __forceinline__ void piece_row_col(int i, int lane, int& row, int& col) {
+// R (16 | 8) rows of a 16-key group, from row `r0` of the tile image on, by LDS-DMA: PIECES of 1 KiB per matrix.  `off`: the lane's byte offsets from the
+// group's first row (piece_row_col); `lds`: where the piece's rows start in the image.
+template <int HD, int R> constexpr int PIECES = R * HD / 512;
+template <int HD> __device__ __forceinline__ void piece_row_col(int i, int lane, int& row, int& col) {      // piece i of a group
     constexpr int NCB = HD / 16;
     const int blk = lane >> 3, cin = lane & 7, rbl = i * (8 / NCB) + blk / NCB, b0 = rbl & 1, b1 = (rbl >> 1) & 1;
     row = rbl * 4 + (cin >> 1);
@@ -83,54 +82,64 @@ __device__ __forceinline__ void dma16(unsigned off, const char* base, unsigned l
     // (from asm, as in attention.hip: with the builtin hipcc waits for every pending LDS-DMA in front of the next transposed read)
     asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(off), "s"(base), "s"(lds) : "memory", "m0");
 }
-template <int HD>
-__device__ __forceinline__ void dma_group(const char* base, unsigned lds, const unsigned (&off)[NPG<HD>]) {
+template <int HD, int R>
+__device__ __forceinline__ void piece_offsets(int r0, int lane, unsigned (&off)[PIECES<HD, R>]) {
 #pragma unroll
-    for (int i = 0; i < NPG<HD>; ++i) dma16(off[i], base, __builtin_amdgcn_readfirstlane(lds + i * 1024));
+    for (int i = 0; i < PIECES<HD, R>; ++i) {
+        int row, col;
+        piece_row_col<HD>((r0 & 15) * HD / 512 + i, lane, row, col);
+        off[i] = (unsigned)((row * HD + col) * 2);
+    }
+}
+template <int N>
+__device__ __forceinline__ void dma_rows(const char* base, unsigned lds, const unsigned (&off)[N]) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) dma16(off[i], base, __builtin_amdgcn_readfirstlane(lds + i * 1024));
 }
 // the same for the group that the last key is in (or lies in front of): rows behind it repeat it, so that nothing behind a sequence's end — stale
 // pages may hold NaN — gets into the tile
-template <int HD>
-__device__ __forceinline__ void dma_group_clamped(const char* base, unsigned lds, int lim, int lane) {
+template <int HD, int R>
+__device__ __forceinline__ void dma_rows_clamped(const char* base, unsigned lds, int r0, int lim, int lane) {
 #pragma unroll
-    for (int i = 0; i < NPG<HD>; ++i) {
+    for (int i = 0; i < PIECES<HD, R>; ++i) {
         int row, col;
-        piece_row_col<HD>(i, lane, row, col);
+        piece_row_col<HD>((r0 & 15) * HD / 512 + i, lane, row, col);
         dma16((unsigned)((min(row, lim) * HD + col) * 2), base, __builtin_amdgcn_readfirstlane(lds + i * 1024));
     }
 }
+template <int N> __device__ __forceinline__ void wait_vm() { asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory"); }
 
-// one 16-key group of e4m3 codes through registers: NL loads of 16 codes a lane and matrix
-template <int HD> constexpr int NL = HD / 64;
-template <int HD> struct Codes {
-    u32x4 k[NL<HD>], v[NL<HD>];
-    uint8_t ke[NL<HD>], ve[NL<HD>];
+// R rows of a 16-key group as e4m3 codes through registers: NL loads of 16 codes a lane, K's units first, then V's.  Lanes go over the 4 rows of a block
+// first: the stores into the image are free of bank conflicts.
+template <int HD, int R> struct Codes {
+    static constexpr int UPM = R * HD / 16, NL = 2 * UPM / 64;       // units of 16 codes per matrix; loads a lane
+    u32x4 c[NL];
+    uint8_t e[NL];
 };
-template <int HD>
-__device__ __forceinline__ void codes_load(Codes<HD>& c, const AttnPagedArgs& p, size_t at, int lim, int lane) {
-    constexpr int NCB = HD / 16, LRB = NCB * 4;      // lanes of a 4-row block: 4 rows on the low lane bits (conflict-free LDS stores), 16 codes each
+template <int HD, int R>
+__device__ __forceinline__ void codes_load(Codes<HD, R>& c, const AttnPagedArgs& p, size_t at, int r0, int lim, int lane) {
+    constexpr int NCB = HD / 16, LRB = NCB * 4, UPM = Codes<HD, R>::UPM;
 #pragma unroll
-    for (int j = 0; j < NL<HD>; ++j) {
-        const int row = min((j * (64 / LRB) + lane / LRB) * 4 + (lane & 3), lim), cb = (lane >> 2) & (NCB - 1);
+    for (int j = 0; j < Codes<HD, R>::NL; ++j) {
+        const int u = j * 64 + lane, w = u % UPM;
+        const bool isv = u >= UPM;
+        const int row = min((r0 & 15) + w / LRB * 4 + (w & 3), lim), cb = (w >> 2) & (NCB - 1);
         const size_t key = at + row;
-        c.k[j] = *reinterpret_cast<const u32x4*>(p.kpool + key * HD + cb * 16);
-        c.v[j] = *reinterpret_cast<const u32x4*>(p.vpool + key * HD + cb * 16);
-        c.ke[j] = p.kscale[key];
-        c.ve[j] = p.vscale[key];
+        c.c[j] = *reinterpret_cast<const u32x4*>((isv ? p.vpool : p.kpool) + key * HD + cb * 16);
+        c.e[j] = (isv ? p.vscale : p.kscale)[key];
     }
 }
-template <int HD>
-__device__ __forceinline__ void codes_store(const Codes<HD>& c, bf16_t* imgk, bf16_t* imgv, int lane) {      // images of the group's 16 rows
-    constexpr int NCB = HD / 16, LRB = NCB * 4;
+template <int HD, int R>
+__device__ __forceinline__ void codes_store(const Codes<HD, R>& c, bf16_t* imgk, bf16_t* imgv, int r0, int lane) {      // the tile's images
+    constexpr int NCB = HD / 16, LRB = NCB * 4, UPM = Codes<HD, R>::UPM;
 #pragma unroll
-    for (int j = 0; j < NL<HD>; ++j) {
-        const int rbl = j * (64 / LRB) + lane / LRB, cb = (lane >> 2) & (NCB - 1), q = lane & 3, b0 = rbl & 1, b1 = (rbl >> 1) & 1;
-        const int o = (rbl * NCB + (cb ^ b0)) * 64 + q * 16;
-        const float ks = exp2i((int)c.ke[j] - 127), vs = exp2i((int)c.ve[j] - 127);
-        *reinterpret_cast<u32x4*>(imgk + o + b1 * 8) = e4m3_to_bf8(u32x2{c.k[j][0], c.k[j][1]}, ks);
-        *reinterpret_cast<u32x4*>(imgk + o + (b1 ^ 1) * 8) = e4m3_to_bf8(u32x2{c.k[j][2], c.k[j][3]}, ks);
-        *reinterpret_cast<u32x4*>(imgv + o + b1 * 8) = e4m3_to_bf8(u32x2{c.v[j][0], c.v[j][1]}, vs);
-        *reinterpret_cast<u32x4*>(imgv + o + (b1 ^ 1) * 8) = e4m3_to_bf8(u32x2{c.v[j][2], c.v[j][3]}, vs);
+    for (int j = 0; j < Codes<HD, R>::NL; ++j) {
+        const int u = j * 64 + lane, w = u % UPM;
+        const int rbl = (r0 >> 2) + w / LRB, cb = (w >> 2) & (NCB - 1), b0 = rbl & 1, b1 = (rbl >> 1) & 1;
+        bf16_t* d = (u >= UPM ? imgv : imgk) + (rbl * NCB + (cb ^ b0)) * 64 + (w & 3) * 16;
+        const float scale = exp2i((int)c.e[j] - 127);
+        *reinterpret_cast<u32x4*>(d + b1 * 8) = e4m3_to_bf8(u32x2{c.c[j][0], c.c[j][1]}, scale);
+        *reinterpret_cast<u32x4*>(d + (b1 ^ 1) * 8) = e4m3_to_bf8(u32x2{c.c[j][2], c.c[j][3]}, scale);
     }
 }
 
@@ -164,11 +173,11 @@ __device__ __forceinline__ void rows_init(Rows<HD>& st, const AttnPagedArgs& p, 
 // V values that are not finite, in a step that some row does not see all of: P is 0 there, and 0 * NaN would be NaN.  attend32 takes them out of such
 // a step (clear_odd) and this adds them to the rows that do see them, at the end.  step0, step0 + stride ..: the wave's steps below k1.
 template <int HD, bool FP8>
-__device__ __forceinline__ void add_odd(Rows<HD>& st, int qmin, const AttnPagedArgs& p, const KvSource& src, int step0, int stride, int k1, int lane) {
+__device__ __forceinline__ void add_odd(Rows<HD>& st, const AttnPagedArgs& p, const KvSource& src, int step0, int stride, int k1, int lane) {
     const int h = lane >> 5;
 #pragma unroll 1
     for (int kb = step0; kb < k1; kb += stride) {
-        if (kb + 31 <= qmin) continue;                // (every row saw these: they went through the product)
+        if (kb + 31 <= st.qmin) continue;                // (every row saw these: they went through the product)
 #pragma unroll 1
         for (int key = kb; key < min(kb + 32, k1); ++key) {
             const size_t at = src.group(key, src.row[key >> src.shift]) + (key & 15);
@@ -227,80 +236,75 @@ __device__ __forceinline__ bool clear_odd(bf16x8 (&vf)[2][ND]) {
     return true;
 }
 
-// one step of 32 keys: rows `sub` * 32 .. of the images, keys kbase ..  RB blocks of 32 query rows share the K and V fragments.
-template <int HD, int RB>
-__device__ __forceinline__ void attend32(Rows<HD> (&st)[RB], const bf16_t* sK, const bf16_t* sV, int sub, int kbase, float scale_log2, int lane) {
+// one step of 32 keys: rows `sub` * 32 .. of the images, keys kbase ..
+template <int HD>
+__device__ __forceinline__ void attend32(Rows<HD>& st, const bf16_t* sK, const bf16_t* sV, int sub, int kbase, float scale_log2, int lane) {
     constexpr int NS = HD / 16, ND = HD / 32;
     const int r = lane & 31, h = lane >> 5;
     bf16x8 kf[NS];
 #pragma unroll
     for (int s = 0; s < NS; ++s) kf[s] = row_frag<HD>(sK, 32 * sub + r, s, h);
     __builtin_amdgcn_sched_barrier(0);               // every read in flight before the first MFMA
-    f32x16 sc[RB];
+    f32x16 sc;
 #pragma unroll
-    for (int b = 0; b < RB; ++b) {
+    for (int e = 0; e < 16; ++e) sc[e] = 0.f;
 #pragma unroll
-        for (int e = 0; e < 16; ++e) sc[b][e] = 0.f;
-#pragma unroll
-        for (int s = 0; s < NS; ++s) sc[b] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kf[s], st[b].qf[s], sc[b], 0, 0, 0);
-    }
+    for (int s = 0; s < NS; ++s) sc = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kf[s], st.qf[s], sc, 0, 0, 0);
     bf16x8 vf[2][ND];
 #pragma unroll
     for (int sp = 0; sp < 2; ++sp)
 #pragma unroll
         for (int d = 0; d < ND; ++d) vf[sp][d] = tr_frag<HD>(sV, 32 * sub, sp, d, lane);
-    const bool edge = kbase + 31 > st[0].qmin;       // (uniform) some row does not see all of the step
+    const bool edge = kbase + 31 > st.qmin;          // (uniform) some row does not see all of the step
     if (edge) {
 #pragma unroll
-        for (int b = 0; b < RB; ++b)
-#pragma unroll
-            for (int e = 0; e < 16; ++e) {
-                const int key = kbase + (e & 3) + 8 * (e >> 2) + 4 * h;
-                sc[b][e] = key <= st[b].qi ? sc[b][e] : -INFINITY;
-            }
-        if (clear_odd<ND>(vf)) st[0].odd = true;
+        for (int e = 0; e < 16; ++e) {
+            const int key = kbase + (e & 3) + 8 * (e >> 2) + 4 * h;
+            sc[e] = key <= st.qi ? sc[e] : -INFINITY;
+        }
+        if (clear_odd<ND>(vf)) st.odd = true;
     }
+    float mx = -INFINITY;
 #pragma unroll
-    for (int b = 0; b < RB; ++b) {
-        float mx = -INFINITY;
+    for (int e = 0; e < 16; ++e) mx = fmaxf(mx, sc[e]);
+    mx = xhalf_max(mx) * scale_log2;
+    if (!__all(mx - st.m <= RESCALE_THR)) {          // the reference maximum follows only where it has grown by more than 2^8
+        const float m_new = fmaxf(st.m, mx);
+        const float alpha = fast_exp2(st.m - (m_new == -INFINITY ? 0.f : m_new));
+        st.l *= alpha;
+        st.m = m_new;
 #pragma unroll
-        for (int e = 0; e < 16; ++e) mx = fmaxf(mx, sc[b][e]);
-        mx = xhalf_max(mx) * scale_log2;
-        if (!__all(mx - st[b].m <= RESCALE_THR)) {   // the reference maximum follows only where it has grown by more than 2^8
-            const float m_new = fmaxf(st[b].m, mx);
-            const float alpha = fast_exp2(st[b].m - (m_new == -INFINITY ? 0.f : m_new));
-            st[b].l *= alpha;
-            st[b].m = m_new;
+        for (int d = 0; d < ND; ++d)
 #pragma unroll
-            for (int d = 0; d < ND; ++d)
+            for (int e = 0; e < 16; ++e) st.o[d][e] *= alpha;
+    }
+    const float m_ref = st.m == -INFINITY ? 0.f : st.m;
 #pragma unroll
-                for (int e = 0; e < 16; ++e) st[b].o[d][e] *= alpha;
-        }
-        const float m_ref = st[b].m == -INFINITY ? 0.f : st[b].m;
+    for (int e = 0; e < 16; ++e) sc[e] = fast_exp2(sc[e] * scale_log2 - m_ref);
+    float rs[4];
 #pragma unroll
-        for (int e = 0; e < 16; ++e) sc[b][e] = fast_exp2(sc[b][e] * scale_log2 - m_ref);
-        float rs[4];
+    for (int g = 0; g < 4; ++g) rs[g] = (sc[4 * g] + sc[4 * g + 1]) + (sc[4 * g + 2] + sc[4 * g + 3]);
+    st.l += (rs[0] + rs[1]) + (rs[2] + rs[3]);
+    const bf16x8 pf[2] = {acc_to_frag(sc, 0), acc_to_frag(sc, 8)};
 #pragma unroll
-        for (int g = 0; g < 4; ++g) rs[g] = (sc[b][4 * g] + sc[b][4 * g + 1]) + (sc[b][4 * g + 2] + sc[b][4 * g + 3]);
-        st[b].l += (rs[0] + rs[1]) + (rs[2] + rs[3]);
-        const bf16x8 pf[2] = {acc_to_frag(sc[b], 0), acc_to_frag(sc[b], 8)};
-#pragma unroll
-        for (int d = 0; d < ND; ++d) {
-            st[b].o[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vf[0][d], pf[0], st[b].o[d], 0, 0, 0);
-            st[b].o[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vf[1][d], pf[1], st[b].o[d], 0, 0, 0);
-        }
+    for (int d = 0; d < ND; ++d) {
+        st.o[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vf[0][d], pf[0], st.o[d], 0, 0, 0);
+        st.o[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vf[1][d], pf[1], st.o[d], 0, 0, 0);
     }
 }
 
 // the first of the keys k0 .. k1 - 1 that lies on a page that is none, by all threads of the block (0x7fffffff: all pages are); *sh is set
 // behind the next barrier
+template <int THREADS>
 __device__ __forceinline__ void scan_pages(const AttnPagedArgs& p, const int* row, int k0, int k1, int* sh) {
     const int last = k1 > k0 ? (k1 - 1) >> p.page_shift : -1;
-    for (int i = (k0 >> p.page_shift) + threadIdx.x; i <= last; i += 256)
+    for (int i = (k0 >> p.page_shift) + threadIdx.x; i <= last; i += THREADS)
         if ((unsigned)row[i] >= (unsigned)p.n_pages) atomicMin(sh, i << p.page_shift);
 }
 
-// ---- short chunks: one tile of up to 32 rows a block, its waves take every fourth step --------------------------------------------------------
+// ---- short chunks: tiles of up to 32 rows; a block's four waves take every fourth step of 32 keys ----------------------------------------------------
+// (Cutting all sequences' keys into equal shares, whatever tiles they belong to, was measured too: 45.7 us against 45.8 for 32 x 1,000..4,000
+// keys, and 64.5 against 57.2 where all are 4,000 long: finding a share's place and a second tile per block cost what the balance gains.)
 template <int HD, bool FP8>
 __global__ __launch_bounds__(256, (HD == 128 && !FP8) ? 1 : 2) void attn_paged_rows_kernel(AttnPagedArgs p) {
     extern __shared__ __attribute__((aligned(16))) char smem[];
@@ -309,32 +313,28 @@ __global__ __launch_bounds__(256, (HD == 128 && !FP8) ? 1 : 2) void attn_paged_r
     constexpr int IMG = 32 * HD;                     // elements of a step's K (or V) image
     constexpr int NBUF = FP8 ? 1 : 2;
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    bf16_t* img = reinterpret_cast<bf16_t*>(smem) + wave * NBUF * 2 * IMG;            // [buffer][K | V]
+    const unsigned img_lds = __builtin_amdgcn_readfirstlane((unsigned)(uintptr_t)LDS_PTR(img));
+    unsigned off[PIECES<HD, 16>];
+    piece_offsets<HD, 16>(0, lane, off);
     int bid = blockIdx.x;
     const int s = bid % p.parts; bid /= p.parts;
     const int kvh = bid % p.nkv; bid /= p.nkv;
     const int b = bid / p.tps;
-    bf16_t* img = reinterpret_cast<bf16_t*>(smem) + wave * NBUF * 2 * IMG;            // [buffer][K | V]
-    const unsigned img_lds = __builtin_amdgcn_readfirstlane((unsigned)(uintptr_t)LDS_PTR(img));
-    unsigned off[NPG<HD>];
-#pragma unroll
-    for (int i = 0; i < NPG<HD>; ++i) {
-        int row, col;
-        piece_row_col<HD>(i, lane, row, col);
-        off[i] = (unsigned)((row * HD + col) * 2);
-    }
     for (int ti = bid % p.tps;; ti += p.tps) {       // (a sequence has more tiles than p.tps only where the caller's max_q was too small)
         const Tile t = make_tile<RROWS>(p, b, ti);
         if (t.rows <= 0) return;
         const int kmax = p.max_pages << p.page_shift;
         const int n_keys = min(t.n_vis, kmax);
-        const int parts = ti < p.tps ? parts_of(n_keys, p.parts, MIN_KEYS_ROWS) : 1;
+        const int parts = ti < p.tps ? parts_of(n_keys, p.parts) : 1;
         if (s >= parts) continue;
         const int chunk = part_keys<128>(n_keys, parts);
-        const int k0 = s * chunk, k1 = min(n_keys, k0 + chunk), last = k1 - 1;
-        const KvSource src{p.table + (size_t)b * p.ld_table, p.n_pages, p.page_shift, p.nkv, kvh};
+        const int k0 = s * chunk, k1 = min(n_keys, k0 + chunk);
+        float* part = parts > 1 ? p.part + ((size_t)((b * p.tps + ti) * p.nkv + kvh) * p.parts + s) * (RROWS * (HD + 2)) : nullptr;
+        const int last = k1 - 1;
+        const KvSource src{p.table + (size_t)t.b * p.ld_table, p.n_pages, p.page_shift, p.nkv, kvh};
         if (tid == 0) s_bad = t.n_vis > kmax ? kmax : 0x7fffffff;
-        Rows<HD> rows[1];
-        Rows<HD>& st = rows[0];
+        Rows<HD> st;
         rows_init<HD>(st, p, t, kvh, 0, lane);
         const int key0 = k0 + 32 * wave;
         // page ids of the wave's next 32 steps, two groups each: lane 2 i + g.  Waited for here, once in 4,096 keys: a wait inside the steps would be a wait
@@ -356,32 +356,34 @@ __global__ __launch_bounds__(256, (HD == 128 && !FP8) ? 1 : 2) void attn_paged_r
                 const size_t at = src.group(kc, __builtin_amdgcn_readlane(pages, 2 * i + g)) * (HD * 2);
                 const unsigned dst = img_lds + (buf * 2 * IMG + g * 16 * HD) * 2;
                 if (kb + 15 <= last) {
-                    dma_group<HD>(p.kpool + at, dst, off);
-                    dma_group<HD>(p.vpool + at, dst + IMG * 2, off);
+                    dma_rows(p.kpool + at, dst, off);
+                    dma_rows(p.vpool + at, dst + IMG * 2, off);
                 } else {
                     const int lim = kb > last ? 0 : last - kc;              // (a group behind the last key: 16 copies of a key that is there)
-                    dma_group_clamped<HD>(p.kpool + at, dst, lim, lane);
-                    dma_group_clamped<HD>(p.vpool + at, dst + IMG * 2, lim, lane);
+                    dma_rows_clamped<HD, 16>(p.kpool + at, dst, 0, lim, lane);
+                    dma_rows_clamped<HD, 16>(p.vpool + at, dst + IMG * 2, 0, lim, lane);
                 }
             }
         };
         if constexpr (FP8) {
-            Codes<HD> c[2];
+            // (one step's codes on their way in registers; three, at one block a CU, were slower: 52.8 us against 45.8 for 32 x 1,000..4,000 keys.  A lone wave
+            // spends 1.3 us a step, 0.65 of it in attend32 and 0.37 in the conversion: it is a second wave on the SIMD that hides them)
+            Codes<HD, 16> c[2];
             auto load_step = [&](int key) {
                 const int i = look(key);
 #pragma unroll
                 for (int g = 0; g < 2; ++g) {
                     const int kb = key + 16 * g, kc = min(kb, last & ~15);
-                    codes_load<HD>(c[g], p, src.group(kc, __builtin_amdgcn_readlane(pages, 2 * i + g)), kb > last ? 0 : min(last - kc, 15), lane);
+                    codes_load<HD, 16>(c[g], p, src.group(kc, __builtin_amdgcn_readlane(pages, 2 * i + g)), 0, kb > last ? 0 : min(last - kc, 15), lane);
                 }
             };
             if (key0 < k1) load_step(key0);
 #pragma unroll 1
             for (int key = key0; key < k1; key += 128) {
 #pragma unroll
-                for (int g = 0; g < 2; ++g) codes_store<HD>(c[g], img + g * 16 * HD, img + IMG + g * 16 * HD, lane);
+                for (int g = 0; g < 2; ++g) codes_store<HD, 16>(c[g], img, img + IMG, 16 * g, lane);
                 if (key + 128 < k1) load_step(key + 128);
-                attend32<HD, 1>(rows, img, img + IMG, 0, key, p.scale_log2, lane);
+                attend32<HD>(st, img, img + IMG, 0, key, p.scale_log2, lane);
             }
         } else {
             int buf = 0;
@@ -393,18 +395,17 @@ __global__ __launch_bounds__(256, (HD == 128 && !FP8) ? 1 : 2) void attn_paged_r
                 if (key + 128 < k1) {
                     dma_step(key + 128, buf ^ 1);
                     // this step's pieces have landed when only the next one's are still out
-                    if (HD == 128) asm volatile("s_waitcnt vmcnt(16)" ::: "memory");
-                    else asm volatile("s_waitcnt vmcnt(8)" ::: "memory");
+                    wait_vm<4 * PIECES<HD, 16>>();
                 } else {
                     dma_wait();
                 }
-                attend32<HD, 1>(rows, img + buf * 2 * IMG, img + buf * 2 * IMG + IMG, 0, key, p.scale_log2, lane);
+                attend32<HD>(st, img + buf * 2 * IMG, img + buf * 2 * IMG + IMG, 0, key, p.scale_log2, lane);
                 buf ^= 1;
             }
         }
-        if (st.odd) add_odd<HD, FP8>(st, st.qmin, p, src, k0 + 32 * wave, 128, k1, lane);
+        if (st.odd) add_odd<HD, FP8>(st, p, src, k0 + 32 * wave, 128, k1, lane);
         __syncthreads();                             // the images are dead; s_bad is set
-        scan_pages(p, src.row, k0, k1, &s_bad);
+        scan_pages<256>(p, src.row, k0, k1, &s_bad);
         // the four waves' rows, un-normalised, through LDS
         const int r = lane & 31, h = lane >> 5;
         const float l = st.l + __shfl_xor(st.l, 32, 64);
@@ -419,7 +420,6 @@ __global__ __launch_bounds__(256, (HD == 128 && !FP8) ? 1 : 2) void attn_paged_r
                         f32x4{st.o[d][4 * g4], st.o[d][4 * g4 + 1], st.o[d][4 * g4 + 2], st.o[d][4 * g4 + 3]};
         __syncthreads();
         const int bad = s_bad;
-        float* part = parts > 1 ? p.part + ((size_t)((b * p.tps + ti) * p.nkv + kvh) * p.parts + s) * (RROWS * (HD + 2)) : nullptr;
         for (int i = tid; i < t.rows * (HD / 4); i += 256) {
             const int row = i / (HD / 4), c4 = (i % (HD / 4)) * 4;
             float m = -INFINITY;
@@ -451,49 +451,65 @@ __global__ __launch_bounds__(256, (HD == 128 && !FP8) ? 1 : 2) void attn_paged_r
     }
 }
 
-// ---- long chunks: 128 * RB rows a block -----------------------------------------------------------------------------------------------------------
-// tile f of the sequences' tiles in reverse order (within a sequence the longest causal range first); -1: there are fewer
+// ---- long chunks: 128 or 64 rows a block -----------------------------------------------------------------------------------------------------------
+// tile f of the sequences' tiles: the longest sequences first (64 sequences at a time), within one the longest causal range first; -1: there are fewer.
+// Blocks start in order, so a compute unit's second block is a shorter one than its first, and the last to start are the shortest.
 template <int TROWS> __device__ __forceinline__ int find_tile(const AttnPagedArgs& p, int f, int lane, int* ti) {
-    auto tiles = [&](int b) {
-        if (b >= p.B) return 0;
-        const int s = min(max(p.cu_q[b], 0), p.n_tok), e = min(max(p.cu_q[b + 1], s), p.n_tok);
-        return ((e - s) * p.G + TROWS - 1) / TROWS;
-    };
-    int total = 0;
-    for (int b0 = 0; b0 < p.B; b0 += 64) total += (int)wave_sum((float)tiles(b0 + lane));      // (exact: below 2^24 tiles, checked by the host)
-    f = total - 1 - f;
-    if (f < 0) return -1;
-    for (int b0 = 0, base = 0; b0 < p.B; b0 += 64) {
-        const int n = tiles(b0 + lane);
-        int inc = n;
-#pragma unroll
-        for (int o = 1; o < 64; o <<= 1) {
-            const int x = __shfl_up(inc, o, 64);
-            inc += lane >= o ? x : 0;
+    for (int b0 = 0; b0 < p.B; b0 += 64) {
+        const int b = b0 + lane, in = min(p.B - b0, 64);
+        int n = 0, len = -1;
+        if (lane < in) {
+            const int s = min(max(p.cu_q[b], 0), p.n_tok), e = min(max(p.cu_q[b + 1], s), p.n_tok);
+            n = ((e - s) * p.G + TROWS - 1) / TROWS;
+            len = p.kv_len[b];
         }
-        const unsigned long long hit = __ballot(base + inc > f);
+        int before = 0, total = 0;                   // tiles of the longer sequences; of all
+        for (int j = 0; j < in; ++j) {
+            const int nj = __builtin_amdgcn_readlane(n, j), lj = __builtin_amdgcn_readlane(len, j);
+            before += lj > len || (lj == len && j < lane) ? nj : 0;
+            total += nj;
+        }
+        const unsigned long long hit = __ballot(f >= before && f < before + n);
         if (hit) {
             const int who = __ffsll((long long)hit) - 1;
-            *ti = f - base - (__builtin_amdgcn_readlane(inc, who) - __builtin_amdgcn_readlane(n, who));
+            *ti = __builtin_amdgcn_readlane(n, who) - 1 - (f - __builtin_amdgcn_readlane(before, who));
             return b0 + who;
         }
-        base += __builtin_amdgcn_readlane(inc, 63);
+        f -= total;
     }
     return -1;
 }
 
-template <int HD, bool FP8, int RB>
-__global__ __launch_bounds__(256, RB == 1 ? 2 : 1) void attn_paged_tile_kernel(AttnPagedArgs p) {
+// KS 1: the waves own 32 rows each (128 a block).  KS 2: two own 32 rows each (64 a block) for the first half of every tile's keys, two the same rows for the
+// second; they meet at the end.  Half the chain of steps a wave goes through, for twice the K / V traffic: for few tiles of unequal length.
+template <int HD, bool FP8, int KS>
+__global__ __launch_bounds__(256, 2) void attn_paged_tile_kernel(AttnPagedArgs p) {
     extern __shared__ __attribute__((aligned(16))) char smem_raw[];
     __shared__ int s_bad;
     bf16_t* smem = reinterpret_cast<bf16_t*>(smem_raw);            // [2 stages][K tile | V tile]
-    constexpr int TILE = 64 * HD, TROWS = 128 * RB, WROWS = 32 * RB;
+    constexpr int TILE = 64 * HD, TROWS = 128 / KS, R = 16;        // R: rows of a tile that a wave stages
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-    // the workgroups of one XCD (every eighth) take a contiguous run of the order (kv head, part, tile): they share a head's keys in its L2
-    const int q8 = gridDim.x >> 3, r8 = gridDim.x & 7, xcd = blockIdx.x & 7;
-    int v = (xcd < r8 ? xcd * (q8 + 1) : r8 * (q8 + 1) + (xcd - r8) * q8) + (blockIdx.x >> 3);
-    const int f = v % p.tps; v /= p.tps;
-    const int s = v % p.parts, kvh = v / p.parts;
+    const int wrow = KS == 1 ? wave * 32 : (wave & 1) * 32, kg = KS == 1 ? 0 : wave >> 1;
+    // The workgroups of one XCD (every eighth) share the keys of as few (kv head, part) units as possible in its L2: whole units to an XCD where they can
+    // be dealt evenly, every X-th tile of a unit to each of its X XCDs where there are fewer, else contiguous runs of (unit, tile).
+    const int units = p.nkv * p.parts, xcd = blockIdx.x & 7, i8 = blockIdx.x >> 3;
+    int f, unit;
+    if (units % 8 == 0) {
+        unit = xcd * (units / 8) + i8 / p.tps;
+        f = i8 % p.tps;
+    } else if (8 % units == 0) {
+        const int X = 8 / units;
+        unit = xcd / X;
+        f = i8 * X + xcd % X;
+    } else {
+        const int run = (units * p.tps + 7) / 8;
+        const int v = xcd * run + i8;
+        if (i8 >= run || v >= units * p.tps) return;
+        unit = v / p.tps;
+        f = v % p.tps;
+    }
+    if (f >= p.tps) return;
+    const int s = unit % p.parts, kvh = unit / p.parts;
     int ti = 0;
     const int b = __builtin_amdgcn_readfirstlane(find_tile<TROWS>(p, f, lane, &ti));
     if (b < 0) return;
@@ -501,215 +517,251 @@ __global__ __launch_bounds__(256, RB == 1 ? 2 : 1) void attn_paged_tile_kernel(A
     const Tile t = make_tile<TROWS>(p, b, ti);
     const int kmax = p.max_pages << p.page_shift;
     const int n_keys = min(t.n_vis, kmax);
-    const int parts = parts_of(n_keys, p.parts, MIN_KEYS_TILE);
+    const int parts = parts_of(n_keys, p.parts);
     if (s >= parts) return;
     const int chunk = part_keys<64>(n_keys, parts);
     const int k0 = s * chunk, k1 = min(n_keys, k0 + chunk), last = k1 - 1;
     const KvSource src{p.table + (size_t)b * p.ld_table, p.n_pages, p.page_shift, p.nkv, kvh};
     if (tid == 0) s_bad = t.n_vis > kmax ? kmax : 0x7fffffff;
-    const bool active = wave * WROWS < t.rows;
-    Rows<HD> st[RB];
+    const bool active = wrow < t.rows;
+    Rows<HD> st;
+    rows_init<HD>(st, p, t, kvh, wrow, lane);
 #pragma unroll
-    for (int rb = 0; rb < RB; ++rb) rows_init<HD>(st[rb], p, t, kvh, wave * WROWS + 32 * rb, lane);
-#pragma unroll
-    for (int rb = 0; rb < RB; ++rb)
-#pragma unroll
-        for (int i = 0; i < HD / 16; ++i) arrived(st[rb].qf[i]);
-    const int qmax = st[RB - 1].qmax;
-    unsigned off[NPG<HD>];
-#pragma unroll
-    for (int i = 0; i < NPG<HD>; ++i) {
-        int row, col;
-        piece_row_col<HD>(i, lane, row, col);
-        off[i] = (unsigned)((row * HD + col) * 2);
-    }
+    for (int i = 0; i < HD / 16; ++i) arrived(st.qf[i]);
+    const int r0 = wave * R;                         // this wave's rows of every tile: within one 16-key group, so on one page
+    unsigned off[PIECES<HD, R>];
+    piece_offsets<HD, R>(r0, lane, off);
     const unsigned smem_lds = __builtin_amdgcn_readfirstlane((unsigned)(uintptr_t)LDS_PTR(smem));
-    int pages = 0;                                   // page ids of this wave's 16 keys of the next 64 tiles (waited for once in 4,096 keys)
-    Codes<HD> c;
-    auto issue = [&](int k, int stg) {               // keys k .. k + 63; this wave's are k + 16 * wave ..
-        const int i = ((k - k0) >> 6) & 63;
-        if (i == 0) {
-            pages = src.row[min(k + 64 * lane + 16 * wave, last) >> p.page_shift];
+    const int tiles = k1 > k0 ? (k1 - k0 + 63) >> 6 : 0;
+    int pages = 0;                                   // page ids of this wave's rows of the next 64 tiles (waited for once in 4,096 keys)
+    Codes<HD, R> c;
+    auto issue = [&](int i) {                        // tile i
+        if ((i & 63) == 0) {
+            pages = src.row[min(k0 + 64 * (i + lane) + (r0 & ~15), last) >> p.page_shift];
             arrived(pages);
         }
-        const int kb = k + 16 * wave, kc = min(kb, last & ~15);
-        const size_t at = src.group(kc, __builtin_amdgcn_readlane(pages, i));
+        const int kb = k0 + 64 * i + (r0 & ~15), kc = min(kb, last & ~15);
+        const size_t at = src.group(kc, __builtin_amdgcn_readlane(pages, i & 63));
         if constexpr (FP8) {
-            codes_load<HD>(c, p, at, kb > last ? 0 : min(last - kc, 15), lane);
+            codes_load<HD, R>(c, p, at, r0, kb > last ? 0 : min(last - kc, 15), lane);
         } else {
-            const unsigned dst = smem_lds + (stg * 2 * TILE + wave * 16 * HD) * 2;
+            const unsigned dst = smem_lds + ((i & 1) * 2 * TILE + r0 * HD) * 2;
             if (kb + 15 <= last) {
-                dma_group<HD>(p.kpool + at * (HD * 2), dst, off);
-                dma_group<HD>(p.vpool + at * (HD * 2), dst + TILE * 2, off);
+                dma_rows(p.kpool + at * (HD * 2), dst, off);
+                dma_rows(p.vpool + at * (HD * 2), dst + TILE * 2, off);
             } else {
                 const int lim = kb > last ? 0 : last - kc;
-                dma_group_clamped<HD>(p.kpool + at * (HD * 2), dst, lim, lane);
-                dma_group_clamped<HD>(p.vpool + at * (HD * 2), dst + TILE * 2, lim, lane);
+                dma_rows_clamped<HD, R>(p.kpool + at * (HD * 2), dst, r0, lim, lane);
+                dma_rows_clamped<HD, R>(p.vpool + at * (HD * 2), dst + TILE * 2, r0, lim, lane);
             }
         }
     };
-    auto land = [&](int stg) {
-        if constexpr (FP8) codes_store<HD>(c, smem + stg * 2 * TILE + wave * 16 * HD, smem + stg * 2 * TILE + TILE + wave * 16 * HD, lane);
-        else dma_wait();
+    auto land = [&](int i) {                         // this wave's rows of tile i are in LDS
+        if constexpr (FP8) {
+            bf16_t* img = smem + (i & 1) * 2 * TILE;
+            codes_store<HD, R>(c, img, img + TILE, r0, lane);
+            if (i + 1 < tiles) issue(i + 1);         // (the codes go out a whole tile ahead)
+        } else {
+            dma_wait();
+        }
     };
-    if (k0 < k1) {
-        issue(k0, 0);
+    if (tiles > 0) {
+        issue(0);
         land(0);
     }
     __syncthreads();
-    scan_pages(p, src.row, k0, k1, &s_bad);
-    int cur = 0;
+    scan_pages<256>(p, src.row, k0, k1, &s_bad);
 #pragma unroll 1
-    for (int k = k0; k < k1; k += 64) {
-        const bf16_t* sK = smem + cur * 2 * TILE;
-        if (k + 64 < k1) issue(k + 64, cur ^ 1);
+    for (int i = 0; i < tiles; ++i) {
+        const bf16_t* sK = smem + (i & 1) * 2 * TILE;
+        if (!FP8 && i + 1 < tiles) issue(i + 1);     // (its stage was read up to the last barrier)
+        const int k = k0 + 64 * i;
         if (active) {
+            if constexpr (KS == 2) {
+                if (k + 32 * kg <= st.qmax) attend32<HD>(st, sK + 32 * HD * kg, sK + TILE + 32 * HD * kg, 0, k + 32 * kg, p.scale_log2, lane);
+            } else {
 #pragma unroll
-            for (int sub = 0; sub < 2; ++sub)
-                if (k + 32 * sub <= qmax) attend32<HD, RB>(st, sK, sK + TILE, sub, k + 32 * sub, p.scale_log2, lane);
-        }
-        if (k + 64 < k1) land(cur ^ 1);
-        __syncthreads();
-        cur ^= 1;
-    }
-    if (k0 >= k1) __syncthreads();                   // (s_bad)
-    // ---- epilogue: this wave's rows, 32 at a time
-    if (!active) return;
-    const int r = lane & 31, h = lane >> 5;
-#pragma unroll
-    for (int rb = 0; rb < RB; ++rb) {
-        const int wrow = wave * WROWS + 32 * rb, rows = min(32, t.rows - wrow);
-        if (rows <= 0) return;
-        if (st[0].odd) add_odd<HD, FP8>(st[rb], st[0].qmin, p, src, k0, 32, min(k1, qmax + 1), lane);
-        float l = st[rb].l + __shfl_xor(st[rb].l, 32, 64);
-        if (st[rb].qi >= s_bad) l = __builtin_nanf("");
-        if (parts > 1) {
-            float* part = p.part + ((size_t)(f * p.nkv + kvh) * p.parts + s) * (TROWS * (HD + 2));
-            if (r < rows) {
-                float* d = part + (size_t)(wrow + r) * HD;
-#pragma unroll
-                for (int dd = 0; dd < HD / 32; ++dd)
-#pragma unroll
-                    for (int g4 = 0; g4 < 4; ++g4)
-                        *reinterpret_cast<f32x4*>(d + 32 * dd + 8 * g4 + 4 * h) = f32x4{st[rb].o[dd][4 * g4], st[rb].o[dd][4 * g4 + 1],
-                                                                                       st[rb].o[dd][4 * g4 + 2], st[rb].o[dd][4 * g4 + 3]};
-                if (h == 0) *reinterpret_cast<f32x2*>(part + TROWS * HD + (wrow + r) * 2) = f32x2{st[rb].m, l};
+                for (int sub = 0; sub < 2; ++sub)
+                    if (k + 32 * sub <= st.qmax) attend32<HD>(st, sK, sK + TILE, sub, k + 32 * sub, p.scale_log2, lane);
             }
-            continue;
         }
-        const float inv = l == 0.f ? 0.f : 1.f / l;
-        // rows through a slab of the wave's own in the dead stages: whole rows leave, 16 bytes a lane
-        constexpr int PITCH = HD + 8, LPR = HD / 8, RPI = 64 / LPR;
-        bf16_t* slab = smem + wave * 32 * PITCH;
+        if (i + 1 < tiles) land(i + 1);
+        __syncthreads();
+    }
+    if (tiles == 0) __syncthreads();                 // (s_bad)
+    // ---- epilogue: this wave's 32 rows
+    if (active && st.odd) add_odd<HD, FP8>(st, p, src, k0 + 32 * kg, 32 * KS, min(k1, st.qmax + 1), lane);
+    const int r = lane & 31, h = lane >> 5, rows = min(32, t.rows - wrow);
+    float l = st.l + __shfl_xor(st.l, 32, 64);
+    if constexpr (KS == 2) {                         // the second half's waves hand their rows over, register by register, in the dead stages
+        f32x4* o2 = reinterpret_cast<f32x4*>(smem_raw) + (wave & 1) * (HD * 32 / 4 + 64) + lane;
+        if (kg == 1) {
+#pragma unroll
+            for (int d = 0; d < HD / 32; ++d)
+#pragma unroll
+                for (int g4 = 0; g4 < 4; ++g4)
+                    o2[(d * 4 + g4) * 64] = f32x4{st.o[d][4 * g4], st.o[d][4 * g4 + 1], st.o[d][4 * g4 + 2], st.o[d][4 * g4 + 3]};
+            o2[HD / 32 * 4 * 64] = f32x4{st.m, l, 0.f, 0.f};
+        }
+        __syncthreads();
+        if (kg == 1) return;
+        const f32x4 ml = o2[HD / 32 * 4 * 64];
+        const float m = fmaxf(st.m, ml[0]), mu = m == -INFINITY ? 0.f : m;
+        const float f0 = fast_exp2(st.m - mu), f1 = fast_exp2(ml[0] - mu);
+        st.m = m;
+        l = l * f0 + ml[1] * f1;
 #pragma unroll
         for (int d = 0; d < HD / 32; ++d)
 #pragma unroll
-            for (int g4 = 0; g4 < 4; ++g4)
-                *reinterpret_cast<u32x2*>(slab + r * PITCH + 32 * d + 8 * g4 + 4 * h) =
-                    u32x2{pack_bf2(st[rb].o[d][4 * g4] * inv, st[rb].o[d][4 * g4 + 1] * inv),
-                          pack_bf2(st[rb].o[d][4 * g4 + 2] * inv, st[rb].o[d][4 * g4 + 3] * inv)};
-        const int lr = lane / LPR, lc = (lane % LPR) * 8;
+            for (int g4 = 0; g4 < 4; ++g4) {
+                const f32x4 x = o2[(d * 4 + g4) * 64];
 #pragma unroll
-        for (int it = 0; it < 32 / RPI; ++it) {
-            const int row = it * RPI + lr;
-            const u32x4 x = *reinterpret_cast<const u32x4*>(slab + row * PITCH + lc);
-            const int R = t.row0 + wrow + row, tok = R / p.G;
-            if (row < rows) *reinterpret_cast<u32x4*>(p.out + (size_t)(t.tok0 + tok) * p.ldo + (kvh * p.G + R - tok * p.G) * HD + lc) = x;
+                for (int e = 0; e < 4; ++e)          // (a half that weighs nothing adds nothing: never 0 * inf)
+                    st.o[d][4 * g4 + e] = (f0 == 0.f ? 0.f : st.o[d][4 * g4 + e] * f0) + (f1 == 0.f ? 0.f : x[e] * f1);
+            }
+    }
+    if (!active) return;
+    if (st.qi >= s_bad) l = __builtin_nanf("");
+    if (parts > 1) {
+        float* part = p.part + ((size_t)(f * p.nkv + kvh) * p.parts + s) * (TROWS * (HD + 2));
+        if (r < rows) {
+            float* d = part + (size_t)(wrow + r) * HD;
+#pragma unroll
+            for (int dd = 0; dd < HD / 32; ++dd)
+#pragma unroll
+                for (int g4 = 0; g4 < 4; ++g4)
+                    *reinterpret_cast<f32x4*>(d + 32 * dd + 8 * g4 + 4 * h) =
+                        f32x4{st.o[dd][4 * g4], st.o[dd][4 * g4 + 1], st.o[dd][4 * g4 + 2], st.o[dd][4 * g4 + 3]};
+            if (h == 0) *reinterpret_cast<f32x2*>(part + TROWS * HD + (wrow + r) * 2) = f32x2{st.m, l};
         }
+        return;
+    }
+    const float inv = l == 0.f ? 0.f : 1.f / l;
+    // rows through a slab of the wave's own in the dead stages: whole rows leave, 16 bytes a lane
+    constexpr int PITCH = HD + 8, LPR = HD / 8, RPI = 64 / LPR;
+    bf16_t* slab = smem + (KS == 2 ? 64 * HD * 2 + 1024 : 0) + wave * 32 * PITCH;      // (KS 2: behind the rows handed over)
+#pragma unroll
+    for (int d = 0; d < HD / 32; ++d)
+#pragma unroll
+        for (int g4 = 0; g4 < 4; ++g4)
+            *reinterpret_cast<u32x2*>(slab + r * PITCH + 32 * d + 8 * g4 + 4 * h) =
+                u32x2{pack_bf2(st.o[d][4 * g4] * inv, st.o[d][4 * g4 + 1] * inv), pack_bf2(st.o[d][4 * g4 + 2] * inv, st.o[d][4 * g4 + 3] * inv)};
+    const int lr = lane / LPR, lc = (lane % LPR) * 8;
+#pragma unroll
+    for (int it = 0; it < 32 / RPI; ++it) {
+        const int row = it * RPI + lr;
+        const u32x4 x = *reinterpret_cast<const u32x4*>(slab + row * PITCH + lc);
+        const int RR = t.row0 + wrow + row, tok = RR / p.G;
+        if (row < rows) *reinterpret_cast<u32x4*>(p.out + (size_t)(t.tok0 + tok) * p.ldo + (kvh * p.G + RR - tok * p.G) * HD + lc) = x;
     }
 }
 
-// ---- the parts of a tile's rows: out = sum_s 2^(m_s - m) o_s / sum_s 2^(m_s - m) l_s; one wave a row, lane s holding part s's maximum and sum
-template <int HD, int ROWS>
-__global__ __launch_bounds__(256) void attn_paged_merge_kernel(AttnPagedArgs p) {
-    constexpr bool TILEK = ROWS != RROWS;
-    constexpr int C = HD / 64, STRIDE = ROWS * (HD + 2);
-    const int lane = threadIdx.x & 63;
-    const int tile = blockIdx.x / p.nkv, kvh = blockIdx.x % p.nkv;
-    int b, ti = 0;
-    if constexpr (TILEK) b = find_tile<ROWS>(p, tile, lane, &ti);
-    else { b = tile / p.tps; ti = tile % p.tps; }
-    if (b < 0) return;
-    const Tile t = make_tile<ROWS>(p, b, ti);
-    const int parts = parts_of(min(t.n_vis, p.max_pages << p.page_shift), p.parts, TILEK ? MIN_KEYS_TILE : MIN_KEYS_ROWS);
-    if (parts == 1) return;                          // written by the attention itself
-    const float* base = p.part + (size_t)(tile * p.nkv + kvh) * p.parts * STRIDE;
-    for (int row = blockIdx.y * 4 + (threadIdx.x >> 6); row < t.rows; row += gridDim.y * 4) {
-        float ms = -INFINITY, ls = 0.f;
-        if (lane < parts) {
-            const f32x2 ml = *reinterpret_cast<const f32x2*>(base + (size_t)lane * STRIDE + ROWS * HD + row * 2);
-            ms = ml[0]; ls = ml[1];
-        }
-        const float m = wave_max(ms), f = fast_exp2(ms - (m == -INFINITY ? 0.f : m));
-        const float l = wave_sum(lane < parts ? ls * f : 0.f);
-        float a[C];
+// ---- joining parts: out = sum_s 2^(m_s - m) o_s / sum_s 2^(m_s - m) l_s.  One wave a row, the lanes holding the parts' maxima and sums; part s is
+// at at(s): HD outputs of the row, `ml` floats behind them its maximum and sum.
+template <int HD, class At>
+__device__ __forceinline__ void join_parts(int parts, At at, size_t ml, bf16_t* dst, int lane) {
+    constexpr int C = HD / 64;
+    float m = -INFINITY;
+    for (int s = lane; s < parts; s += 64) m = fmaxf(m, at(s)[ml]);
+    m = wave_max(m);
+    const float mu = m == -INFINITY ? 0.f : m;
+    float l = 0.f, a[C];
 #pragma unroll
-        for (int c = 0; c < C; ++c) a[c] = 0.f;
-        const float* po = base + row * HD + lane * C;
-        for (int s0 = 0; s0 < parts; s0 += 8) {      // eight parts' loads in flight
+    for (int c = 0; c < C; ++c) a[c] = 0.f;
+    for (int s0 = 0; s0 < parts; s0 += 64) {
+        float f = 0.f;
+        if (s0 + lane < parts) {
+            const f32x2 v = *reinterpret_cast<const f32x2*>(at(s0 + lane) + ml);
+            f = fast_exp2(v[0] - mu);
+            l += v[1] * f;
+        }
+        const int n = min(parts - s0, 64);
+        for (int i0 = 0; i0 < n; i0 += 8) {          // eight parts' loads in flight
             float x[8][C];
 #pragma unroll
             for (int i = 0; i < 8; ++i)
 #pragma unroll
-                for (int c = 0; c < C; ++c) x[i][c] = po[(size_t)min(s0 + i, parts - 1) * STRIDE + c];
+                for (int c = 0; c < C; ++c) x[i][c] = at(s0 + min(i0 + i, n - 1))[lane * C + c];
 #pragma unroll
-            for (int i = 0; i < 8; ++i) {            // (lanes behind the last part weigh 0; a part that weighs nothing adds nothing: never 0 * inf)
-                const float fs = s0 + i < parts ? __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, f), (s0 + i) & 63)) : 0.f;
+            for (int i = 0; i < 8; ++i) {            // (a part that weighs nothing adds nothing: never 0 * inf)
+                const float fs = i0 + i < n ? __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, f), (i0 + i) & 63)) : 0.f;
 #pragma unroll
                 for (int c = 0; c < C; ++c) a[c] += fs == 0.f ? 0.f : x[i][c] * fs;
             }
         }
-        const float inv = l == 0.f ? 0.f : 1.f / l;
+    }
+    l = wave_sum(l);
+    const float inv = l == 0.f ? 0.f : 1.f / l;
+    if (C == 2) *reinterpret_cast<unsigned*>(dst + lane * C) = pack_bf2(a[0] * inv, a[C - 1] * inv);
+    else dst[lane] = f2bf(a[0] * inv);
+}
+
+// a block takes every gridDim.y-th group of four rows of a tile
+template <int HD, int ROWS>
+__global__ __launch_bounds__(256) void attn_paged_join_kernel(AttnPagedArgs p) {
+    constexpr int STRIDE = ROWS * (HD + 2);
+    const int lane = threadIdx.x & 63, tile = blockIdx.x / p.nkv, kvh = blockIdx.x % p.nkv;
+    int b = tile / p.tps, ti = tile % p.tps;
+    if constexpr (ROWS != RROWS) b = find_tile<ROWS>(p, tile, lane, &ti);
+    if (b < 0) return;
+    const Tile t = make_tile<ROWS>(p, b, ti);
+    const int parts = parts_of(min(t.n_vis, p.max_pages << p.page_shift), p.parts);
+    if (parts == 1) return;                          // written by the attention itself
+    const float* base = p.part + (size_t)(tile * p.nkv + kvh) * p.parts * STRIDE;
+    for (int row = blockIdx.y * 4 + (threadIdx.x >> 6); row < t.rows; row += gridDim.y * 4) {
         const int R = t.row0 + row, tok = R / p.G;
-        bf16_t* d = p.out + (size_t)(t.tok0 + tok) * p.ldo + (kvh * p.G + R - tok * p.G) * HD + lane * C;
-        if (C == 2) *reinterpret_cast<unsigned*>(d) = pack_bf2(a[0] * inv, a[C - 1] * inv);
-        else d[0] = f2bf(a[0] * inv);
+        join_parts<HD>(parts, [&](int s) { return base + (size_t)s * STRIDE + row * HD; }, (size_t)ROWS * HD + row * 2 - row * HD,
+                       p.out + (size_t)(t.tok0 + tok) * p.ldo + (kvh * p.G + R - tok * p.G) * HD, lane);
     }
 }
 
 // ---- host: which kernel, and how many parts
-struct Shape { int rb, tps, parts, rows; long part_floats; };
+struct Shape { int ks, tps, parts, rows; long tiles, part_floats; };      // ks 0: the rows kernel
 Shape pick_shape(int n_tok, int B, int nkv, int G, int HD, bool fp8, long max_keys, int max_q, int max_kv) {
     Shape sh{};
     const long mq = max_q > 0 && max_q < n_tok ? max_q : n_tok;
     const long keys = max_kv > 0 && max_kv < max_keys ? max_kv : max_keys;
-    // 256-row tiles (one block a CU) where they still give every CU one; 128-row ones (two a CU) below that; the rows kernel for single steps
-    static const int force = [] { const char* e = getenv("MOLLY_PAGED_RB"); return e ? atoi(e) : -1; }();
-    sh.rb = mq * G <= RROWS ? 0 : ((long)n_tok * G / 256) * nkv >= 256 ? 2 : 1;
-    if (force > 0 && sh.rb) sh.rb = force;
-    const int rows = sh.rb ? 128 * sh.rb : RROWS;
-    const long tps = sh.rb ? (long)n_tok * G / rows + B : (mq * G + RROWS - 1) / RROWS;
-    sh.tps = (int)tps;
+    // 64-row tiles where 128-row ones would leave compute units without a second block: 512 tokens x 4 heads a kv head over 8,192 keys 137 -> 116 us, one
+    // sequence of 64 over 20,000 52 -> 46 us; but 2,048 tokens over 16,384 keys 518 -> 560 us, 24 mixed sequences 103 -> 111 us
+    sh.ks = mq * G <= RROWS ? 0 : ((long)n_tok * G / 128 + B) * nkv < 512 ? 2 : 1;
+    const int rows = sh.ks ? 128 / sh.ks : RROWS;
+    sh.tps = (int)(sh.ks ? (long)n_tok * G / rows + B : (mq * G + RROWS - 1) / RROWS);
     sh.rows = (int)(mq * G < rows ? mq * G : rows);      // rows of a tile, as far as the caller knows
-    const long units = (sh.rb ? tps : tps * B) * nkv;
-    // resident blocks: 2 a CU, 1 for the rows kernel with 128 KB of images
-    const long want = sh.rb ? 512 / sh.rb : (HD == 128 && !fp8 ? 512 : 1024);
-    long parts = want / (units > 0 ? units : 1);
-    const long most = keys / (sh.rb ? MIN_KEYS_TILE : MIN_KEYS_ROWS);
-    if (parts > most) parts = most;
+    sh.tiles = sh.ks ? sh.tps : (long)sh.tps * B;
+    const long units = sh.tiles * nkv, slots = HD == 128 && !fp8 && !sh.ks ? 256 : 512;      // blocks that are resident at a time
+    long parts = units > 0 ? slots / units : 1;
+    if (parts > keys / MIN_KEYS) parts = keys / MIN_KEYS;
     if (parts > MAX_PARTS) parts = MAX_PARTS;
     sh.parts = parts < 1 ? 1 : (int)parts;
     sh.part_floats = sh.parts > 1 ? units * sh.parts * rows * (HD + 2) : 0;
     return sh;
 }
 
-template <int HD, bool FP8, int RB>
+template <int HD, int ROWS>
+void launch_join(hipStream_t st, const AttnPagedArgs& p, const Shape& sh) {
+    const long n = sh.tiles * p.nkv, most = (sh.rows + 3) / 4, y = (4095 + n) / n;      // a group of four rows a block, up to some 4,096 blocks
+    hipLaunchKernelGGL((attn_paged_join_kernel<HD, ROWS>), dim3((unsigned)n, (unsigned)(y < most ? y : most)), dim3(256), 0, st, p);
+}
+template <int HD, bool FP8, int KS>
 void launch_tile(hipStream_t st, const AttnPagedArgs& p, const Shape& sh) {
-    const size_t lds = 2 * 2 * 64 * HD * 2;
-    static const hipError_t once = hipFuncSetAttribute((const void*)attn_paged_tile_kernel<HD, FP8, RB>, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
+    // two stages; behind the loop the waves' rows (KS 2: 64 rows in fp32 with their maxima and sums, and the slabs)
+    constexpr size_t stages = 2 * 2 * 64 * HD * 2, tail = KS == 2 ? 64 * HD * 4 + 2048 + 2 * 32 * (HD + 8) * 2 : 4 * 32 * (HD + 8) * 2, lds = stages > tail ? stages : tail;
+    static const hipError_t once = hipFuncSetAttribute((const void*)attn_paged_tile_kernel<HD, FP8, KS>, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
     (void)once;
-    hipLaunchKernelGGL((attn_paged_tile_kernel<HD, FP8, RB>), dim3(sh.tps * p.nkv * sh.parts), dim3(256), lds, st, p);
-    if (sh.parts > 1) hipLaunchKernelGGL((attn_paged_merge_kernel<HD, 128 * RB>), dim3(sh.tps * p.nkv, 32 * RB), dim3(256), 0, st, p);
+    const int units = p.nkv * sh.parts;              // (the kernel's three ways to deal them to the 8 XCDs)
+    const long blocks = 8 % units == 0 ? 8L * cdiv(sh.tps, 8 / units) : 8L * cdiv((long)units * sh.tps, 8);
+    hipLaunchKernelGGL((attn_paged_tile_kernel<HD, FP8, KS>), dim3((unsigned)blocks), dim3(256), lds, st, p);
+    if (sh.parts > 1) launch_join<HD, 128 / KS>(st, p, sh);
 }
 template <int HD, bool FP8>
 void launch(hipStream_t st, const AttnPagedArgs& p, const Shape& sh) {
-    if (sh.rb == 2) return launch_tile<HD, FP8, 2>(st, p, sh);
-    if (sh.rb == 1) return launch_tile<HD, FP8, 1>(st, p, sh);
+    if (sh.ks == 2) return launch_tile<HD, FP8, 2>(st, p, sh);
+    if (sh.ks == 1) return launch_tile<HD, FP8, 1>(st, p, sh);
     const size_t lds = 4 * RROWS * HD * 4 * (FP8 ? 1 : 2);            // images (e4m3: one buffer of 32 rows K | V in bf16), at the end the four waves' rows in fp32
     static const hipError_t once = hipFuncSetAttribute((const void*)attn_paged_rows_kernel<HD, FP8>, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
     (void)once;
-    hipLaunchKernelGGL((attn_paged_rows_kernel<HD, FP8>), dim3(p.B * sh.tps * p.nkv * sh.parts), dim3(256), lds, st, p);
-    if (sh.parts > 1) hipLaunchKernelGGL((attn_paged_merge_kernel<HD, RROWS>), dim3(p.B * sh.tps * p.nkv, cdiv(sh.rows, 4)), dim3(256), 0, st, p);
+    hipLaunchKernelGGL((attn_paged_rows_kernel<HD, FP8>), dim3((unsigned)(sh.tiles * p.nkv * sh.parts)), dim3(256), lds, st, p);
+    if (sh.parts > 1) launch_join<HD, RROWS>(st, p, sh);
 }
 
 int check_sizes(int n_tokens, int B, int n_heads, int n_kv_heads, int max_pages, int page_size) {
@@ -751,7 +803,7 @@ extern "C" int molly_attn_paged(void* stream, const void* q, void* out, const vo
     p.n_pages = n_pages; p.page_shift = log2_exact(page_size); p.max_pages = max_pages; p.ld_table = ld_table;
     p.nh = n_heads; p.nkv = n_kv_heads; p.G = n_heads / n_kv_heads; p.ldq = ldq; p.ldo = ldo; p.scale_log2 = scale * LOG2E;
     Shape sh = pick_shape(n_tokens, B, n_kv_heads, p.G, head_dim, kscale_or_null != nullptr, (long)max_pages * page_size, max_q, max_kv);
-    if (sh.parts > 1 && (!workspace || workspace_floats < sh.part_floats)) sh.parts = 1;
+    if (!workspace || workspace_floats < sh.part_floats) sh.parts = 1;
     p.part = workspace; p.tps = sh.tps; p.parts = sh.parts;
     hipStream_t st = (hipStream_t)stream;
     if (head_dim == 128) {

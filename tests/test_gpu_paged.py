@@ -221,6 +221,30 @@ def test_attn_paged(new, keys, nh, nkv, hd, page, fp8):
     assert torch.equal(out, ops().attn_paged(q, kp, vp, table, cu_t, len_t, nh, kscale=ks, vscale=vs, max_q=max(new), max_kv=max(keys)))
 
 
+@pytest.mark.parametrize("fp8", [False, True])
+@pytest.mark.parametrize("kind", ["decode", "short", "mixed", "long"])
+def test_attn_paged_many_sequences(kind, fp8):
+    """More sequences than a wave has lanes, some without new tokens, lengths from none to thousands; few long ones over few heads."""
+    import random
+    r = random.Random(3)
+    B = 150 if kind != "long" else 3
+    keys = [int(5000 * r.random() ** 4) for _ in range(B)] if kind != "long" else [20000, 100, 9000]
+    new = {"decode": [1] * B, "short": [r.choice([0, 1, 3, 7]) for _ in range(B)], "mixed": [r.choice([0, 1, 1, 40]) for _ in range(B)],
+           "long": [1, 0, 2]}[kind]
+    nh, nkv = (8, 2) if kind != "long" else (4, 1)
+    q, kp, vp, ks, vs, table, cu, keys, cu_t, len_t = case(new, keys, nh, nkv, 64, 32, fp8, seed=6)
+    o = ops()
+    n, max_pages = q.shape[0], table.shape[1]
+    floats = o.attn_paged_workspace(n, B, nh, nkv, 64, 32, max_pages, fp8, max(new), max(keys))
+    outs = []
+    for ws in (None, torch.full((max(floats, 1),), math.nan, device=DEV), torch.empty(16, device=DEV)):      # its own; the caller's; too small: uncut
+        outs.append(o.attn_paged(q, kp, vp, table, cu_t, len_t, nh, kscale=ks, vscale=vs, max_q=max(new), max_kv=max(keys), workspace=ws))
+        check(outs[-1], q, kp, vp, ks, vs, table, cu, keys, nh)
+    assert torch.equal(outs[0], outs[1])
+    for mq, mk in ((1, 1), (0, 0)):                               # hints that are wrong
+        check(o.attn_paged(q, kp, vp, table, cu_t, len_t, nh, kscale=ks, vscale=vs, max_q=mq, max_kv=mk), q, kp, vp, ks, vs, table, cu, keys, nh)
+
+
 @pytest.mark.parametrize("new,keys", [([1, 1], [2100, 33]), ([90, 3], [400, 3])])
 def test_attn_paged_e4m3_is_bf16_of_the_held_values(new, keys):
     q, kp, vp, ks, vs, table, cu, keys, cu_t, len_t = case(new, keys, 8, 2, 128, 32, True, seed=5)

@@ -6,7 +6,7 @@
 // The query heads of a kv head are packed into the rows of one tile (row = token * G + head of the group), so K and V are read once for all of
 // them whatever G is; the arithmetic is that of attention.hip: S^T = K Q^T and O^T = V^T P^T by 32x32x16 MFMA, online softmax in the exp2
 // domain in fp32, P rounded to bf16 (2^-8 of a term) for the second product.  Two kernels:
-//   attn_paged_rows_kernel : up to 32 rows a tile (decode, short chunks).  The four waves of a block take every fourth step of 32 keys, each with
+//   attn_paged_rows_kernel : up to 32 rows a tile (decode, short chunks).  The 4 | 8 waves of a block take turns at steps of 32 keys, each with
 //                            K / V images of its own in LDS: no workgroup barrier in the loop, the waves meet at the end.  Bound by HBM.
 //   attn_paged_tile_kernel : 128 rows a tile (prompt chunks, mixed batches).  The waves own 32 rows each and share K / V tiles of 64
 //                            keys, double-buffered.  Bound by the matrix pipes where the chunk is long.
@@ -78,9 +78,10 @@ template <int HD> __device__ __forceinline__ void piece_row_col(int i, int lane,
     row = rbl * 4 + (cin >> 1);
     col = (((blk % NCB) ^ b0) << 4) + (((cin & 1) ^ b1) << 3);
 }
-__device__ __forceinline__ void dma16(unsigned off, const char* base, unsigned lds) {
+template <bool NT> __device__ __forceinline__ void dma16(unsigned off, const char* base, unsigned lds) {
     // (from asm, as in attention.hip: with the builtin hipcc waits for every pending LDS-DMA in front of the next transposed read)
-    asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(off), "s"(base), "s"(lds) : "memory", "m0");
+    if (NT) asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1 nt" ::"v"(off), "s"(base), "s"(lds) : "memory", "m0");
+    else asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(off), "s"(base), "s"(lds) : "memory", "m0");
 }
 template <int HD, int R>
 __device__ __forceinline__ void piece_offsets(int r0, int lane, unsigned (&off)[PIECES<HD, R>]) {
@@ -91,10 +92,10 @@ __device__ __forceinline__ void piece_offsets(int r0, int lane, unsigned (&off)[
         off[i] = (unsigned)((row * HD + col) * 2);
     }
 }
-template <int N>
+template <bool NT, int N>
 __device__ __forceinline__ void dma_rows(const char* base, unsigned lds, const unsigned (&off)[N]) {
 #pragma unroll
-    for (int i = 0; i < N; ++i) dma16(off[i], base, __builtin_amdgcn_readfirstlane(lds + i * 1024));
+    for (int i = 0; i < N; ++i) dma16<NT>(off[i], base, __builtin_amdgcn_readfirstlane(lds + i * 1024));
 }
 // the same for the group that the last key is in (or lies in front of): rows behind it repeat it, so that nothing behind a sequence's end — stale
 // pages may hold NaN — gets into the tile
@@ -104,9 +105,11 @@ __device__ __forceinline__ void dma_rows_clamped(const char* base, unsigned lds,
     for (int i = 0; i < PIECES<HD, R>; ++i) {
         int row, col;
         piece_row_col<HD>((r0 & 15) * HD / 512 + i, lane, row, col);
-        dma16((unsigned)((min(row, lim) * HD + col) * 2), base, __builtin_amdgcn_readfirstlane(lds + i * 1024));
+        dma16<false>((unsigned)((min(row, lim) * HD + col) * 2), base, __builtin_amdgcn_readfirstlane(lds + i * 1024));
     }
 }
+// every LDS read of this wave has its data: what it read may be overwritten
+__device__ __forceinline__ void lds_read_done() { asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory"); }
 template <int N> __device__ __forceinline__ void wait_vm() { asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory"); }
 
 // R rows of a 16-key group as e4m3 codes through registers: NL loads of 16 codes a lane, K's units first, then V's.  Lanes go over the 4 rows of a block
@@ -116,7 +119,7 @@ template <int HD, int R> struct Codes {
     u32x4 c[NL];
     uint8_t e[NL];
 };
-template <int HD, int R>
+template <int HD, int R, bool NT>
 __device__ __forceinline__ void codes_load(Codes<HD, R>& c, const AttnPagedArgs& p, size_t at, int r0, int lim, int lane) {
     constexpr int NCB = HD / 16, LRB = NCB * 4, UPM = Codes<HD, R>::UPM;
 #pragma unroll
@@ -125,7 +128,8 @@ __device__ __forceinline__ void codes_load(Codes<HD, R>& c, const AttnPagedArgs&
         const bool isv = u >= UPM;
         const int row = min((r0 & 15) + w / LRB * 4 + (w & 3), lim), cb = (w >> 2) & (NCB - 1);
         const size_t key = at + row;
-        c.c[j] = *reinterpret_cast<const u32x4*>((isv ? p.vpool : p.kpool) + key * HD + cb * 16);
+        const u32x4* src = reinterpret_cast<const u32x4*>((isv ? p.vpool : p.kpool) + key * HD + cb * 16);
+        c.c[j] = NT ? __builtin_nontemporal_load(src) : *src;
         c.e[j] = (isv ? p.vscale : p.kscale)[key];
     }
 }
@@ -302,14 +306,18 @@ __device__ __forceinline__ void scan_pages(const AttnPagedArgs& p, const int* ro
         if ((unsigned)row[i] >= (unsigned)p.n_pages) atomicMin(sh, i << p.page_shift);
 }
 
-// ---- short chunks: tiles of up to 32 rows; a block's four waves take every fourth step of 32 keys ----------------------------------------------------
+// ---- short chunks: tiles of up to 32 rows; a block's NW waves take every NW-th step of 32 keys ------------------------------------------------------------
 // (Cutting all sequences' keys into equal shares, whatever tiles they belong to, was measured too: 45.7 us against 45.8 for 32 x 1,000..4,000
 // keys, and 64.5 against 57.2 where all are 4,000 long: finding a share's place and a second tile per block cost what the balance gains.)
+// NW: as many waves as their images leave room for on a compute unit (128 KB for all but e4m3 at dim 64, two blocks there), two a SIMD but for bf16 at dim 128
+// (eight waves with one buffer each there: 106.4 us against 104.6 for 32 x 4,000 keys, 97.4 against 94.5 for 4 x 32,768)
+constexpr int rows_waves(int head_dim, bool fp8) { return head_dim == 128 && !fp8 ? 4 : 8; }
 template <int HD, bool FP8>
-__global__ __launch_bounds__(256, (HD == 128 && !FP8) ? 1 : 2) void attn_paged_rows_kernel(AttnPagedArgs p) {
+__global__ __launch_bounds__(64 * rows_waves(HD, FP8), rows_waves(HD, FP8) / 4) void attn_paged_rows_kernel(AttnPagedArgs p) {
+    constexpr int NW = rows_waves(HD, FP8), STRIDE = 32 * NW;      // keys between two steps of a wave
     extern __shared__ __attribute__((aligned(16))) char smem[];
     __shared__ int s_bad;
-    __shared__ float s_ml[4][RROWS][2];
+    __shared__ float s_ml[NW][RROWS][2];
     constexpr int IMG = 32 * HD;                     // elements of a step's K (or V) image
     constexpr int NBUF = FP8 ? 1 : 2;
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -328,7 +336,7 @@ __global__ __launch_bounds__(256, (HD == 128 && !FP8) ? 1 : 2) void attn_paged_r
         const int n_keys = min(t.n_vis, kmax);
         const int parts = ti < p.tps ? parts_of(n_keys, p.parts) : 1;
         if (s >= parts) continue;
-        const int chunk = part_keys<128>(n_keys, parts);
+        const int chunk = part_keys<STRIDE>(n_keys, parts);
         const int k0 = s * chunk, k1 = min(n_keys, k0 + chunk);
         float* part = parts > 1 ? p.part + ((size_t)((b * p.tps + ti) * p.nkv + kvh) * p.parts + s) * (RROWS * (HD + 2)) : nullptr;
         const int last = k1 - 1;
@@ -337,13 +345,13 @@ __global__ __launch_bounds__(256, (HD == 128 && !FP8) ? 1 : 2) void attn_paged_r
         Rows<HD> st;
         rows_init<HD>(st, p, t, kvh, 0, lane);
         const int key0 = k0 + 32 * wave;
-        // page ids of the wave's next 32 steps, two groups each: lane 2 i + g.  Waited for here, once in 4,096 keys: a wait inside the steps would be a wait
-        // for the DMA in flight.
+        // page ids of the wave's next 32 steps, two groups each: lane 2 i + g.  Waited for here, once in 32 steps: a wait inside the steps would be a wait for
+        // the DMA in flight.
         int pages = 0;
         auto look = [&](int key) {
-            const int i = (key - key0) >> 7;
+            const int i = (key - key0) / STRIDE;
             if ((i & 31) == 0) {
-                pages = src.row[min(key + (lane >> 1) * 128 + (lane & 1) * 16, last) >> p.page_shift];
+                pages = src.row[min(key + (lane >> 1) * STRIDE + (lane & 1) * 16, last) >> p.page_shift];
                 arrived(pages);
             }
             return i & 31;
@@ -356,8 +364,8 @@ __global__ __launch_bounds__(256, (HD == 128 && !FP8) ? 1 : 2) void attn_paged_r
                 const size_t at = src.group(kc, __builtin_amdgcn_readlane(pages, 2 * i + g)) * (HD * 2);
                 const unsigned dst = img_lds + (buf * 2 * IMG + g * 16 * HD) * 2;
                 if (kb + 15 <= last) {
-                    dma_rows(p.kpool + at, dst, off);
-                    dma_rows(p.vpool + at, dst + IMG * 2, off);
+                    dma_rows<true>(p.kpool + at, dst, off);
+                    dma_rows<true>(p.vpool + at, dst + IMG * 2, off);
                 } else {
                     const int lim = kb > last ? 0 : last - kc;              // (a group behind the last key: 16 copies of a key that is there)
                     dma_rows_clamped<HD, 16>(p.kpool + at, dst, 0, lim, lane);
@@ -374,26 +382,27 @@ __global__ __launch_bounds__(256, (HD == 128 && !FP8) ? 1 : 2) void attn_paged_r
 #pragma unroll
                 for (int g = 0; g < 2; ++g) {
                     const int kb = key + 16 * g, kc = min(kb, last & ~15);
-                    codes_load<HD, 16>(c[g], p, src.group(kc, __builtin_amdgcn_readlane(pages, 2 * i + g)), 0, kb > last ? 0 : min(last - kc, 15), lane);
+                    codes_load<HD, 16, true>(c[g], p, src.group(kc, __builtin_amdgcn_readlane(pages, 2 * i + g)), 0, kb > last ? 0 : min(last - kc, 15), lane);
                 }
             };
             if (key0 < k1) load_step(key0);
 #pragma unroll 1
-            for (int key = key0; key < k1; key += 128) {
+            for (int key = key0; key < k1; key += STRIDE) {
 #pragma unroll
                 for (int g = 0; g < 2; ++g) codes_store<HD, 16>(c[g], img, img + IMG, 16 * g, lane);
-                if (key + 128 < k1) load_step(key + 128);
+                if (key + STRIDE < k1) load_step(key + STRIDE);
                 attend32<HD>(st, img, img + IMG, 0, key, p.scale_log2, lane);
             }
         } else {
-            int buf = 0;
 #pragma unroll
             for (int i = 0; i < HD / 16; ++i) arrived(st.qf[i]);
             if (key0 < k1) dma_step(key0, 0);
+            int buf = 0;
 #pragma unroll 1
-            for (int key = key0; key < k1; key += 128) {
-                if (key + 128 < k1) {
-                    dma_step(key + 128, buf ^ 1);
+            for (int key = key0; key < k1; key += STRIDE) {
+                if (key + STRIDE < k1) {
+                    lds_read_done();                 // (the other buffer, in the step before)
+                    dma_step(key + STRIDE, buf ^ 1);
                     // this step's pieces have landed when only the next one's are still out
                     wait_vm<4 * PIECES<HD, 16>>();
                 } else {
@@ -403,10 +412,10 @@ __global__ __launch_bounds__(256, (HD == 128 && !FP8) ? 1 : 2) void attn_paged_r
                 buf ^= 1;
             }
         }
-        if (st.odd) add_odd<HD, FP8>(st, p, src, k0 + 32 * wave, 128, k1, lane);
+        if (st.odd) add_odd<HD, FP8>(st, p, src, k0 + 32 * wave, STRIDE, k1, lane);
         __syncthreads();                             // the images are dead; s_bad is set
-        scan_pages<256>(p, src.row, k0, k1, &s_bad);
-        // the four waves' rows, un-normalised, through LDS
+        scan_pages<64 * NW>(p, src.row, k0, k1, &s_bad);
+        // the waves' rows, un-normalised, through LDS
         const int r = lane & 31, h = lane >> 5;
         const float l = st.l + __shfl_xor(st.l, 32, 64);
         if (h == 0) { s_ml[wave][r][0] = st.m; s_ml[wave][r][1] = l; }
@@ -420,16 +429,16 @@ __global__ __launch_bounds__(256, (HD == 128 && !FP8) ? 1 : 2) void attn_paged_r
                         f32x4{st.o[d][4 * g4], st.o[d][4 * g4 + 1], st.o[d][4 * g4 + 2], st.o[d][4 * g4 + 3]};
         __syncthreads();
         const int bad = s_bad;
-        for (int i = tid; i < t.rows * (HD / 4); i += 256) {
+        for (int i = tid; i < t.rows * (HD / 4); i += 64 * NW) {
             const int row = i / (HD / 4), c4 = (i % (HD / 4)) * 4;
             float m = -INFINITY;
 #pragma unroll
-            for (int w = 0; w < 4; ++w) m = fmaxf(m, s_ml[w][row][0]);
+            for (int w = 0; w < NW; ++w) m = fmaxf(m, s_ml[w][row][0]);
             const float mu = m == -INFINITY ? 0.f : m;
             f32x4 a = {0.f, 0.f, 0.f, 0.f};
             float ls = 0.f;
 #pragma unroll
-            for (int w = 0; w < 4; ++w) {
+            for (int w = 0; w < NW; ++w) {
                 const float f = fast_exp2(s_ml[w][row][0] - mu);
                 const f32x4 x = *reinterpret_cast<const f32x4*>(reinterpret_cast<const float*>(smem) + ((size_t)w * RROWS + row) * HD + c4);
                 ls += s_ml[w][row][1] * f;
@@ -543,12 +552,12 @@ __global__ __launch_bounds__(256, 2) void attn_paged_tile_kernel(AttnPagedArgs p
         const int kb = k0 + 64 * i + (r0 & ~15), kc = min(kb, last & ~15);
         const size_t at = src.group(kc, __builtin_amdgcn_readlane(pages, i & 63));
         if constexpr (FP8) {
-            codes_load<HD, R>(c, p, at, r0, kb > last ? 0 : min(last - kc, 15), lane);
+            codes_load<HD, R, false>(c, p, at, r0, kb > last ? 0 : min(last - kc, 15), lane);
         } else {
             const unsigned dst = smem_lds + ((i & 1) * 2 * TILE + r0 * HD) * 2;
             if (kb + 15 <= last) {
-                dma_rows(p.kpool + at * (HD * 2), dst, off);
-                dma_rows(p.vpool + at * (HD * 2), dst + TILE * 2, off);
+                dma_rows<false>(p.kpool + at * (HD * 2), dst, off);
+                dma_rows<false>(p.vpool + at * (HD * 2), dst + TILE * 2, off);
             } else {
                 const int lim = kb > last ? 0 : last - kc;
                 dma_rows_clamped<HD, R>(p.kpool + at * (HD * 2), dst, r0, lim, lane);
@@ -728,7 +737,7 @@ Shape pick_shape(int n_tok, int B, int nkv, int G, int HD, bool fp8, long max_ke
     sh.tps = (int)(sh.ks ? (long)n_tok * G / rows + B : (mq * G + RROWS - 1) / RROWS);
     sh.rows = (int)(mq * G < rows ? mq * G : rows);      // rows of a tile, as far as the caller knows
     sh.tiles = sh.ks ? sh.tps : (long)sh.tps * B;
-    const long units = sh.tiles * nkv, slots = HD == 128 && !fp8 && !sh.ks ? 256 : 512;      // blocks that are resident at a time
+    const long units = sh.tiles * nkv, slots = sh.ks || (HD == 64 && fp8) ? 512 : 256;      // blocks that are resident at a time
     long parts = units > 0 ? slots / units : 1;
     if (parts > keys / MIN_KEYS) parts = keys / MIN_KEYS;
     if (parts > MAX_PARTS) parts = MAX_PARTS;
@@ -757,10 +766,11 @@ template <int HD, bool FP8>
 void launch(hipStream_t st, const AttnPagedArgs& p, const Shape& sh) {
     if (sh.ks == 2) return launch_tile<HD, FP8, 2>(st, p, sh);
     if (sh.ks == 1) return launch_tile<HD, FP8, 1>(st, p, sh);
-    const size_t lds = 4 * RROWS * HD * 4 * (FP8 ? 1 : 2);            // images (e4m3: one buffer of 32 rows K | V in bf16), at the end the four waves' rows in fp32
+    constexpr int NW = rows_waves(HD, FP8);
+    const size_t lds = NW * RROWS * HD * 4 * (FP8 ? 1 : 2);           // images (e4m3: one buffer of 32 rows K | V in bf16), at the end the waves' rows in fp32
     static const hipError_t once = hipFuncSetAttribute((const void*)attn_paged_rows_kernel<HD, FP8>, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
     (void)once;
-    hipLaunchKernelGGL((attn_paged_rows_kernel<HD, FP8>), dim3((unsigned)(sh.tiles * p.nkv * sh.parts)), dim3(256), lds, st, p);
+    hipLaunchKernelGGL((attn_paged_rows_kernel<HD, FP8>), dim3((unsigned)(sh.tiles * p.nkv * sh.parts)), dim3(64 * NW), lds, st, p);
     if (sh.parts > 1) launch_join<HD, RROWS>(st, p, sh);
 }
 

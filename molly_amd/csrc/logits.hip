@@ -24,24 +24,31 @@ struct LogitArgs {
 };
 
 // THREADS * 16 tokens a workgroup, four groups of four a thread: 16-byte loads and stores at whatever token the row's first aligned address falls on
-// (`shift` tokens of the first group lie in front of the row).  The logits are asked for in front of the history's pass.
+// (`shift` tokens of the first group lie in front of the row).  Logits, bias and mask are asked for in front of the
+// history's pass and wait in registers.
 template <int THREADS, bool BF16, bool HIST>
 __global__ __launch_bounds__(THREADS) void logits_kernel(LogitArgs p) {
     constexpr int SLICE = THREADS * 16;
     __shared__ unsigned cnt[HIST ? SLICE : 1];
     const int row = blockIdx.y, t = threadIdx.x;
     const size_t x0 = (size_t)row * p.ldx, o0 = (size_t)row * p.ldo;
-    // tokens in front of the row in its first aligned group; -1: the two rows are aligned differently, one token at a time
+    // tokens of the first aligned group that lie in front of the row; where the two rows are aligned differently: one token at a time
     const int sx = (int)((((uintptr_t)p.x >> (BF16 ? 1 : 2)) + x0) & 3), so = (int)((((uintptr_t)p.out >> 2) + o0) & 3);
     const int shift = sx == so ? sx : 0;
     const bool vec = sx == so;
     const int v0 = blockIdx.x * SLICE - shift;       // token of the slice's first place
     if (v0 >= p.V) return;
+    const unsigned* m = p.mask ? p.mask + (size_t)row * p.ldm : nullptr;
+    const float* bias = p.bias ? p.bias + (size_t)row * p.ldb : nullptr;
+    const bool bias_vec = bias && ((uintptr_t)(bias + v0) & 15) == 0;
     float x[4][4];
+    f32x4 add[4];
+    unsigned wa[4], wb[4];                           // mask words of the group's first and last token
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
         const int v = v0 + (j * THREADS + t) * 4;
-        if (vec && v >= 0 && v + 4 <= p.V) {
+        const bool whole = v >= 0 && v + 4 <= p.V;
+        if (vec && whole) {
             if constexpr (BF16) {
                 const u32x2 w = *reinterpret_cast<const u32x2*>((const bf16_t*)p.x + x0 + v);
                 x[j][0] = bflo(w[0]); x[j][1] = bfhi(w[0]); x[j][2] = bflo(w[1]); x[j][3] = bfhi(w[1]);
@@ -54,6 +61,18 @@ __global__ __launch_bounds__(THREADS) void logits_kernel(LogitArgs p) {
 #pragma unroll
             for (int e = 0; e < 4; ++e)
                 x[j][e] = v + e < 0 || v + e >= p.V ? 0.f : BF16 ? bf2f(((const bf16_t*)p.x)[x0 + v + e]) : ((const float*)p.x)[x0 + v + e];
+        }
+        if (bias) {
+            if (whole && bias_vec) {
+                add[j] = *reinterpret_cast<const f32x4*>(bias + v);
+            } else {
+#pragma unroll
+                for (int e = 0; e < 4; ++e) add[j][e] = v + e >= 0 && v + e < p.V ? bias[v + e] : 0.f;
+            }
+        }
+        if (m && v + 4 > 0 && v < p.V) {
+            wa[j] = m[max(v, 0) >> 5];
+            wb[j] = m[min(v + 3, p.V - 1) >> 5];
         }
     }
     if constexpr (HIST) {
@@ -70,9 +89,6 @@ __global__ __launch_bounds__(THREADS) void logits_kernel(LogitArgs p) {
         __syncthreads();
     }
     const float rep = p.rep_v ? p.rep_v[row] : p.rep, pres = p.pres_v ? p.pres_v[row] : p.pres, freq = p.freq_v ? p.freq_v[row] : p.freq;
-    const unsigned* m = p.mask ? p.mask + (size_t)row * p.ldm : nullptr;
-    const float* bias = p.bias ? p.bias + (size_t)row * p.ldb : nullptr;
-    const bool bias_vec = bias && ((uintptr_t)(bias + v0) & 15) == 0;
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
         const int v = v0 + (j * THREADS + t) * 4;
@@ -84,25 +100,15 @@ __global__ __launch_bounds__(THREADS) void logits_kernel(LogitArgs p) {
             for (int e = 0; e < 4; ++e)
                 if (c[e]) x[j][e] = (x[j][e] < 0.f ? x[j][e] * rep : x[j][e] / rep) - pres - freq * (float)c[e];
         }
-        if (bias) {
-            if (whole && bias_vec) {
-                const f32x4 b = *reinterpret_cast<const f32x4*>(bias + v);
+        if (bias)
 #pragma unroll
-                for (int e = 0; e < 4; ++e) x[j][e] += b[e];
-            } else {
-#pragma unroll
-                for (int e = 0; e < 4; ++e) x[j][e] += v + e >= 0 && v + e < p.V ? bias[v + e] : 0.f;
-            }
-        }
-        if (m) {
-            const int first = max(v, 0), last = min(v + 3, p.V - 1);
-            const unsigned wa = m[first >> 5], wb = (last >> 5) != (first >> 5) ? m[last >> 5] : wa;
+            for (int e = 0; e < 4; ++e) x[j][e] += add[j][e];
+        if (m)
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
-                const unsigned w = ((v + e) >> 5) == (first >> 5) ? wa : wb;
+                const unsigned w = ((v + e) >> 5) == (max(v, 0) >> 5) ? wa[j] : wb[j];
                 if (!((w >> ((v + e) & 31)) & 1u)) x[j][e] = -INFINITY;
             }
-        }
         float* o = p.out + o0 + v;
         if (vec && whole) {
             *reinterpret_cast<f32x4*>(o) = f32x4{x[j][0], x[j][1], x[j][2], x[j][3]};

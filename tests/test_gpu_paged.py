@@ -28,10 +28,6 @@ def gen(seed):
     return torch.Generator(device=DEV).manual_seed(seed)
 
 
-def nan_like(x):
-    return torch.full_like(x, math.nan)
-
-
 # ---- store and read ---------------------------------------------------------------------------------------------------------------
 def store_inputs(n, nq, nkv, hd, seed, scale=1.0):
     g = gen(seed)
@@ -175,7 +171,7 @@ def case(new, keys, nh, nkv, hd, page, fp8, seed=0):
     return q, kp, vp, ks, vs, table, cu, keys, cu_t, len_t
 
 
-def check(out, q, kp, vp, ks, vs, table, cu, keys, nh, scale=None, bound=None):
+def check(out, q, kp, vp, ks, vs, table, cu, keys, nh, scale=None):
     hd = kp.shape[-1]
     ref, mag = C.attend(q, C.held(kp, ks), C.held(vp, vs), table, cu, keys, nh, hd ** -0.5 if scale is None else scale)
     got = out.double().view(ref.shape)
@@ -247,10 +243,16 @@ def test_attn_paged_many_sequences(kind, fp8):
 
 @pytest.mark.parametrize("new,keys", [([1, 1], [2100, 33]), ([90, 3], [400, 3])])
 def test_attn_paged_e4m3_is_bf16_of_the_held_values(new, keys):
+    """The held values are exact in bf16, so both calls compute the same numbers: bit for bit where the keys go by in the same order (the tile kernel),
+    within the bound of either where a block has another number of waves to deal them to (single steps: the sums are taken in another order, and the
+    parts' maxima, which P is rounded against, differ)."""
     q, kp, vp, ks, vs, table, cu, keys, cu_t, len_t = case(new, keys, 8, 2, 128, 32, True, seed=5)
     a = ops().attn_paged(q, kp, vp, table, cu_t, len_t, 8, kscale=ks, vscale=vs, max_q=max(new), max_kv=max(keys))
     b = ops().attn_paged(q, C.held(kp, ks).bfloat16(), C.held(vp, vs).bfloat16(), table, cu_t, len_t, 8, max_q=max(new), max_kv=max(keys))
-    assert torch.equal(a, b)
+    for x in (a, b):
+        check(x, q, kp, vp, ks, vs, table, cu, keys, 8)
+    if max(new) * 4 > 32:
+        assert torch.equal(a, b)
 
 
 @pytest.mark.parametrize("fp8", [False, True])
@@ -429,8 +431,9 @@ def test_refusals():
         (ValueError, lambda: o.attn_paged(q, bf, bf, table, cu_t[:-1], len_t, 4)),
         (ValueError, lambda: o.attn_paged(q, bf, bf, table, cu_t, len_t.cpu(), 4)),
         (ValueError, lambda: o.attn_paged(q, bf.transpose(1, 2), bf.transpose(1, 2), table, cu_t, len_t, 4)),
-        (RuntimeError, lambda: o.attn_paged(q[:, 1:].clone()[:, :255], bf, bf, table, cu_t, len_t, 4) if False else o.attn_paged(
-            torch.zeros(5 * 256 + 1, dtype=torch.bfloat16, device=DEV)[1:].view(5, 256), bf, bf, table, cu_t, len_t, 4)),      # not 16-byte aligned
+        (RuntimeError, lambda: o.attn_paged(torch.zeros(5 * 256 + 1, dtype=torch.bfloat16, device=DEV)[1:].view(5, 256), bf, bf, table, cu_t, len_t,
+                                            4)),                                                                          # not 16-byte aligned
+        (RuntimeError, lambda: o.attn_paged(q, bf, bf, table, cu_t, len_t, 4, scale=-1.0)),
         (RuntimeError, lambda: o.attn_paged(q, bf[:, :, :8].contiguous(), bf[:, :, :8].contiguous(), table, cu_t, len_t, 4)),     # pages of 8
         (RuntimeError, lambda: o.attn_paged(q[:, :128], bf[..., :32].contiguous(), bf[..., :32].contiguous(), table, cu_t, len_t, 4)),   # dim 32
         (RuntimeError, lambda: o.attn_paged(q.cpu(), bf.cpu(), bf.cpu(), table.cpu(), cu_t.cpu(), len_t.cpu(), 4)),

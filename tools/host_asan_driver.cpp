@@ -151,6 +151,30 @@ int main(int argc, char** argv) {
         }
     }
 
+    // ---- the paged cache, its attention and the logit processors
+    for (int it = 0; it < n_attn; ++it) {
+        const int hd = r.pick((const int[]){64, 64, 128, 128, 128, 96}), nkv = r.pick((const int[]){1, 2, 4, 8, 20}), group = r.pick((const int[]){1, 2, 3, 4, 7, 40});
+        const int nh = nkv * group + (it % 50 == 0), page = r.pick((const int[]){16, 32, 64, 128, 256, 48});
+        const int Bn = r.pick((const int[]){0, 1, 3, 32, 200, 70000}), max_pages = r.pick((const int[]){0, 1, 17, 512, 1 << 20, 1 << 27});
+        const int new_q = r.pick((const int[]){1, 1, 1, 5, 300, 4096}), e4m3 = (int)(r.next() & 1), max_q = (int)(r.next() & 1) ? new_q : 0;
+        const int n = r.pick((const int[]){0, Bn, Bn < 1000 ? Bn * new_q : Bn, 1 << 28}), max_kv = (int)(r.next() & 1) ? r.range(1, 40000) : 0;
+        const long need = molly_attn_paged_workspace(n, Bn, nh, nkv, hd, page, max_pages, e4m3, max_q, max_kv);
+        seen(molly_attn_paged(st, A, C, B, fake(4), e4m3 ? fake(5) : nullptr, e4m3 ? fake(6) : nullptr, (const int*)fake(7), (const int*)fake(8),
+                              (const int*)fake(9), n, Bn, 1000, page, max_pages, max_pages, nh, nkv, hd, nh * hd, nh * hd, 0.125f, max_q, max_kv,
+                              (it & 1) ? (float*)fake(11) : nullptr, need), "attn_paged");
+        const int rows = r.pick((const int[]){0, 1, 33, 5000, 1 << 20, 1 << 30}), nq = r.pick((const int[]){0, nh});
+        seen(molly_paged_kv_append(st, A, B, nq ? C : nullptr, nq ? C : nullptr, fake(4), fake(5), e4m3 ? fake(6) : nullptr, e4m3 ? fake(7) : nullptr,
+                                   (const int*)fake(8), rows, r.pick((const int[]){1, 1000, 1 << 20, 1 << 28}), page, nq, nkv, hd, nh * hd, nkv * hd, nkv * hd, nh * hd,
+                                   (it & 1) ? fake(9) : nullptr, (it & 2) ? fake(10) : nullptr, (it & 4) ? (const float*)fake(11) : nullptr,
+                                   (it & 4) ? (const float*)fake(12) : nullptr, (it & 4) ? (const int*)fake(13) : nullptr, 4096, 1e-6f), "paged_kv_append");
+        seen(molly_paged_kv_read(st, fake(4), fake(5), e4m3 ? fake(6) : nullptr, e4m3 ? fake(7) : nullptr, (const int*)fake(8), rows, 1000, page, nkv, hd, A, B,
+                                 nkv * hd, nkv * hd), "paged_kv_read");
+        const int V = r.pick((const int[]){1, 1000, 50257, 151936, 1 << 30}), hist = r.pick((const int[]){0, 5, 4096, 4097, 100000});
+        seen(molly_process_logits(st, A, (int)(r.next() & 1), (float*)C, rows, V, V, V, hist ? (const int64_t*)B : nullptr, (const int*)fake(4), hist, hist, 1.1f, 0.f, 0.f,
+                                  nullptr, (const float*)fake(5), nullptr, (it & 1) ? (const float*)fake(6) : nullptr, 0, (it & 2) ? fake(7) : nullptr,
+                                  (V + 31) / 32), "process_logits");
+    }
+
     // ---- elementwise / optimizer / batch entry points at edge sizes
     const long ns[] = {0, 1, 7, 8, 64, 1000, 4096, 1L << 20, (1L << 31) - 8, 1L << 31, 3L << 30};
     const int rows_[] = {0, 1, 3, 64, 4096, 16384, 65536};

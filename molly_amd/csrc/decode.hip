@@ -171,12 +171,17 @@ __global__ __launch_bounds__(64 * NW) void attn_decode_kernel(DecodeArgs p) {
                 sc[u] = ok[u] ? d * p.qscale : NEG_BIG;
                 mx = fmaxf(mx, sc[u]);
             }
-            const float c = __builtin_amdgcn_exp2f(m[g] - mx);
-            m[g] = mx;
-            float lsum = l[g] * c;
-            const f32x2 c2 = f32x2{c, c};
+            // (only where some lane's maximum grew: a factor of 2^0 changes nothing, and it rarely grows behind the first keys.  With scalar fmas for p . v this
+            // is what keeps the loop on HBM's side of the balance: 32 x 3,100 keys, 4 heads a kv head, 77.9 us without the branch, 72.7 with it)
+            if (__any(mx > m[g])) {
+                const float c = __builtin_amdgcn_exp2f(m[g] - mx);
+                m[g] = mx;
+                l[g] *= c;
+                const f32x2 c2 = f32x2{c, c};
 #pragma unroll
-            for (int e = 0; e < 4; ++e) acc[g][e] *= c2;
+                for (int e = 0; e < 4; ++e) acc[g][e] *= c2;
+            }
+            float lsum = l[g];
 #pragma unroll
             for (int u = 0; u < U; ++u) {
                 const float pe = __builtin_amdgcn_exp2f(sc[u] - mx);

@@ -3,7 +3,11 @@
 left-padded prompt, positions = cumsum(mask)-1 as HF does: HF:generation/utils.py:751-773) and writes every layer's
 post-RoPE K and V into a token-major cache; each decode step is M = batch GEMMs + one `molly_attn_decode` per layer.
 Token selection (temperature / top-k / top-p / repetition penalty, HF logits processors) runs on the [B, V] logits with
-torch ops — a few KB of work per step, not a kernel target.
+torch ops — a few KB of work per step, not a kernel target; presence / frequency penalties, biases and masks of allowed tokens are one kernel
+(`molly_process_logits`).
+
+kv_cache="paged" | "paged_e4m3" keeps K and V in pages (molly_amd.paged): no padding in the cache nor in the prompt's rows, the prompt in chunks of
+`prefill_chunk` tokens a sequence, attention over the pages for chunks and decode steps alike (`molly_attn_paged`), e4m3 at half the bytes.
 """
 from __future__ import annotations
 
@@ -19,8 +23,17 @@ BF16 = torch.bfloat16
 
 
 class GenerationSession:
-    def __init__(self, model, max_new_tokens: int, use_graph: bool = None):
+    def __init__(self, model, max_new_tokens: int, use_graph: bool = None, kv_cache: str = "dense", prefill_chunk: Optional[int] = None,
+                 page_size: int = 64):
+        """kv_cache: 'dense' (one [B, T + max_new] rectangle a layer), 'paged' or 'paged_e4m3'; prefill_chunk: most prompt tokens of a sequence taken at a
+        time (paged caches; None: the whole prompt)."""
         import os
+        if kv_cache not in ("dense", "paged", "paged_e4m3"):
+            raise ValueError(f"GenerationSession: kv_cache must be 'dense', 'paged' or 'paged_e4m3', got {kv_cache!r}")
+        if prefill_chunk is not None and (kv_cache == "dense" or prefill_chunk < 1):
+            raise ValueError("GenerationSession: prefill_chunk is a positive number of tokens, for the paged caches")
+        self.kv_cache, self.prefill_chunk, self.page_size = kv_cache, prefill_chunk, page_size
+        self.paged = None                               # PagedKVCache of a paged session
         self.use_graph = (os.environ.get("MOLLY_DECODE_GRAPH", "1") != "0") if use_graph is None else use_graph
         self.m = model
         self.rt = model._runtime()
@@ -50,6 +63,8 @@ class GenerationSession:
         ops.ensure_gemm_workspace(32 * 4 * max(B, 8) * max(2 * e.ff, e.nqkv), dev)
         hs, _ = m._embed_and_inject(m._stage(input_ids, None, None, omic_ids, omic_info_list, want_sort=False), False)
         e.reserve(B * T, B, T, training=False)
+        if self.kv_cache != "dense":
+            return self._prefill_paged(hs, mask, pos)
         # rope tables must cover prompt + generated positions
         from .qwen3 import rope_tables
         self.cos, self.sin = rope_tables(self.Tmax, e.hd, e.cfg.rope_theta, dev, e.rope_table_dtype)
@@ -77,23 +92,100 @@ class GenerationSession:
                               kcache=self.kc[i].view(B * self.Tmax, nkvd), vcache=self.vc[i].view(B * self.Tmax, nkvd), slot=rows)
             ops.attn_fwd(a["qk"][:, :nq], a["qk"][:, nq:], a["qkv"][:, e.nqk:], B, T, e.nh, e.nkv, e.hd, e.hd ** -0.5, True,
                          lo, hi, out=a["attn"], lse=False)
-            ops.gemm_nt(a["attn"], w["o"], out=a["x2"], res=x)
-            self._lora(i, "o_proj", a["attn"], a["x2"])
-            ops.rmsnorm_fwd(a["x2"], w["ln2"], e.cfg.rms_norm_eps, out=a["xn2"])
-            if e.fused_swiglu:                                              # (no live adapters) SwiGLU in the gate|up GEMM's epilogue, as in training
-                ops.gemm_gate_up_swiglu(a["xn2"], w["gu"], a["gu"], a["act"])
-            else:
-                ops.gemm_nt(a["xn2"], w["gu"], out=a["gu"])
-                self._lora(i, "gate_proj", a["xn2"], a["gu"][:, :e.ff])
-                self._lora(i, "up_proj", a["xn2"], a["gu"][:, e.ff:])
-                ops.swiglu_fwd(a["gu"], out=a["act"])
-            ops.gemm_nt(a["act"], w["down"], out=e.x_out, res=a["x2"])
-            self._lora(i, "down_proj", a["act"], e.x_out)
+            self._layer_tail(i, a, x, e.x_out)
             x = e.x_out
         last = x.view(B, T, e.h)[:, T - 1, :].contiguous()                    # left-padded prompts end at T-1
         self.cur_len = T
         self._alloc_step(B)
         return self._head(last)
+
+    def _layer_tail(self, i, a, x, out):
+        """From the attention's output to the layer's: o-projection + residual, norm, SwiGLU, down-projection + residual."""
+        e = self.eng
+        w = e.W[i]
+        ops.gemm_nt(a["attn"], w["o"], out=a["x2"], res=x)
+        self._lora(i, "o_proj", a["attn"], a["x2"])
+        ops.rmsnorm_fwd(a["x2"], w["ln2"], e.cfg.rms_norm_eps, out=a["xn2"])
+        if e.fused_swiglu:                                              # (no live adapters) SwiGLU in the gate|up GEMM's epilogue, as in training
+            ops.gemm_gate_up_swiglu(a["xn2"], w["gu"], a["gu"], a["act"])
+        else:
+            ops.gemm_nt(a["xn2"], w["gu"], out=a["gu"])
+            self._lora(i, "gate_proj", a["xn2"], a["gu"][:, :e.ff])
+            self._lora(i, "up_proj", a["xn2"], a["gu"][:, e.ff:])
+            ops.swiglu_fwd(a["gu"], out=a["act"])
+        ops.gemm_nt(a["act"], w["down"], out=out, res=a["x2"])
+        self._lora(i, "down_proj", a["act"], out)
+
+    def _prefill_paged(self, hs, mask, pos) -> torch.Tensor:
+        """The prompts' tokens without their padding, `prefill_chunk` of every sequence at a time, through the layers and into the pages."""
+        from .paged import PagedKVCache
+        from .qwen3 import rope_tables
+        e, dev = self.eng, self.rt.dev
+        B, T = mask.shape
+        n_valid = mask.sum(1).tolist()
+        if min(n_valid) == 0:
+            raise ValueError("generate: a prompt without tokens")
+        L, nq, nk = e.L, e.nh * e.hd, e.nkv * e.hd
+        most = max(n_valid) + self.max_new
+        self.cos, self.sin = rope_tables(most, e.hd, e.cfg.rope_theta, dev, e.rope_table_dtype)
+        need = [-(-(n + self.max_new) // self.page_size) for n in n_valid]
+        self.paged = PagedKVCache(L, sum(need), e.nkv, e.hd, self.page_size, "bf16" if self.kv_cache == "paged" else "e4m3", dev)
+        pages = [self.paged.allocate(n + self.max_new) for n in n_valid]
+        self.table = self.paged.block_table(pages)
+        # places of every sequence's tokens in the pools, [B, pages * page size] (behind the last page: none)
+        at = self.table.cpu()
+        places = torch.where(at[:, :, None] < 0, -1, at[:, :, None] * self.page_size + torch.arange(self.page_size, dtype=torch.int32)).flatten(1)
+        self.places = places.to(dev)
+        cols = [mask[b].nonzero().flatten() for b in range(B)]                # the columns that hold tokens
+        chunk = self.prefill_chunk or max(n_valid)
+        if e.lora is not None:
+            self.lt = torch.empty(max(sum(min(chunk, n) for n in n_valid), B), e.lora.rp, dtype=BF16, device=dev)
+        last = torch.empty(B, e.h, dtype=BF16, device=dev)
+        i32 = lambda x: torch.tensor(x, dtype=torch.int32, device=dev)        # noqa: E731
+        for c0 in range(0, max(n_valid), chunk):
+            new = [max(0, min(n - c0, chunk)) for n in n_valid]
+            n = sum(new)
+            rows = torch.cat([b * T + cols[b][c0:c0 + k] for b, k in enumerate(new)]).to(torch.int32).to(dev)
+            positions = torch.cat([pos[b, cols[b][c0:c0 + k]] for b, k in enumerate(new)]).to(torch.int32).to(dev)
+            slot = torch.cat([places[b, c0:c0 + k] for b, k in enumerate(new)]).to(torch.int32).to(dev)
+            cu = [0]
+            for k in new:
+                cu.append(cu[-1] + k)
+            cu_q, kv_len = i32(cu), i32([min(c0 + chunk, m) for m in n_valid])
+            a = {k: v[:n] for k, v in e.A[0].items() if k in ("xn", "qkv", "qk", "attn", "x2", "xn2", "gu", "act")}
+            x, out = (torch.empty(n, e.h, dtype=BF16, device=dev) for _ in range(2))
+            ops.copy_rows(hs, x, n, src_idx32=rows)
+            for i in range(L):
+                w = e.W[i]
+                ops.rmsnorm_fwd(x, w["ln1"], e.cfg.rms_norm_eps, out=a["xn"])
+                ops.gemm_nt(a["xn"], w["qkv"], out=a["qkv"])
+                self._lora(i, "q_proj", a["xn"], a["qkv"][:, :nq])
+                self._lora(i, "k_proj", a["xn"], a["qkv"][:, nq:nq + nk])
+                self._lora(i, "v_proj", a["xn"], a["qkv"][:, nq + nk:])
+                self._attend_paged(i, a["qkv"], a["qk"], a["attn"], slot, positions, cu_q, kv_len, max(new), min(c0 + chunk, max(n_valid)))
+                self._layer_tail(i, a, x, out)
+                x, out = out, x
+            done = [b for b, m in enumerate(n_valid) if c0 < m <= c0 + chunk]  # their last token was in this chunk
+            if done:
+                ops.copy_rows(x, last, len(done), src_idx32=i32([cu[b + 1] - 1 for b in done]), dst_idx32=i32(done))
+        self.cur_len = T
+        self._alloc_step(B)
+        self.hi.copy_(self.n_valid + 1)                                        # keys once the step's own token is in the pages
+        self.cu_one = torch.arange(B + 1, dtype=torch.int32, device=dev)
+        self.max_kv = most
+        floats = ops.attn_paged_workspace(B, B, e.nh, e.nkv, e.hd, self.page_size, self.table.shape[1], self.kv_cache == "paged_e4m3", 1, most)
+        self.dec_ws = torch.empty(max(floats, 4), dtype=torch.float32, device=dev)
+        return self._head(last)
+
+    def _attend_paged(self, i, qkv, qk, attn, slot, positions, cu_q, kv_len, max_q, max_kv, workspace=None):
+        """One layer's q/k-norm, rotary and cache write in one launch, then attention over the pages."""
+        e = self.eng
+        w, nq = e.W[i], e.nh * e.hd
+        pools = self.paged.layer(i)
+        q = ops.paged_kv_append(qkv[:, nq:e.nqk], qkv[:, e.nqk:], slot=slot, q=qkv[:, :nq], q_out=qk[:, :nq], qw=w["qn"], kw=w["kn"], cos=self.cos,
+                                sin=self.sin, positions=positions, eps=e.cfg.rms_norm_eps, **pools)
+        ops.attn_paged(q, block_table=self.table, cu_q=cu_q, kv_len=kv_len, n_heads=e.nh, max_q=max_q, max_kv=max_kv, out=attn, workspace=workspace,
+                       **pools)
 
     def _lora(self, i, mod, x, y):
         """live (un-merged) adapter: y += s * (x A^T) B^T, no dropout at inference (PEFT eval mode)."""
@@ -143,7 +235,9 @@ class GenerationSession:
         # the larger matrices) — residual + next RMSNorm behind o / down, SwiGLU behind gate|up — and the cache appends into norm + rope
         fuse = e.lora is None and os.environ.get("MOLLY_DECODE_FUSE", "1") != "0"
         H = x.shape[1]
-        f_qkv = fuse and ops.gemm_rows_tail_supported(B, nq + 2 * nkvd, H, "qkv")
+        if self.paged is not None:                      # the places of the step's tokens
+            self.slot.copy_(torch.gather(self.places, 1, self.pos.long()[:, None]).squeeze(1))
+        f_qkv = self.paged is None and fuse and ops.gemm_rows_tail_supported(B, nq + 2 * nkvd, H, "qkv")
         # (the fused attention is built for groups of 1 / 2 / 4 / 8 query heads per KV head: other ratios take the plain path)
         f_att = (f_qkv and e.hd in (64, 128) and e.nh % e.nkv == 0 and e.nh // e.nkv in (1, 2, 4, 8)
                  and os.environ.get("MOLLY_DECODE_FUSE_ATTN", "1") != "0")
@@ -155,7 +249,8 @@ class GenerationSession:
             w = e.W[i]
             if not normed:
                 ops.rmsnorm_fwd(x, w["ln1"], eps, out=s["xn"])
-            kc_i, vc_i = self.kc[i].view(B * self.Tmax, nkvd), self.vc[i].view(B * self.Tmax, nkvd)
+            if self.paged is None:
+                kc_i, vc_i = self.kc[i].view(B * self.Tmax, nkvd), self.vc[i].view(B * self.Tmax, nkvd)
             if f_att:                                   # projection as K-slice slabs; everything up to the attention output in ONE launch
                 slabs, n_slabs = ops.gemm_rows_slabs(s["xn"], w["qkv"])
                 ops.attn_decode_qkv(slabs, n_slabs, w["qn"], w["kn"], self.cos, self.sin, self.pos, eps, self.kc[i], self.vc[i], self.slot,
@@ -169,7 +264,9 @@ class GenerationSession:
                 self._lora(i, "q_proj", s["xn"], s["qkv"][:, :nq])
                 self._lora(i, "k_proj", s["xn"], s["qkv"][:, nq:nq + nkvd])
                 self._lora(i, "v_proj", s["xn"], s["qkv"][:, nq + nkvd:])
-                if fuse:
+                if self.paged is not None:
+                    self._attend_paged(i, s["qkv"], s["qk"], s["attn"], self.slot, self.pos, self.cu_one, self.hi, 1, self.max_kv, self.dec_ws)
+                elif fuse:
                     ops.norm_rope_fwd(s["qkv"], s["qk"], e.nh, e.nkv, e.hd, 1, w["qn"], w["kn"], self.cos, self.sin, positions=self.pos,
                                       eps=eps, kcache=kc_i, vcache=vc_i, slot=self.slot)
                 else:
@@ -177,7 +274,7 @@ class GenerationSession:
                                       positions=self.pos, eps=eps)
                     ops.copy_rows(s["qk"][:, nq:], kc_i, B, dst_idx32=self.slot)
                     ops.copy_rows(s["qkv"][:, e.nqk:], vc_i, B, dst_idx32=self.slot)
-            if not f_att:
+            if not f_att and self.paged is None:
                 ops.attn_decode(s["qk"], self.kc[i], self.vc[i], s["attn"], self.lo, self.hi, B, self.Tmax, e.nh, e.nkv, e.hd,
                                 e.hd ** -0.5, kv_len_hint=self.Tmax, workspace=self.dec_ws)
             if f_o:
@@ -218,6 +315,15 @@ class GenerationSession:
         if bool((rows == torch.arange(rows.numel(), device=rows.device)).all()):
             return                                      # every beam stays where it is: nothing moves
         n = self.cur_len
+        if self.paged is not None:
+            # what the rows hold of their pages moves; a row's own page list stays (the captured graph's tables)
+            used = -(-int(self.hi.max()) // self.page_size)
+            src, dst = self.table[rows, :used], self.table[:, :used]
+            moved = (src != dst) & (src >= 0) & (dst >= 0)
+            self.paged.copy_pages(src[moved].long(), dst[moved].long())
+            for t in (self.pos, self.hi, self.lo, self.n_valid):
+                t.copy_(t.index_select(0, rows))
+            return
         # layer by layer: the temporary is one layer's filled cache (B x n x kv width), not all L of them — at Qwen3-8B with a 3 k-token
         # prompt and B * num_beams rows the whole-cache gather was a multi-GB allocation beside a cache sized for 3,072 new tokens
         for i in range(self.kc.shape[0]):
@@ -323,24 +429,63 @@ class NoRepeatNGram:
         return logits
 
 
+def allowed_bits(allowed, vocab: int, device) -> torch.Tensor:
+    """int32 [rows, ceil(vocab / 32)] for ops.process_logits: bit v % 32 of word v // 32 set for every v in allowed[row]."""
+    rows, words = len(allowed), (vocab + 31) // 32
+    on = torch.zeros(rows, words * 32, dtype=torch.bool)
+    for r, ids in enumerate(allowed):
+        ids = torch.as_tensor(ids, dtype=torch.int64).reshape(-1)
+        if ids.numel() == 0:
+            raise ValueError(f"generate: no token is allowed in row {r}")
+        if int(ids.min()) < 0 or int(ids.max()) >= vocab:
+            raise ValueError(f"generate: an allowed token of row {r} lies outside the vocabulary of {vocab}")
+        on[r, ids] = True
+    w = (on.view(rows, words, 32).long() << torch.arange(32)).sum(-1)
+    return torch.where(w >= 1 << 31, w - (1 << 32), w).to(torch.int32).to(device)
+
+
+def _bias_row(logit_bias, vocab: int, device) -> torch.Tensor:
+    """{token: bias} or a [vocab] tensor -> fp32 [vocab]"""
+    if torch.is_tensor(logit_bias):
+        if tuple(logit_bias.shape) != (vocab,):
+            raise ValueError(f"generate: logit_bias must have one value for each of {vocab} tokens, got {tuple(logit_bias.shape)}")
+        return logit_bias.to(device=device, dtype=torch.float32).contiguous()
+    b = torch.zeros(vocab)
+    for t, x in logit_bias.items():
+        if not 0 <= int(t) < vocab:
+            raise ValueError(f"generate: logit_bias of token {t} outside the vocabulary of {vocab}")
+        b[int(t)] = float(x)
+    return b.to(device)
+
+
 @torch.no_grad()
 def generate(model, input_ids, attention_mask=None, omic_ids=None, omic_info_list=None, max_new_tokens=3072, do_sample=True,
              temperature=0.8, top_p=0.95, top_k=None, repetition_penalty=None, pad_token_id=None, eos_token_id=None,
              generator: Optional[torch.Generator] = None, no_repeat_ngram_size: Optional[int] = None, num_beams: int = 1,
-             length_penalty: float = 1.0, early_stopping=False, min_new_tokens: int = 0) -> torch.Tensor:
+             length_penalty: float = 1.0, early_stopping=False, min_new_tokens: int = 0, kv_cache: str = "dense",
+             prefill_chunk: Optional[int] = None, presence_penalty: float = 0.0, frequency_penalty: float = 0.0, logit_bias=None,
+             prefix_allowed_tokens_fn=None) -> torch.Tensor:
     """Returns the NEW tokens only, int64 [B, n_new] (what HF returns when called with inputs_embeds and no input_ids).
     min_new_tokens: HF's MinNewTokensLengthLogitsProcessor — the eos scores are -inf while fewer new tokens than that exist (it runs among
-    the processors, in front of the warpers)."""
+    the processors, in front of the warpers).
+    kv_cache / prefill_chunk: GenerationSession.  presence_penalty, frequency_penalty (subtracted once / once an occurrence for every token generated
+    so far), logit_bias ({token: added} or [V]) and prefix_allowed_tokens_fn(row, generated ids) -> allowed tokens (HF's) go, with the repetition
+    penalty, through one kernel in front of the warpers (ops.process_logits)."""
+    extra = bool(presence_penalty or frequency_penalty or logit_bias is not None or prefix_allowed_tokens_fn is not None)
     if num_beams and num_beams > 1:
         if min_new_tokens:
             raise NotImplementedError("generate: min_new_tokens together with molly_num_beams > 1 is not built")
+        if extra or kv_cache != "dense" or prefill_chunk is not None:
+            raise NotImplementedError("generate: the paged caches, presence / frequency penalties, biases and allowed tokens together with "
+                                      "molly_num_beams > 1 are not built")
         return _generate_beams(model, input_ids, attention_mask, omic_ids, omic_info_list, max_new_tokens, do_sample, repetition_penalty,
                                pad_token_id, eos_token_id, no_repeat_ngram_size, int(num_beams), length_penalty, early_stopping,
                                temperature, top_k, top_p, generator)
-    sess = GenerationSession(model, max_new_tokens)
+    sess = GenerationSession(model, max_new_tokens, kv_cache=kv_cache, prefill_chunk=prefill_chunk)
     logits = sess.prefill(input_ids, attention_mask, omic_ids, omic_info_list)
     B = input_ids.shape[0]
     dev = logits.device
+    bias = None if logit_bias is None else _bias_row(logit_bias, logits.shape[1], dev)
     eos = None if eos_token_id is None else torch.as_tensor(eos_token_id, device=dev).reshape(-1)
     pad = pad_token_id if pad_token_id is not None else (int(eos[0]) if eos is not None else 0)
     out = torch.empty(B, 0, dtype=torch.int64, device=dev)
@@ -364,12 +509,21 @@ def generate(model, input_ids, attention_mask=None, omic_ids=None, omic_info_lis
         if min_new_tokens and it < min_new_tokens and eos is not None:
             logits = logits.clone()
             logits[:, eos] = float("-inf")
+        penalty = repetition_penalty
+        if extra:
+            allowed = None
+            if prefix_allowed_tokens_fn is not None:
+                so_far = out.cpu()
+                allowed = allowed_bits([prefix_allowed_tokens_fn(b, so_far[b]) for b in range(B)], logits.shape[1], dev)
+            logits = ops.process_logits(logits, generated=out if out.shape[1] else None, repetition_penalty=float(repetition_penalty or 1.0),
+                                        presence_penalty=float(presence_penalty), frequency_penalty=float(frequency_penalty), bias=bias, allowed=allowed)
+            penalty = None                                  # (done)
         if fused:
-            nxt = ops.sample_logits(logits, out if out.shape[1] else None, repetition_penalty, temperature, top_k, top_p,
+            nxt = ops.sample_logits(logits, out if out.shape[1] else None, penalty, temperature, top_k, top_p,
                                     seed, it)
         else:
             lg = _process_logits(logits, out, temperature if do_sample else None, top_k if do_sample else None,
-                                 top_p if do_sample else None, repetition_penalty)
+                                 top_p if do_sample else None, penalty)
             if do_sample:
                 nxt = torch.multinomial(lg.softmax(-1), 1, generator=generator).squeeze(1)
             else:

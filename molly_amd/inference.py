@@ -47,6 +47,10 @@ def parse_args(argv=None):
     ap.add_argument("--use_liger", default=False)
     ap.add_argument("--no-load-pretrained", action="store_true", help="random-init sub-models (offline smoke runs)")
     ap.add_argument("--max-new-tokens", type=int, default=3072, help="reference hard-codes 3072 (src/model/omics_one.py:223)")
+    ap.add_argument("--kv-cache", default="dense", choices=["dense", "paged", "paged_e4m3"], help="paged: no padding in the cache; _e4m3: half the bytes")
+    ap.add_argument("--prefill-chunk", type=int, default=None, help="most prompt tokens of a sequence taken at a time (paged caches)")
+    ap.add_argument("--presence-penalty", type=float, default=0.0)
+    ap.add_argument("--frequency-penalty", type=float, default=0.0)
     ap.add_argument("--greedy", action="store_true", help="do_sample=False (the reference always samples)")
     return ap.parse_args(argv)
 
@@ -126,7 +130,8 @@ class MultiModalInfer:
                         input_ids=batch["input_ids"], attention_mask=batch["attention_mask"], omic_ids=batch["omic_ids"],
                         omic_info_list=batch["omic_info_list"], do_sample=not a.greedy, max_length=a.max_length,
                         temperature=a.temperature, top_p=a.top_p, top_k=a.top_k, repetition_penalty=a.repetition_penalty,
-                        max_new_tokens=a.max_new_tokens, generator=gen)
+                        max_new_tokens=a.max_new_tokens, generator=gen, molly_kv_cache=a.kv_cache, molly_prefill_chunk=a.prefill_chunk,
+                        molly_presence_penalty=a.presence_penalty, molly_frequency_penalty=a.frequency_penalty)
                 decoded = self.text_tokenizer.batch_decode(outputs.cpu(), skip_special_tokens=True)
                 for i, value in enumerate(decoded):
                     json.dump({"decoded_output": value, "input": batch["input"][i], "gt_output": batch["raw_output"][i],

@@ -658,7 +658,9 @@ class OmicsOne(_MetaSafe):
         `self.model.generate` (:220-232) forwards do_sample, temperature, top_p, top_k, no_repeat_ngram_size, the pad / eos ids and
         **generate_kwargs only, so `num_beams=4` there still samples (or decodes greedily).  The same happens here (one warning).
         Beam search / beam sampling (molly_amd/beam.py, pinned to HuggingFace's `_beam_search`) is an EXTENSION of this build,
-        opt-in through `generate_kwargs["molly_num_beams"]`."""
+        opt-in through `generate_kwargs["molly_num_beams"]`.  So are `molly_kv_cache` ('dense' | 'paged' | 'paged_e4m3'), `molly_prefill_chunk`,
+        `molly_presence_penalty`, `molly_frequency_penalty` and `molly_logit_bias` (molly_amd/generate.py); HuggingFace's
+        `prefix_allowed_tokens_fn` is honoured."""
         if num_beams not in (None, 1) and not getattr(OmicsOne, "_warned_num_beams", False):
             import warnings
             warnings.warn("OmicsOne.generate: `num_beams` is accepted and ignored, as in the reference (src/model/omics_one.py:220-232 "
@@ -681,15 +683,19 @@ class OmicsOne(_MetaSafe):
         kw = dict(max_new_tokens=generate_kwargs.pop("max_new_tokens", 3072), repetition_penalty=generate_kwargs.pop("repetition_penalty", None),
                   generator=generate_kwargs.pop("generator", None), num_beams=int(generate_kwargs.pop("molly_num_beams", 1) or 1),
                   length_penalty=generate_kwargs.pop("length_penalty", 1.0), early_stopping=generate_kwargs.pop("early_stopping", False),
-                  min_new_tokens=int(generate_kwargs.pop("min_new_tokens", 0) or 0))
+                  min_new_tokens=int(generate_kwargs.pop("min_new_tokens", 0) or 0),
+                  kv_cache=generate_kwargs.pop("molly_kv_cache", "dense"), prefill_chunk=generate_kwargs.pop("molly_prefill_chunk", None),
+                  presence_penalty=generate_kwargs.pop("molly_presence_penalty", 0.0), frequency_penalty=generate_kwargs.pop("molly_frequency_penalty", 0.0),
+                  logit_bias=generate_kwargs.pop("molly_logit_bias", None),
+                  prefix_allowed_tokens_fn=generate_kwargs.pop("prefix_allowed_tokens_fn", None))
         for k in ("pad_token_id", "eos_token_id"):                 # (the reference passes these itself: a second copy in **kwargs is a TypeError there too)
             if k in generate_kwargs:
                 raise TypeError(f"OmicsOne.generate() got multiple values for keyword argument '{k}' (the reference passes the model config's)")
         if generate_kwargs:
             raise NotImplementedError(
                 "OmicsOne.generate: generate_kwargs not honoured by this build: " + ", ".join(sorted(generate_kwargs)) +
-                " (honoured: max_new_tokens, min_new_tokens, repetition_penalty, use_cache, generator, length_penalty / early_stopping with "
-                "molly_num_beams); the reference forwards them to HuggingFace's generate (src/model/omics_one.py:220-232)")
+                " (honoured: max_new_tokens, min_new_tokens, repetition_penalty, use_cache, generator, prefix_allowed_tokens_fn, length_penalty / "
+                "early_stopping with molly_num_beams, molly_*); the reference forwards them to HuggingFace's generate (src/model/omics_one.py:220-232)")
         return _gen(self, input_ids, attention_mask, omic_ids, omic_info_list, do_sample=do_sample, temperature=temperature,
                     top_p=top_p, top_k=top_k, pad_token_id=cfg.pad_token_id, eos_token_id=cfg.eos_token_id,
                     no_repeat_ngram_size=no_repeat_ngram_size, **kw)

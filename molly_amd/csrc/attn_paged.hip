@@ -5,12 +5,12 @@
 //
 // The query heads of a kv head are packed into the rows of one tile (row = token * G + head of the group), so K and V are read once for all of
 // them whatever G is; the arithmetic is that of attention.hip: S^T = K Q^T and O^T = V^T P^T by 32x32x16 MFMA, online softmax in the exp2
-// domain in fp32, P rounded to bf16 (2^-8 of a term) for the second product.  Two kernels:
+// domain in fp32, P in bf16 for the second product (one bf16 in the tiles, the sum of two in the rows: attend32).  Two kernels:
 //   attn_paged_rows_kernel : up to 32 rows a tile (decode, short chunks).  The 4 | 8 waves of a block take turns at steps of 32 keys, each with
 //                            K / V images of its own in LDS: no workgroup barrier in the loop, the waves meet at the end.  Bound by HBM.
 //   attn_paged_tile_kernel : 128 rows a tile (prompt chunks, mixed batches).  The waves own 32 rows each and share K / V tiles of 64
 //                            keys, double-buffered.  Bound by the matrix pipes where the chunk is long.
-// Either cuts the key axis over blocks where there are too few tiles to fill the chip; attn_paged_merge_kernel joins the parts.
+// Either cuts the key axis over blocks where there are too few tiles to fill the chip; attn_paged_join_kernel joins the parts.
 // A bf16 step's rows go straight to LDS by DMA (16 keys lie within one page, so one page id serves a wave's piece); e4m3 codes pass through registers,
 // are turned into bf16 there (exact) and stored into the same image: one set of fragment reads serves both.
 #include "attn_frag.h"
@@ -240,8 +240,19 @@ __device__ __forceinline__ bool clear_odd(bf16x8 (&vf)[2][ND]) {
     return true;
 }
 
+// the upper halves of floats: bf16, rounded towards 0
+__device__ __forceinline__ float cut_bf(float x) { return __builtin_bit_cast(float, __builtin_bit_cast(unsigned, x) & 0xffff0000u); }
+__device__ __forceinline__ unsigned cut_bf2(float lo, float hi) {
+    return __builtin_amdgcn_perm(__builtin_bit_cast(unsigned, hi), __builtin_bit_cast(unsigned, lo), 0x07060302);
+}
+
 // one step of 32 keys: rows `sub` * 32 .. of the images, keys kbase ..
-template <int HD>
+// FINE: P goes through the second product as two bf16, cut off and rest, which leaves 2^-16 of a term where one bf16 leaves 2^-8: the output has
+// no error but its own rounding then (relative to 64 bits 0.0017 instead of 0.0023).  The rest is taken from P (1 + 2^-20): positive wherever P is, so that
+// an infinite V makes it infinite and not 0 * inf.  Single steps wait for memory and pay little for it:
+// 32 x 4,000 keys e4m3 49.6 -> 50.0 us, bf16 93.2 -> 94.7, 1 x 700 bf16 11.0 -> 11.5, 64 x 2,000 at head dim 64 e4m3 25.5 -> 26.7.  The tiles
+// are bound by the matrix pipes, where it would be half as much work again.
+template <int HD, bool FINE>
 __device__ __forceinline__ void attend32(Rows<HD>& st, const bf16_t* sK, const bf16_t* sV, int sub, int kbase, float scale_log2, int lane) {
     constexpr int NS = HD / 16, ND = HD / 32;
     const int r = lane & 31, h = lane >> 5;
@@ -289,11 +300,33 @@ __device__ __forceinline__ void attend32(Rows<HD>& st, const bf16_t* sK, const b
 #pragma unroll
     for (int g = 0; g < 4; ++g) rs[g] = (sc[4 * g] + sc[4 * g + 1]) + (sc[4 * g + 2] + sc[4 * g + 3]);
     st.l += (rs[0] + rs[1]) + (rs[2] + rs[3]);
-    const bf16x8 pf[2] = {acc_to_frag(sc, 0), acc_to_frag(sc, 8)};
+    bf16x8 pf[2];
+#pragma unroll
+    for (int sp = 0; sp < 2; ++sp) {
+        if constexpr (FINE) {
+            u32x4 w;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) w[j] = cut_bf2(sc[8 * sp + 2 * j], sc[8 * sp + 2 * j + 1]);
+            pf[sp] = __builtin_bit_cast(bf16x8, w);
+        } else {
+            pf[sp] = acc_to_frag(sc, 8 * sp);
+        }
+    }
 #pragma unroll
     for (int d = 0; d < ND; ++d) {
         st.o[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vf[0][d], pf[0], st.o[d], 0, 0, 0);
         st.o[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vf[1][d], pf[1], st.o[d], 0, 0, 0);
+    }
+    if constexpr (FINE) {
+#pragma unroll
+        for (int e = 0; e < 16; ++e) sc[e] = __builtin_fmaf(sc[e], 1.f + 0x1p-20f, -cut_bf(sc[e]));
+#pragma unroll
+        for (int sp = 0; sp < 2; ++sp) pf[sp] = acc_to_frag(sc, 8 * sp);
+#pragma unroll
+        for (int d = 0; d < ND; ++d) {
+            st.o[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vf[0][d], pf[0], st.o[d], 0, 0, 0);
+            st.o[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vf[1][d], pf[1], st.o[d], 0, 0, 0);
+        }
     }
 }
 
@@ -391,7 +424,7 @@ __global__ __launch_bounds__(64 * rows_waves(HD, FP8), rows_waves(HD, FP8) / 4) 
 #pragma unroll
                 for (int g = 0; g < 2; ++g) codes_store<HD, 16>(c[g], img, img + IMG, 16 * g, lane);
                 if (key + STRIDE < k1) load_step(key + STRIDE);
-                attend32<HD>(st, img, img + IMG, 0, key, p.scale_log2, lane);
+                attend32<HD, true>(st, img, img + IMG, 0, key, p.scale_log2, lane);
             }
         } else {
 #pragma unroll
@@ -408,7 +441,7 @@ __global__ __launch_bounds__(64 * rows_waves(HD, FP8), rows_waves(HD, FP8) / 4) 
                 } else {
                     dma_wait();
                 }
-                attend32<HD>(st, img + buf * 2 * IMG, img + buf * 2 * IMG + IMG, 0, key, p.scale_log2, lane);
+                attend32<HD, true>(st, img + buf * 2 * IMG, img + buf * 2 * IMG + IMG, 0, key, p.scale_log2, lane);
                 buf ^= 1;
             }
         }
@@ -472,19 +505,22 @@ template <int TROWS> __device__ __forceinline__ int find_tile(const AttnPagedArg
             n = ((e - s) * p.G + TROWS - 1) / TROWS;
             len = p.kv_len[b];
         }
-        int before = 0, total = 0;                   // tiles of the longer sequences; of all
+        int total = n;
+#pragma unroll
+        for (int o = 32; o > 0; o >>= 1) total += __shfl_xor(total, o, 64);
+        total = __builtin_amdgcn_readfirstlane(total);
+        if (f >= total) {                            // not among these 64 sequences
+            f -= total;
+            continue;
+        }
+        int before = 0;                              // tiles of the longer sequences
         for (int j = 0; j < in; ++j) {
             const int nj = __builtin_amdgcn_readlane(n, j), lj = __builtin_amdgcn_readlane(len, j);
             before += lj > len || (lj == len && j < lane) ? nj : 0;
-            total += nj;
         }
-        const unsigned long long hit = __ballot(f >= before && f < before + n);
-        if (hit) {
-            const int who = __ffsll((long long)hit) - 1;
-            *ti = __builtin_amdgcn_readlane(n, who) - 1 - (f - __builtin_amdgcn_readlane(before, who));
-            return b0 + who;
-        }
-        f -= total;
+        const int who = __ffsll((long long)__ballot(f >= before && f < before + n)) - 1;
+        *ti = __builtin_amdgcn_readlane(n, who) - 1 - (f - __builtin_amdgcn_readlane(before, who));
+        return b0 + who;
     }
     return -1;
 }
@@ -587,11 +623,11 @@ __global__ __launch_bounds__(256, 2) void attn_paged_tile_kernel(AttnPagedArgs p
         const int k = k0 + 64 * i;
         if (active) {
             if constexpr (KS == 2) {
-                if (k + 32 * kg <= st.qmax) attend32<HD>(st, sK + 32 * HD * kg, sK + TILE + 32 * HD * kg, 0, k + 32 * kg, p.scale_log2, lane);
+                if (k + 32 * kg <= st.qmax) attend32<HD, false>(st, sK + 32 * HD * kg, sK + TILE + 32 * HD * kg, 0, k + 32 * kg, p.scale_log2, lane);
             } else {
 #pragma unroll
                 for (int sub = 0; sub < 2; ++sub)
-                    if (k + 32 * sub <= st.qmax) attend32<HD>(st, sK, sK + TILE, sub, k + 32 * sub, p.scale_log2, lane);
+                    if (k + 32 * sub <= st.qmax) attend32<HD, false>(st, sK, sK + TILE, sub, k + 32 * sub, p.scale_log2, lane);
             }
         }
         if (i + 1 < tiles) land(i + 1);

@@ -2,7 +2,7 @@
 
 Tolerances.  A value stored as bf16 is off by at most half a step, 2^-8 of it; e4m3 by 2^-4 of it, or by half a subnormal step, 2^-10 of the
 head's scale.  In front of that rounding everything is float32 (2^-24 an operation, a few operations: 2^-20 of the magnitudes summed).
-Attention rounds the probabilities to bf16 in front of the product with V (2^-8 of every term), its scores are float32 sums of dim products
+Attention rounds the probabilities to bf16 in front of the product with V (at most 2^-8 of every term: one bf16 in the tiles, two in the rows), its scores are float32 sums of dim products
 (2^-24 * dim of |q| |k| * scale, below 2^-12 in the exponent for the values used here, so 2^-11 of a probability) and the result is rounded
 once: (2^-8 + 2^-10) * sum p |v| + 2^-8 * |out|."""
 import math
@@ -319,6 +319,22 @@ def test_attn_paged_nothing_leaks_from_later_tokens(what, new, keys, nh, nkv):
     check(out, q, kp, vp, ks, vs, table, cu, keys, nh)
     if what == "inf":
         assert (out.view(-1, nh, 128)[first:new[0], :, ::3] == math.inf).all()
+
+
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("new,keys,nh,nkv", [([1], [700], 16, 8), ([1, 1], [2050, 40], 8, 2), ([5], [900], 2, 2), ([150], [400], 8, 2)])
+def test_attn_paged_infinite_values_that_every_row_sees(new, keys, nh, nkv, hd):
+    """p * inf is inf with V's sign (two of opposite signs: NaN), as by the formula; the other columns are as they were."""
+    q, kp, vp, ks, vs, table, cu, keys, cu_t, len_t = case(new, keys, nh, nkv, hd, 16, False, seed=8)
+    a = dict(max_q=max(new), max_kv=max(keys))
+    good = ops().attn_paged(q, kp, vp, table, cu_t, len_t, nh, **a).view(-1, nh, hd)
+    for j, col, x in ((5, 0, math.inf), (130, 33, -math.inf), (7, 50, math.inf), (140, 50, -math.inf)):
+        vp[table[0, j // 16].long(), :, j % 16, col] = x
+    out = ops().attn_paged(q, kp, vp, table, cu_t, len_t, nh, **a).view(-1, nh, hd)
+    own = out[:new[0]]
+    assert (own[..., 0] == math.inf).all() and (own[..., 33] == -math.inf).all() and torch.isnan(own[..., 50]).all()
+    rest = [c for c in range(hd) if c not in (0, 33, 50)]
+    assert torch.equal(own[..., rest], good[:new[0]][..., rest]) and torch.equal(out[new[0]:], good[new[0]:])
 
 
 def test_attn_paged_strides_scale_and_shared_pages():

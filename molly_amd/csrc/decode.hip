@@ -5,13 +5,13 @@
 // HBM-bound: every step streams the whole K and V cache of each sample once (2 * kv_len * n_kv_heads * hd * 2 B).
 //  * one block = (sample, KV head, key range): the G = n_heads / n_kv_heads query heads that share the KV head are
 //    processed together, so K/V rows are read ONCE (GQA), 16 B per lane, whole rows coalesced (hd*2 B contiguous);
-//  * split-KV ("flash-decoding"): the key range of a sample is cut into `splits` chunks so B * n_kv_heads * splits blocks
+//  * split-KV: the key range of a sample is cut into `splits` chunks so B * n_kv_heads * splits blocks
 //    fill the chip; each writes an un-normalised partial (m, l, acc) and a small second kernel merges them;
 //  * 8 independent 16-B loads in flight per lane (4 keys x {K, V}) and online softmax with one rescale per 4 keys;
 //  * the arithmetic per key and query head is what bounds a group of 4 heads (Qwen3-8B: 3.45 TB/s against 5.0 for the groups of
 //    2 of Qwen3-1.7B with the first form of this kernel), so it is cut to the bone: q . k as four v_dot2_f32_bf16 on the raw
 //    bf16 pairs (no conversions, scale applied to the sum), the sum over the 8 / 16 lanes of a key row by DPP adds (quad_perm,
-//    row_half_mirror, row_mirror: one VALU instruction each, no LDS permute), p . v as packed fp32 FMAs on V converted once per key.
+//    row_half_mirror, row_mirror: one VALU instruction each, no LDS permute), p . v as fp32 FMAs on V converted once per key.
 #include "common.h"
 #include "molly_hip.h"
 

@@ -3,9 +3,9 @@
 vOFF, s[B:B+1]`).  hipcc pads hazards only between its OWN instructions, so one hazard is ours to rule out: a VALU write of an
 SGPR (v_readfirstlane_b32 / v_readlane_b32 / v_cmp writing an SGPR pair) needs 5 wait states before a VMEM instruction reads
 that SGPR as its base (guide §5.7 item 2).  An `s_nop 4` in front of every DMA costs 2-6 % of GEMM throughput (measured, same
-box), so instead this script PROVES the hazard absent in the generated code: it compiles the sources to assembly and checks
+box), so instead this script PROVES the hazard absent in the generated code: it compiles the sources to assembly, with the build's flags, and checks
 that no SGPR used as the base of an asm-issued global_load_lds was written by a VALU instruction within the 5 preceding
-instructions.  Run after every edit of gemm.hip / attention.hip (tests/test_abi.py runs it on the built sources).
+instructions.  Run after every edit of gemm.hip / attention.hip / attn_paged.hip / lora.hip (tests/test_abi.py runs it on the built sources).
 
     python tools/check_asm_dma_hazards.py            # exit code 0 = clean"""
 import os
@@ -16,14 +16,14 @@ import tempfile
 
 ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
 CSRC = os.path.join(ROOT, "molly_amd", "csrc")
-HIPCC = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
+sys.path.insert(0, ROOT)
+from molly_amd import build as B  # noqa: E402
 
 
 def assembly(src):
     with tempfile.TemporaryDirectory() as d:
         out = os.path.join(d, "k.s")
-        cmd = [HIPCC, "--offload-arch=gfx950", "-O3", "-std=c++17", "-I" + CSRC, "-I" + os.path.join(ROOT, "include"),
-               "-ffp-contract=fast", "-Wno-inline-asm", "-x", "hip", "-S", "--cuda-device-only", "-o", out, os.path.join(CSRC, src)]
+        cmd = [B.HIPCC] + B.FLAGS + B.EXTRA.get(src, []) + ["-x", "hip", "-S", "--cuda-device-only", "-o", out, os.path.join(CSRC, src)]
         r = subprocess.run(cmd, capture_output=True, text=True)
         if r.returncode != 0:
             raise RuntimeError(r.stderr[-2000:])

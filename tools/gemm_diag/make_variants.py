@@ -203,7 +203,7 @@ for n in names:
     out = os.path.join(ROOT, f"tools/gemm_diag/libgemm_{n}.so")
     inc = ["-I" + os.path.join(ROOT, "molly_amd/csrc"), "-I" + os.path.join(ROOT, "include")]
     obj = p[:-4] + ".o"
-    r = subprocess.run(["/opt/rocm/bin/hipcc", "--offload-arch=gfx950", "-O3", "-fPIC", "-std=c++17", "-ffp-contract=fast"] + inc +
+    r = subprocess.run(["/opt/rocm/bin/hipcc", "--offload-arch=gfx950", "-O3", "-fPIC", "-std=c++17", "-ffp-contract=fast", "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"] + inc +
                        ["-x", "hip", "-c", p, "-o", obj], capture_output=True, text=True)
     if r.returncode == 0:
         r = subprocess.run(["/opt/rocm/bin/hipcc", "--offload-arch=gfx950", "-shared", "-fPIC", "-o", out, obj,

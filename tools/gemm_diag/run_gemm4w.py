@@ -13,7 +13,7 @@ SO = os.path.join(HERE, "libgemm4w" + ("_" + VAR.replace(",", "_") if VAR else "
 
 
 def build():
-    cmd = ["/opt/rocm/bin/hipcc", "--offload-arch=gfx950", "-O3", "-fPIC", "-std=c++17", "-ffp-contract=fast", "-shared",
+    cmd = ["/opt/rocm/bin/hipcc", "--offload-arch=gfx950", "-O3", "-fPIC", "-std=c++17", "-ffp-contract=fast", "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops", "-shared",
            *["-DABL_" + v for v in VAR.split(",") if v], "-I" + os.path.join(ROOT, "molly_amd/csrc"), "-I" + os.path.join(ROOT, "include"), "-x", "hip",
            os.path.join(HERE, "gemm4w.hip"), "-o", SO]
     r = subprocess.run(cmd, capture_output=True, text=True)

@@ -19,7 +19,7 @@ def build(var):
     so = so_for(var)
     if os.path.exists(so) and os.path.getmtime(so) >= os.path.getmtime(os.path.join(HERE, SRC)):
         return so
-    cmd = ["/opt/rocm/bin/hipcc", "--offload-arch=gfx950", "-O3", "-fPIC", "-std=c++17", "-ffp-contract=fast", "-shared",
+    cmd = ["/opt/rocm/bin/hipcc", "--offload-arch=gfx950", "-O3", "-fPIC", "-std=c++17", "-ffp-contract=fast", "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops", "-shared",
            *["-DABL_" + v for v in var.split(",") if v], "-I" + os.path.join(ROOT, "molly_amd/csrc"), "-I" + os.path.join(ROOT, "include"), "-x", "hip",
            os.path.join(HERE, SRC), "-o", so]
     r = subprocess.run(cmd, capture_output=True, text=True)

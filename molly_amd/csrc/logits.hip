@@ -11,7 +11,9 @@
 
 namespace {
 
-constexpr int LONG_HISTORY = 4096;
+// every workgroup reads the row's whole history: from this many tokens on, four times fewer, larger workgroups do (V = 151,936, one row | 32 rows, 256 -> 1,024
+// threads: 1,024 tokens 4.2 -> 4.4 | 8.2 -> 8.6 us, 2,048 5.0 -> 4.9 | 9.4 -> 9.3, 8,192 9.0 -> 6.3 | 18.3 -> 13.2, 32,768 22.6 -> 10.1 | 49.5 -> 22.7)
+constexpr int LONG_HISTORY = 2048;
 
 struct LogitArgs {
     const void* x; float* out;
@@ -135,7 +137,7 @@ extern "C" int molly_process_logits(void* stream, const void* logits, int logits
                                     const float* presence_rows, const float* frequency_rows, const float* bias, long ld_bias,
                                     const void* allowed, long ld_allowed) {
     MOLLY_ENTER();
-    MOLLY_CHECK(rows >= 0 && rows <= 65535 && V > 0 && ld_logits >= V && ld_out >= V, "process_logits: rows=%d (at most 65535) V=%d ld=%ld/%ld", rows, V,
+    MOLLY_CHECK(rows >= 0 && rows <= 65535 && V > 0 && V <= 0x40000000 && ld_logits >= V && ld_out >= V, "process_logits: rows=%d (at most 65535) V=%d (at most 2^30) ld=%ld/%ld", rows, V,
                 ld_logits, ld_out);
     MOLLY_CHECK(n_history >= 0 && (n_history == 0 || (generated && ld_generated >= n_history)), "process_logits: %d generated tokens, ld=%ld", n_history,
                 ld_generated);
@@ -149,10 +151,9 @@ extern "C" int molly_process_logits(void* stream, const void* logits, int logits
     p.rep_v = repetition_rows; p.pres_v = presence_rows; p.freq_v = frequency_rows; p.bias = bias; p.mask = (const unsigned*)allowed;
     p.rep = repetition; p.pres = presence; p.freq = frequency; p.V = V; p.n_hist = n_history;
     p.ldx = ld_logits; p.ldo = ld_out; p.ldg = ld_generated; p.ldb = ld_bias; p.ldm = ld_allowed;
-    // every workgroup reads the row's whole history: long ones are read by fewer, larger workgroups
     hipStream_t st = (hipStream_t)stream;
     if (n_history == 0) launch<256, false>(st, p, rows, logits_bf16 != 0);
-    else if (n_history <= LONG_HISTORY) launch<256, true>(st, p, rows, logits_bf16 != 0);
+    else if (n_history < LONG_HISTORY) launch<256, true>(st, p, rows, logits_bf16 != 0);
     else launch<1024, true>(st, p, rows, logits_bf16 != 0);
     MOLLY_LAUNCH_CHECK();
     return 0;

@@ -130,6 +130,7 @@ class GenerationSession:
         self.cos, self.sin = rope_tables(most, e.hd, e.cfg.rope_theta, dev, e.rope_table_dtype)
         need = [-(-(n + self.max_new) // self.page_size) for n in n_valid]
         self.paged = PagedKVCache(L, sum(need), e.nkv, e.hd, self.page_size, "bf16" if self.kv_cache == "paged" else "e4m3", dev)
+        self.need, self.own = need, list(need)                                # pages that the sequence in a row needs; that the row owns
         pages = [self.paged.allocate(n + self.max_new) for n in n_valid]
         self.table = self.paged.block_table(pages)
         # places of every sequence's tokens in the pools, [B, pages * page size] (behind the last page: none)
@@ -317,6 +318,11 @@ class GenerationSession:
         n = self.cur_len
         if self.paged is not None:
             # what the rows hold of their pages moves; a row's own page list stays (the captured graph's tables)
+            need = [self.need[r] for r in rows.tolist()]
+            for i, (n, own) in enumerate(zip(need, self.own)):
+                if n > own:
+                    raise ValueError(f"reorder: row {i} owns {own} pages, the sequence that is to move there needs {n}")
+            self.need = need
             used = -(-int(self.hi.max()) // self.page_size)
             src, dst = self.table[rows, :used], self.table[:, :used]
             moved = (src != dst) & (src >= 0) & (dst >= 0)
@@ -434,7 +440,7 @@ def allowed_bits(allowed, vocab: int, device) -> torch.Tensor:
     rows, words = len(allowed), (vocab + 31) // 32
     on = torch.zeros(rows, words * 32, dtype=torch.bool)
     for r, ids in enumerate(allowed):
-        ids = torch.as_tensor(ids, dtype=torch.int64).reshape(-1)
+        ids = torch.as_tensor(ids, dtype=torch.int64).reshape(-1).cpu()
         if ids.numel() == 0:
             raise ValueError(f"generate: no token is allowed in row {r}")
         if int(ids.min()) < 0 or int(ids.max()) >= vocab:

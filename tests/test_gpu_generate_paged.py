@@ -75,6 +75,26 @@ def test_paged_reorder(tiny_meta, kv_cache):
         assert (lb[0] - la[2]).abs().max() <= tol and (lb[1] - la[0]).abs().max() <= tol
 
 
+def test_paged_reorder_into_a_row_with_fewer_pages_is_refused(tiny_meta):
+    """A row keeps the pages its prompt was given; a longer sequence does not fit into fewer of them."""
+    m = build_tiny(tiny_meta)
+    batch = _left_padded_batch(tiny_meta)
+    n = batch[1].sum(1).tolist()
+    assert n[0] != n[1]
+    small, large = (0, 1) if n[0] < n[1] else (1, 0)
+    a, la = _session(m, batch, kv_cache="paged", page_size=16)
+    assert len(set(a.own)) == 2
+    first = la.argmax(-1)
+    state = a.state.clone()
+    with pytest.raises(ValueError):
+        a.reorder(torch.tensor([large, large]))
+    assert torch.equal(a.state, state)
+    a.reorder(torch.tensor([small, small]))                       # the shorter one fits into both, and both say the same from here on
+    for tok in (int(first[small]), 9):
+        l = a.step(torch.tensor([tok, tok]))
+        assert torch.equal(l[0], l[1]) and torch.isfinite(l).all()
+
+
 def test_live_adapters_with_a_paged_cache(tiny_meta):
     """Un-merged adapters (plain projections + rank-r additions) go the same way: paged and dense caches agree to bf16 (the bound of the test above)."""
     from molly_amd.lora import LoraConfig
@@ -117,6 +137,10 @@ def test_generate_with_paged_cache_and_processors(tiny_meta):
     s = m.generate(ids, mask, omic, info, do_sample=True, top_k=20, temperature=0.8, top_p=0.95, repetition_penalty=1.1, max_new_tokens=4, generator=g,
                    molly_kv_cache="paged_e4m3", molly_presence_penalty=0.3, prefix_allowed_tokens_fn=lambda r, x: range(100, 200))
     assert s.shape == (2, 4) and bool(((s >= 100) & (s < 200)).all())
+    # fewer allowed tokens than top_k, as a tensor of any device
+    few = torch.tensor([700, 3], device="cuda")
+    s = m.generate(ids, mask, omic, info, do_sample=True, top_k=20, temperature=0.8, top_p=1.0, max_new_tokens=8, prefix_allowed_tokens_fn=lambda r, x: few)
+    assert s.shape == (2, 8) and bool(((s == 700) | (s == 3)).all())
 
 
 def test_refusals(tiny_meta):

@@ -218,6 +218,14 @@ def test_attn_paged(new, keys, nh, nkv, hd, page, fp8):
 
 
 @pytest.mark.parametrize("fp8", [False, True])
+@pytest.mark.parametrize("new,keys,nh,nkv,hd", [([1, 1], [900, 40], 48, 1, 128), ([1], [6000], 71, 1, 64), ([2, 1], [70, 3000], 64, 2, 128)])
+def test_attn_paged_more_query_heads_than_a_tile_of_single_steps_has_rows(new, keys, nh, nkv, hd, fp8):
+    q, kp, vp, ks, vs, table, cu, keys, cu_t, len_t = case(new, keys, nh, nkv, hd, 32, fp8, seed=12)
+    for mq, mk in ((max(new), max(keys)), (0, 0)):
+        check(ops().attn_paged(q, kp, vp, table, cu_t, len_t, nh, kscale=ks, vscale=vs, max_q=mq, max_kv=mk), q, kp, vp, ks, vs, table, cu, keys, nh)
+
+
+@pytest.mark.parametrize("fp8", [False, True])
 @pytest.mark.parametrize("kind", ["decode", "short", "mixed", "long"])
 def test_attn_paged_many_sequences(kind, fp8):
     """More sequences than a wave has lanes, some without new tokens, lengths from none to thousands; few long ones over few heads."""

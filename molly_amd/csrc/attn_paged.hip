@@ -32,6 +32,7 @@ struct AttnPagedArgs {
     int n_tok, B, n_pages, page_shift, max_pages, ld_table, nh, nkv, G, ldq, ldo;
     int tps;                                         // rows kernel: tiles per sequence; tile kernel: bound of the tiles of all of them
     int parts;                                       // most parts of a tile's key axis
+    int class_bits;                                  // find_tile: 2^class_bits classes of 64 keys
     float scale_log2;                                // softmax scale * log2(e), > 0
 };
 
@@ -494,35 +495,63 @@ __global__ __launch_bounds__(64 * rows_waves(HD, FP8), rows_waves(HD, FP8) / 4) 
 }
 
 // ---- long chunks: 128 or 64 rows a block -----------------------------------------------------------------------------------------------------------
-// tile f of the sequences' tiles: the longest sequences first (64 sequences at a time), within one the longest causal range first; -1: there are fewer.
-// Blocks start in order, so a compute unit's second block is a shorter one than its first, and the last to start are the shortest.
-template <int TROWS> __device__ __forceinline__ int find_tile(const AttnPagedArgs& p, int f, int lane, int* ti) {
-    for (int b0 = 0; b0 < p.B; b0 += 64) {
-        const int b = b0 + lane, in = min(p.B - b0, 64);
-        int n = 0, len = -1;
-        if (lane < in) {
-            const int s = min(max(p.cu_q[b], 0), p.n_tok), e = min(max(p.cu_q[b + 1], s), p.n_tok);
-            n = ((e - s) * p.G + TROWS - 1) / TROWS;
-            len = p.kv_len[b];
+// Sum over the lanes up to and including each (lane 63: all).
+__device__ __forceinline__ int wave_scan(int x) {
+    x += __builtin_amdgcn_update_dpp(0, x, 0x111, 0xf, 0xf, false);      // row_shr 1, 2, 4, 8: within rows of 16
+    x += __builtin_amdgcn_update_dpp(0, x, 0x112, 0xf, 0xf, false);
+    x += __builtin_amdgcn_update_dpp(0, x, 0x114, 0xf, 0xf, false);
+    x += __builtin_amdgcn_update_dpp(0, x, 0x118, 0xf, 0xf, false);
+    x += __builtin_amdgcn_update_dpp(0, x, 0x142, 0xa, 0xf, false);      // row_bcast 15: rows 1 and 3
+    x += __builtin_amdgcn_update_dpp(0, x, 0x143, 0xc, 0xf, false);      // row_bcast 31: rows 2 and 3
+    return x;
+}
+__device__ __forceinline__ int wave_total(int x) { return __builtin_amdgcn_readlane(wave_scan(x), 63); }
+// one sequence a lane: its tiles (0 behind the last sequence) and its keys, as far as they are ranked (at least 0)
+struct Seq { int n, len; };
+template <int TROWS> __device__ __forceinline__ Seq load_seq(const AttnPagedArgs& p, int b) {
+    const int i = min(b, p.B - 1), s0 = p.cu_q[i], e0 = p.cu_q[i + 1], keys = p.kv_len[i];
+    const int s = min(max(s0, 0), p.n_tok), rows = (min(max(e0, s), p.n_tok) - s) * p.G;
+    return {b < p.B ? (rows + TROWS - 1) / TROWS : 0, min(max(keys, 0), (64 << p.class_bits) - 1)};
+}
+// The tile of a rank, 64 sequences after the other (the first 64 in `q`), of these the tile with the most keys first, in classes of 64 keys; within a class by sequence.
+// A sequence's tiles are TROWS / G keys apart.  -1: there are fewer tiles.  (Ranked by their sequences' lengths only: 8 prompts of 314..1,111 tokens at head dim 64 32.5
+// us against 27.0, 64 of 1,111 290 against 269; tiles of single steps ranked by half their keys: 24 sequences, a quarter of them with 301 new tokens, 89 us against 86.)
+template <int TROWS> __device__ __forceinline__ int find_tile(const AttnPagedArgs& p, Seq q, int rank, int lane, int* ti) {
+    const float per_key = (float)p.G / TROWS;
+    for (int b0 = 0;;) {
+        const int total = wave_total(q.n);
+        if (rank < total) {
+            if (p.B == 1) {
+                *ti = total - 1 - rank;
+                return 0;
+            }
+            auto least = [&](int c) {                // this sequence's tiles of class c or above
+                const int over = q.len - 64 * c;
+                return c == 0 ? q.n : over < 0 ? 0 : min(q.n, (int)fminf((float)over * per_key, 0x1p30f) + 1);
+            };
+            int c = 0;                               // the rank's class: the highest that has more than `rank` tiles in it and above it
+            for (int bit = p.class_bits - 1; bit >= 0; --bit)
+                if (wave_total(least(c | 1 << bit)) > rank) c |= 1 << bit;
+            const int above = least(c + 1), here = least(c) - above;
+            rank -= wave_total(above);
+            const int upto = wave_scan(here), k = above + rank - (upto - here);      // (k-th from the sequence's last tile)
+            const int who = __ffsll((long long)__ballot(rank < upto)) - 1;
+            *ti = __builtin_amdgcn_readlane(q.n - 1 - k, who);
+            return b0 + who;
         }
-        int total = n;
-#pragma unroll
-        for (int o = 32; o > 0; o >>= 1) total += __shfl_xor(total, o, 64);
-        total = __builtin_amdgcn_readfirstlane(total);
-        if (f >= total) {                            // not among these 64 sequences
-            f -= total;
-            continue;
-        }
-        int before = 0;                              // tiles of the longer sequences
-        for (int j = 0; j < in; ++j) {
-            const int nj = __builtin_amdgcn_readlane(n, j), lj = __builtin_amdgcn_readlane(len, j);
-            before += lj > len || (lj == len && j < lane) ? nj : 0;
-        }
-        const int who = __ffsll((long long)__ballot(f >= before && f < before + n)) - 1;
-        *ti = __builtin_amdgcn_readlane(n, who) - 1 - (f - __builtin_amdgcn_readlane(before, who));
-        return b0 + who;
+        rank -= total;
+        b0 += 64;
+        if (b0 >= p.B) return -1;
+        q = load_seq<TROWS>(p, b0 + lane);
     }
-    return -1;
+}
+// The rank of an XCD's block `pos`, of N.  Blocks start in order, the first 32 on a compute unit each, the next 32 on the same ones in the same order, while there is
+// room (SLOTS blocks a unit); later ones where a block has ended.  So of every 64 the second half goes backwards: the longest shares its unit with the shortest; where
+// the second half is not full, the longest are alone.  (2,048 tokens over 16,384 keys 512 -> 509 us, e4m3 548 -> 539; 4 x 512 over 3,000 e4m3 108.7 -> 107.)
+template <int SLOTS> __device__ __forceinline__ int deal(int pos, int N) {
+    const int base = pos & ~63, n = min(N - base, 64), i = pos & 63, k = n - 32;
+    if (base >= 32 * SLOTS || k <= 0) return pos;
+    return base + (i >= 32 ? n - 1 - (i - 32) : i < k ? 64 - n + i : i - k);
 }
 
 // KS 1: the waves own 32 rows each (128 a block).  KS 2: two own 32 rows each (64 a block) for the first half of every tile's keys, two the same rows for the
@@ -538,25 +567,34 @@ __global__ __launch_bounds__(256, 2) void attn_paged_tile_kernel(AttnPagedArgs p
     // The workgroups of one XCD (every eighth) share the keys of as few (kv head, part) units as possible in its L2: whole units to an XCD where they can
     // be dealt evenly, every X-th tile of a unit to each of its X XCDs where there are fewer, else contiguous runs of (unit, tile).
     const int units = p.nkv * p.parts, xcd = blockIdx.x & 7, i8 = blockIdx.x >> 3;
-    int f, unit;
+    int pos, unit, x = 0, X = 1;                     // the unit's XCDs take every X-th tile, this one those of rank x, x + X ..
+    bool whole = true;
     if (units % 8 == 0) {
         unit = xcd * (units / 8) + i8 / p.tps;
-        f = i8 % p.tps;
+        pos = i8 % p.tps;
     } else if (8 % units == 0) {
-        const int X = 8 / units;
+        X = 8 / units;
         unit = xcd / X;
-        f = i8 * X + xcd % X;
+        x = xcd % X;
+        pos = i8;
     } else {
         const int run = (units * p.tps + 7) / 8;
         const int v = xcd * run + i8;
         if (i8 >= run || v >= units * p.tps) return;
         unit = v / p.tps;
-        f = v % p.tps;
+        pos = v % p.tps;
+        whole = false;
     }
-    if (f >= p.tps) return;
+    const Seq seq = load_seq<TROWS>(p, lane);
+    int total = wave_total(seq.n);
+    for (int b0 = 64; b0 < p.B; b0 += 64) total += wave_total(load_seq<TROWS>(p, b0 + lane).n);
+    total = min(total, p.tps);                       // (more only where cu_q does not ascend)
+    const int N = (total - x + X - 1) / X;
+    if (pos >= N) return;
+    const int f = (whole ? deal<HD == 128 || FP8 ? 2 : 4>(pos, N) : pos) * X + x;
     const int s = unit % p.parts, kvh = unit / p.parts;
     int ti = 0;
-    const int b = __builtin_amdgcn_readfirstlane(find_tile<TROWS>(p, f, lane, &ti));
+    const int b = __builtin_amdgcn_readfirstlane(find_tile<TROWS>(p, seq, f, lane, &ti));
     if (b < 0) return;
     ti = __builtin_amdgcn_readfirstlane(ti);
     const Tile t = make_tile<TROWS>(p, b, ti);
@@ -747,7 +785,7 @@ __global__ __launch_bounds__(256) void attn_paged_join_kernel(AttnPagedArgs p) {
     constexpr int STRIDE = ROWS * (HD + 2);
     const int lane = threadIdx.x & 63, tile = blockIdx.x / p.nkv, kvh = blockIdx.x % p.nkv;
     int b = tile / p.tps, ti = tile % p.tps;
-    if constexpr (ROWS != RROWS) b = find_tile<ROWS>(p, tile, lane, &ti);
+    if constexpr (ROWS != RROWS) b = find_tile<ROWS>(p, load_seq<ROWS>(p, lane), tile, lane, &ti);
     if (b < 0) return;
     const Tile t = make_tile<ROWS>(p, b, ti);
     const int parts = parts_of(min(t.n_vis, p.max_pages << p.page_shift), p.parts);
@@ -761,7 +799,7 @@ __global__ __launch_bounds__(256) void attn_paged_join_kernel(AttnPagedArgs p) {
 }
 
 // ---- host: which kernel, and how many parts
-struct Shape { int ks, tps, parts, rows; long tiles, part_floats; };      // ks 0: the rows kernel
+struct Shape { int ks, tps, parts, rows, class_bits; long tiles, part_floats; };      // ks 0: the rows kernel
 Shape pick_shape(int n_tok, int B, int nkv, int G, int HD, bool fp8, long max_keys, int max_q, int max_kv) {
     Shape sh{};
     const long mq = max_q > 0 && max_q < n_tok ? max_q : n_tok;
@@ -770,6 +808,7 @@ Shape pick_shape(int n_tok, int B, int nkv, int G, int HD, bool fp8, long max_ke
     // sequence of 64 over 20,000 52 -> 46 us; but 2,048 tokens over 16,384 keys 518 -> 560 us, 24 mixed sequences 103 -> 111 us
     sh.ks = mq * G <= RROWS ? 0 : ((long)n_tok * G / 128 + B) * nkv < 512 ? 2 : 1;
     const int rows = sh.ks ? 128 / sh.ks : RROWS;
+    for (sh.class_bits = 0; sh.class_bits < 24 && (64L << sh.class_bits) <= keys; ++sh.class_bits) {}
     sh.tps = (int)(sh.ks ? (long)n_tok * G / rows + B : (mq * G + RROWS - 1) / RROWS);
     sh.rows = (int)(mq * G < rows ? mq * G : rows);      // rows of a tile, as far as the caller knows
     sh.tiles = sh.ks ? sh.tps : (long)sh.tps * B;
@@ -850,7 +889,7 @@ extern "C" int molly_attn_paged(void* stream, const void* q, void* out, const vo
     p.nh = n_heads; p.nkv = n_kv_heads; p.G = n_heads / n_kv_heads; p.ldq = ldq; p.ldo = ldo; p.scale_log2 = scale * LOG2E;
     Shape sh = pick_shape(n_tokens, B, n_kv_heads, p.G, head_dim, kscale_or_null != nullptr, (long)max_pages * page_size, max_q, max_kv);
     if (!workspace || workspace_floats < sh.part_floats) sh.parts = 1;
-    p.part = workspace; p.tps = sh.tps; p.parts = sh.parts;
+    p.part = workspace; p.tps = sh.tps; p.parts = sh.parts; p.class_bits = sh.class_bits;
     hipStream_t st = (hipStream_t)stream;
     if (head_dim == 128) {
         if (kscale_or_null) launch<128, true>(st, p, sh);

@@ -834,7 +834,8 @@ def paged_kv_append(k, v, kpool, vpool, slot, kscale=None, vscale=None, q=None, 
                     positions=None, eps=1e-6):
     """Rows of k and v [n, kv heads * dim] into the places slot (int32 [n], page * page_size + offset; -1: the row is padding) of the pools, with
     q/k-norm (gains qw / kw [dim]) and rotary (cos / sin fp32 [n_pos, dim / 2], positions int32 [n]) of k, and of q [n, heads * dim], in the same
-    pass where they are given (molly_paged_kv_append).  Row strides are free.  -> q's rows after both (q_out; q_out may be q), or None."""
+    pass where they are given (molly_paged_kv_append; qw without q is not used).  Row strides are free.
+    -> q's rows after both (q_out; q_out may be q), or None."""
     what = "paged_kv_append"
     dev, (P, nkv, page, hd), (kp, vp, ks, vs) = _pools(kpool, vpool, kscale, vscale, what)
     n = k.shape[0]
@@ -852,8 +853,8 @@ def paged_kv_append(k, v, kpool, vpool, slot, kscale=None, vscale=None, q=None, 
         if q_out is None:
             q_out = torch.empty((n, width), dtype=BF16, device=q.device)
         qo_at, ldqo = _rows(q_out, dev, what, "q_out", n, width)
-    elif q_out is not None or qw is not None:
-        raise ValueError(f"{what}: q_out / qw without q")
+    elif q_out is not None:
+        raise ValueError(f"{what}: q_out without q")
     for w in (qw, kw):
         if w is not None and (w.dtype != BF16 or w.shape != (hd,) or not w.is_contiguous()):
             raise ValueError(f"{what}: gains must be contiguous bfloat16 [{hd}]")
@@ -940,7 +941,8 @@ def process_logits(logits, generated=None, n_generated=None, repetition_penalty=
     With c = occurrences of a token among the row's first n_generated (int32 [rows]; None: all) entries of `generated` (int64 [rows, n]; ids
     outside the vocabulary do not count): c > 0: s = (s < 0 ? s * repetition : s / repetition) - presence - frequency * c; then s += bias
     (fp32 [V] or [rows, V]); then -inf where a token is not allowed (`allowed`: int32 bits [ceil(V / 32)] or [rows, ceil(V / 32)], bit v % 32 of
-    word v // 32).  The penalties: numbers, or fp32 [rows]."""
+    word v // 32).  The penalties: numbers, or fp32 [rows].  float32 logits with nothing to apply (no `generated`, bias, mask nor `out`) come back as
+    they are, the same tensor."""
     what = "process_logits"
     dev, dtype = logits.get_device(), logits.dtype
     if dev < 0:
@@ -949,6 +951,9 @@ def process_logits(logits, generated=None, n_generated=None, repetition_penalty=
         raise ValueError(f"{what}: logits must be float32 or bfloat16 [rows, V] with contiguous rows, got {dtype} {tuple(logits.shape)}")
     rows, V = logits.shape
     if out is None:
+        if generated is None and n_generated is None and bias is None and allowed is None and dtype == torch.float32 and not any(
+                isinstance(x, torch.Tensor) for x in (repetition_penalty, presence_penalty, frequency_penalty)) and repetition_penalty > 0:
+            return logits
         out = torch.empty((rows, V), dtype=torch.float32, device=logits.device)
     elif out.dtype != torch.float32 or out.shape != logits.shape or (out.stride(1) != 1 and V != 1):
         raise ValueError(f"{what}: out must be float32 {tuple(logits.shape)} with contiguous rows")

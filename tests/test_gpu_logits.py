@@ -107,6 +107,15 @@ def test_strides_and_graph():
         same(got, reference(x, ids, None, 1.2, 0.0, 0.3))
 
 
+def test_nothing_to_apply():
+    """float32 logits come back as they are; bf16 ones, or ones with an `out`, are converted / copied."""
+    x = torch.randn(3, 100, device=DEV)
+    out = torch.empty_like(x)
+    assert ops().process_logits(x, repetition_penalty=1.2, presence_penalty=0.5) is x
+    assert ops().process_logits(x, out=out) is out and torch.equal(out, x)
+    assert torch.equal(ops().process_logits(x.bfloat16()), x.bfloat16().float())
+
+
 def test_refusals():
     o = ops()
     x = torch.randn(3, 100, device=DEV)

@@ -112,6 +112,16 @@ def test_append_codes_match_the_format():
     assert torch.equal(kr.double().nan_to_num(7.0), val.bfloat16().double().nan_to_num(7.0)) and torch.equal(torch.isnan(kr), torch.isnan(vr))
 
 
+def test_append_without_queries_takes_their_gain_too():
+    _, k, v, qw, kw, *_ = store_inputs(9, 4, 2, 64, 3)
+    slot = torch.arange(9, device=DEV, dtype=torch.int32)
+    kp, vp, _, _ = empty_pools(1, 2, 16, 64, False)
+    kp2, vp2 = kp.clone(), vp.clone()
+    assert ops().paged_kv_append(k, v, kp, vp, slot, qw=qw, kw=kw) is None
+    ops().paged_kv_append(k, v, kp2, vp2, slot, kw=kw)
+    assert all(torch.equal(a.view(torch.int16), b.view(torch.int16)) for a, b in ((kp, kp2), (vp, vp2)))
+
+
 def test_append_in_place_strided_and_bad_positions():
     n, nq, nkv, hd = 9, 4, 2, 64
     q, k, v, qw, kw, cos, sin, pos = store_inputs(n, nq, nkv, hd, 3)

@@ -851,7 +851,7 @@ def paged_kv_append(k, v, kpool, vpool, slot, kscale=None, vscale=None, q=None, 
             raise ValueError(f"{what}: q must be [{n}, heads * {hd}], got {tuple(q.shape)}")
         q_at, ldq = _rows(q, dev, what, "q", n, width)
         if q_out is None:
-            q_out = torch.empty((n, width), dtype=BF16, device=q.device)
+            q_out = q.new_empty((n, width))
         qo_at, ldqo = _rows(q_out, dev, what, "q_out", n, width)
     elif q_out is not None:
         raise ValueError(f"{what}: q_out without q")
@@ -879,9 +879,9 @@ def paged_kv_read(kpool, vpool, slot, kscale=None, vscale=None, k_out=None, v_ou
     n = slot.shape[0] if slot.dim() == 1 else -1
     slot_at = _ints(slot, dev, what, "slot", (n,))
     if k_out is None:
-        k_out = torch.empty((n, nkv * hd), dtype=BF16, device=kpool.device)
+        k_out = kpool.new_empty((n, nkv * hd), dtype=BF16)
     if v_out is None:
-        v_out = torch.empty((n, nkv * hd), dtype=BF16, device=kpool.device)
+        v_out = kpool.new_empty((n, nkv * hd), dtype=BF16)
     k_at, ldk = _rows(k_out, dev, what, "k_out", n, nkv * hd)
     v_at, ldv = _rows(v_out, dev, what, "v_out", n, nkv * hd)
     _launch("molly_paged_kv_read", dev, kp, vp, ks, vs, slot_at, n, P, page, nkv, hd, k_at, v_at, ldk, ldv)
@@ -911,7 +911,7 @@ def attn_paged(q, kpool, vpool, block_table, cu_q, kv_len, n_heads, scale=None, 
     B, max_pages = block_table.shape
     cu_at, len_at, table_at = _ints(cu_q, dev, what, "cu_q", (B + 1,)), _ints(kv_len, dev, what, "kv_len", (B,)), _on(block_table, dev, what, "block_table")
     if out is None:
-        out = torch.empty((n, n_heads * hd), dtype=BF16, device=q.device)
+        out = q.new_empty((n, n_heads * hd))
     out_at, ldo = _rows(out, dev, what, "out", n, n_heads * hd)
     if workspace is None:
         floats = attn_paged_workspace(n, B, n_heads, nkv, hd, page, max_pages, ks is not None, max_q, max_kv)
@@ -954,7 +954,7 @@ def process_logits(logits, generated=None, n_generated=None, repetition_penalty=
         if generated is None and n_generated is None and bias is None and allowed is None and dtype == torch.float32 and not any(
                 isinstance(x, torch.Tensor) for x in (repetition_penalty, presence_penalty, frequency_penalty)) and repetition_penalty > 0:
             return logits
-        out = torch.empty((rows, V), dtype=torch.float32, device=logits.device)
+        out = logits.new_empty((rows, V), dtype=torch.float32)
     elif out.dtype != torch.float32 or out.shape != logits.shape or (out.stride(1) != 1 and V != 1):
         raise ValueError(f"{what}: out must be float32 {tuple(logits.shape)} with contiguous rows")
     ldx, ldo = (logits.stride(0), out.stride(0)) if rows > 1 else (V, V)

@@ -950,10 +950,10 @@ def process_logits(logits, generated=None, n_generated=None, repetition_penalty=
     if logits.dim() != 2 or dtype not in (torch.float32, BF16) or (logits.stride(1) != 1 and logits.shape[1] != 1):
         raise ValueError(f"{what}: logits must be float32 or bfloat16 [rows, V] with contiguous rows, got {dtype} {tuple(logits.shape)}")
     rows, V = logits.shape
-    if out is None:
-        if generated is None and n_generated is None and bias is None and allowed is None and dtype == torch.float32 and not any(
-                isinstance(x, torch.Tensor) for x in (repetition_penalty, presence_penalty, frequency_penalty)) and repetition_penalty > 0:
-            return logits
+    nothing = out is None and generated is None and bias is None and allowed is None and dtype == torch.float32
+    if nothing:
+        out = logits                                              # (the arguments are checked all the same)
+    elif out is None:
         out = logits.new_empty((rows, V), dtype=torch.float32)
     elif out.dtype != torch.float32 or out.shape != logits.shape or (out.stride(1) != 1 and V != 1):
         raise ValueError(f"{what}: out must be float32 {tuple(logits.shape)} with contiguous rows")
@@ -981,6 +981,8 @@ def process_logits(logits, generated=None, n_generated=None, repetition_penalty=
         else:
             pen.append(x)
             pen_at.append(None)
+    if nothing and pen[0] > 0:
+        return logits
     bias_at, ldb = _vocab_rows(bias, dev, what, "bias", torch.float32, rows, V)
     allowed_at, ldm = _vocab_rows(allowed, dev, what, "allowed", torch.int32, rows, (V + 31) // 32)
     _launch("molly_process_logits", dev, logits.data_ptr(), dtype == BF16, _on(out, dev, what, "out"), rows, V, ldx, ldo, gen_at, n_at, n_hist, ldg,

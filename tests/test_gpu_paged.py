@@ -477,7 +477,7 @@ def test_refusals():
         (ValueError, lambda: o.paged_kv_append(k, k, bf, bf, slot.long())),
         (ValueError, lambda: o.paged_kv_append(k, k, bf, bf, slot, cos=cos, sin=cos)),
         (ValueError, lambda: o.paged_kv_append(k, k, bf, bf, slot, cos=cos[:, :16], sin=cos[:, :16], positions=slot)),
-        (ValueError, lambda: o.paged_kv_append(k, k, bf, bf, slot, qw=k[0, :64])),
+        (ValueError, lambda: o.paged_kv_append(k, k, bf, bf, slot, q_out=k)),
         (ValueError, lambda: o.paged_kv_append(k, k, bf, bf, slot, q=k[:, :100])),
         (ValueError, lambda: o.paged_kv_append(k, k, bf, bf, slot, kw=k[0])),
         (TypeError, lambda: o.paged_kv_append(k.half(), k, bf, bf, slot)),

@@ -21,8 +21,22 @@
 namespace {
 
 constexpr int RROWS = 32;                            // rows of a tile in the rows kernel; the tile kernel has 32 a wave
-constexpr int MIN_KEYS = 512;                        // fewest keys that a part of a cut key axis gets
 constexpr int MAX_PARTS = 64;
+
+// The parts that a tile's key axis is cut into, at most `parts`, and a part's keys (whole ones of `align`).  A part has 2^shift keys or so at least (`round`: what
+// counts as the last one); an axis of which a cut would take fewer than min_cut keys out of a block's way stays whole.
+//   single steps: a round of the block's waves or more, min_cut 400: the join costs 4 us and a key 9 ns.  1 x 700 keys bf16 11.1 -> 10.0 us, 1 x 2,000 15.1 (parts of 512 and
+//     more) -> 11.3, 4 x 2,000 15.9 -> 12.5; cut all the same, 1 x 300 7.9 -> 9.8, 16 x 700 e4m3 12.7 -> 14.7
+//   tiles: 512 keys or more, for their parts carry more rows (2 x 100 new tokens x 32 heads over 1,000 keys 19.7 us, parts of 128 21.8); 128 where that makes
+//     more parts, up to 16 and as long as they come to 10,240 rows (32 new tokens x 32 heads over 700 keys 15.3 -> 13.1 us, over 2,500 18.5 -> 15.5)
+struct CutRule { int parts, align, shift, round, min_cut; };
+struct Cut { int parts, keys; };
+__host__ __device__ inline Cut cut_keys(const CutRule& c, int n) {
+    const int most = (n + c.round) >> c.shift, d = c.parts < most ? c.parts : most;
+    if (d <= 1) return {1, n};
+    const int keys = ((n - 1) / d + c.align) / c.align * c.align;                     // n / d rounded up, to the next multiple
+    return n - keys < c.min_cut ? Cut{1, n} : Cut{(n - 1) / keys + 1, keys};
+}
 
 struct AttnPagedArgs {
     const bf16_t* q; bf16_t* out;
@@ -31,7 +45,7 @@ struct AttnPagedArgs {
     float* part;                                     // [tile][kv head][parts]: ROWS * HD un-normalised outputs, ROWS * 2 (max, sum)
     int n_tok, B, n_pages, page_shift, max_pages, ld_table, nh, nkv, G, ldq, ldo;
     int tps;                                         // rows kernel: tiles per sequence; tile kernel: bound of the tiles of all of them
-    int parts;                                       // most parts of a tile's key axis
+    CutRule cut;
     int class_bits;                                  // find_tile: 2^class_bits classes of 64 keys
     float scale_log2;                                // softmax scale * log2(e), > 0
 };
@@ -54,10 +68,6 @@ __device__ __forceinline__ Tile make_tile(const AttnPagedArgs& p, int b, int ti)
     t.n_vis = t.rows > 0 ? t.first + (t.row0 + t.rows - 1) / p.G + 1 : 0;
     return t;
 }
-// parts that a tile's key axis is cut into, and a part's keys (whole steps of ALIGN)
-__device__ __forceinline__ int parts_of(int n_keys, int parts) { return min(parts, max(n_keys / MIN_KEYS, 1)); }
-template <int ALIGN> __device__ __forceinline__ int part_keys(int n_keys, int parts) { return ((n_keys + parts - 1) / parts + ALIGN - 1) / ALIGN * ALIGN; }
-
 // ---- K / V steps ------------------------------------------------------------------------------------------------------------------------
 struct KvSource {
     const int* row;                                  // the sequence's page ids
@@ -360,7 +370,7 @@ __global__ __launch_bounds__(64 * rows_waves(HD, FP8), rows_waves(HD, FP8) / 4) 
     unsigned off[PIECES<HD, 16>];
     piece_offsets<HD, 16>(0, lane, off);
     int bid = blockIdx.x;
-    const int s = bid % p.parts; bid /= p.parts;
+    const int s = bid % p.cut.parts; bid /= p.cut.parts;
     const int kvh = bid % p.nkv; bid /= p.nkv;
     const int b = bid / p.tps;
     for (int ti = bid % p.tps;; ti += p.tps) {       // (a sequence has more tiles than p.tps only where the caller's max_q was too small)
@@ -368,11 +378,11 @@ __global__ __launch_bounds__(64 * rows_waves(HD, FP8), rows_waves(HD, FP8) / 4) 
         if (t.rows <= 0) return;
         const int kmax = p.max_pages << p.page_shift;
         const int n_keys = min(t.n_vis, kmax);
-        const int parts = ti < p.tps ? parts_of(n_keys, p.parts) : 1;
+        const Cut cut = ti < p.tps ? cut_keys(p.cut, n_keys) : Cut{1, n_keys};
+        const int parts = cut.parts, chunk = cut.keys;
         if (s >= parts) continue;
-        const int chunk = part_keys<STRIDE>(n_keys, parts);
         const int k0 = s * chunk, k1 = min(n_keys, k0 + chunk);
-        float* part = parts > 1 ? p.part + ((size_t)((b * p.tps + ti) * p.nkv + kvh) * p.parts + s) * (RROWS * (HD + 2)) : nullptr;
+        float* part = parts > 1 ? p.part + ((size_t)((b * p.tps + ti) * p.nkv + kvh) * p.cut.parts + s) * (RROWS * (HD + 2)) : nullptr;
         const int last = k1 - 1;
         const KvSource src{p.table + (size_t)t.b * p.ld_table, p.n_pages, p.page_shift, p.nkv, kvh};
         if (tid == 0) s_bad = t.n_vis > kmax ? kmax : 0x7fffffff;
@@ -566,7 +576,7 @@ __global__ __launch_bounds__(256, 2) void attn_paged_tile_kernel(AttnPagedArgs p
     const int wrow = KS == 1 ? wave * 32 : (wave & 1) * 32, kg = KS == 1 ? 0 : wave >> 1;
     // The workgroups of one XCD (every eighth) share the keys of as few (kv head, part) units as possible in its L2: whole units to an XCD where they can
     // be dealt evenly, every X-th tile of a unit to each of its X XCDs where there are fewer, else contiguous runs of (unit, tile).
-    const int units = p.nkv * p.parts, xcd = blockIdx.x & 7, i8 = blockIdx.x >> 3;
+    const int units = p.nkv * p.cut.parts, xcd = blockIdx.x & 7, i8 = blockIdx.x >> 3;
     int pos, unit, x = 0, X = 1;                     // the unit's XCDs take every X-th tile, this one those of rank x, x + X ..
     bool whole = true;
     if (units % 8 == 0) {
@@ -592,7 +602,7 @@ __global__ __launch_bounds__(256, 2) void attn_paged_tile_kernel(AttnPagedArgs p
     const int N = (total - x + X - 1) / X;
     if (pos >= N) return;
     const int f = (whole ? deal<HD == 128 || FP8 ? 2 : 4>(pos, N) : pos) * X + x;
-    const int s = unit % p.parts, kvh = unit / p.parts;
+    const int s = unit % p.cut.parts, kvh = unit / p.cut.parts;
     int ti = 0;
     const int b = __builtin_amdgcn_readfirstlane(find_tile<TROWS>(p, seq, f, lane, &ti));
     if (b < 0) return;
@@ -600,9 +610,9 @@ __global__ __launch_bounds__(256, 2) void attn_paged_tile_kernel(AttnPagedArgs p
     const Tile t = make_tile<TROWS>(p, b, ti);
     const int kmax = p.max_pages << p.page_shift;
     const int n_keys = min(t.n_vis, kmax);
-    const int parts = parts_of(n_keys, p.parts);
+    const Cut cut = cut_keys(p.cut, n_keys);
+    const int parts = cut.parts, chunk = cut.keys;
     if (s >= parts) return;
-    const int chunk = part_keys<64>(n_keys, parts);
     const int k0 = s * chunk, k1 = min(n_keys, k0 + chunk), last = k1 - 1;
     const KvSource src{p.table + (size_t)b * p.ld_table, p.n_pages, p.page_shift, p.nkv, kvh};
     if (tid == 0) s_bad = t.n_vis > kmax ? kmax : 0x7fffffff;
@@ -706,7 +716,7 @@ __global__ __launch_bounds__(256, 2) void attn_paged_tile_kernel(AttnPagedArgs p
     if (!active) return;
     if (st.qi >= s_bad) l = __builtin_nanf("");
     if (parts > 1) {
-        float* part = p.part + ((size_t)(f * p.nkv + kvh) * p.parts + s) * (TROWS * (HD + 2));
+        float* part = p.part + ((size_t)(f * p.nkv + kvh) * p.cut.parts + s) * (TROWS * (HD + 2));
         if (r < rows) {
             float* d = part + (size_t)(wrow + r) * HD;
 #pragma unroll
@@ -788,9 +798,9 @@ __global__ __launch_bounds__(256) void attn_paged_join_kernel(AttnPagedArgs p) {
     if constexpr (ROWS != RROWS) b = find_tile<ROWS>(p, load_seq<ROWS>(p, lane), tile, lane, &ti);
     if (b < 0) return;
     const Tile t = make_tile<ROWS>(p, b, ti);
-    const int parts = parts_of(min(t.n_vis, p.max_pages << p.page_shift), p.parts);
+    const int parts = cut_keys(p.cut, min(t.n_vis, p.max_pages << p.page_shift)).parts;
     if (parts == 1) return;                          // written by the attention itself
-    const float* base = p.part + (size_t)(tile * p.nkv + kvh) * p.parts * STRIDE;
+    const float* base = p.part + (size_t)(tile * p.nkv + kvh) * p.cut.parts * STRIDE;
     for (int row = blockIdx.y * 4 + (threadIdx.x >> 6); row < t.rows; row += gridDim.y * 4) {
         const int R = t.row0 + row, tok = R / p.G;
         join_parts<HD>(parts, [&](int s) { return base + (size_t)s * STRIDE + row * HD; }, (size_t)ROWS * HD + row * 2 - row * HD,
@@ -799,7 +809,7 @@ __global__ __launch_bounds__(256) void attn_paged_join_kernel(AttnPagedArgs p) {
 }
 
 // ---- host: which kernel, and how many parts
-struct Shape { int ks, tps, parts, rows, class_bits; long tiles, part_floats; };      // ks 0: the rows kernel
+struct Shape { int ks, tps, rows, class_bits; CutRule cut; long tiles, part_floats; };      // ks 0: the rows kernel
 Shape pick_shape(int n_tok, int B, int nkv, int G, int HD, bool fp8, long max_keys, int max_q, int max_kv) {
     Shape sh{};
     const long mq = max_q > 0 && max_q < n_tok ? max_q : n_tok;
@@ -814,10 +824,16 @@ Shape pick_shape(int n_tok, int B, int nkv, int G, int HD, bool fp8, long max_ke
     sh.tiles = sh.ks ? sh.tps : (long)sh.tps * B;
     const long units = sh.tiles * nkv, slots = sh.ks || (HD == 64 && fp8) ? 512 : 256;      // blocks that are resident at a time
     long parts = units > 0 ? slots / units : 1;
-    if (parts > keys / MIN_KEYS) parts = keys / MIN_KEYS;
-    if (parts > MAX_PARTS) parts = MAX_PARTS;
-    sh.parts = parts < 1 ? 1 : (int)parts;
-    sh.part_floats = sh.parts > 1 ? units * sh.parts * rows * (HD + 2) : 0;
+    parts = parts < 1 ? 1 : parts > MAX_PARTS ? MAX_PARTS : parts;
+    const int round = 32 * rows_waves(HD, fp8);
+    long few = 10240 / ((long)n_tok * G * nkv);
+    few = few < 16 ? few : 16;                       // (the join takes 8 parts at a time)
+    const long coarse = parts < keys / 512 ? parts : keys / 512;
+    if (!sh.ks) sh.cut = CutRule{(int)parts, round, round == 256 ? 8 : 7, round - 1, 400};
+    else if (few > coarse) sh.cut = CutRule{(int)(parts < few ? parts : few), 64, 7, 0, 400};
+    else sh.cut = CutRule{(int)parts, 64, 9, 0, 0};
+    sh.cut.parts = cut_keys(sh.cut, (int)(keys < 0x7ffffe00L ? keys : 0x7ffffe00L)).parts;
+    sh.part_floats = sh.cut.parts > 1 ? units * sh.cut.parts * rows * (HD + 2) : 0;
     return sh;
 }
 
@@ -832,10 +848,10 @@ void launch_tile(hipStream_t st, const AttnPagedArgs& p, const Shape& sh) {
     constexpr size_t stages = 2 * 2 * 64 * HD * 2, tail = KS == 2 ? 64 * HD * 4 + 2048 + 2 * 32 * (HD + 8) * 2 : 4 * 32 * (HD + 8) * 2, lds = stages > tail ? stages : tail;
     static const hipError_t once = hipFuncSetAttribute((const void*)attn_paged_tile_kernel<HD, FP8, KS>, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
     (void)once;
-    const int units = p.nkv * sh.parts;              // (the kernel's three ways to deal them to the 8 XCDs)
+    const int units = p.nkv * sh.cut.parts;              // (the kernel's three ways to deal them to the 8 XCDs)
     const long blocks = 8 % units == 0 ? 8L * cdiv(sh.tps, 8 / units) : 8L * cdiv((long)units * sh.tps, 8);
     hipLaunchKernelGGL((attn_paged_tile_kernel<HD, FP8, KS>), dim3((unsigned)blocks), dim3(256), lds, st, p);
-    if (sh.parts > 1) launch_join<HD, 128 / KS>(st, p, sh);
+    if (sh.cut.parts > 1) launch_join<HD, 128 / KS>(st, p, sh);
 }
 template <int HD, bool FP8>
 void launch(hipStream_t st, const AttnPagedArgs& p, const Shape& sh) {
@@ -845,8 +861,8 @@ void launch(hipStream_t st, const AttnPagedArgs& p, const Shape& sh) {
     const size_t lds = NW * RROWS * HD * 4 * (FP8 ? 1 : 2);           // images (e4m3: one buffer of 32 rows K | V in bf16), at the end the waves' rows in fp32
     static const hipError_t once = hipFuncSetAttribute((const void*)attn_paged_rows_kernel<HD, FP8>, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
     (void)once;
-    hipLaunchKernelGGL((attn_paged_rows_kernel<HD, FP8>), dim3((unsigned)(sh.tiles * p.nkv * sh.parts)), dim3(64 * NW), lds, st, p);
-    if (sh.parts > 1) launch_join<HD, RROWS>(st, p, sh);
+    hipLaunchKernelGGL((attn_paged_rows_kernel<HD, FP8>), dim3((unsigned)(sh.tiles * p.nkv * sh.cut.parts)), dim3(64 * NW), lds, st, p);
+    if (sh.cut.parts > 1) launch_join<HD, RROWS>(st, p, sh);
 }
 
 int check_sizes(int n_tokens, int B, int n_heads, int n_kv_heads, int max_pages, int page_size) {
@@ -888,8 +904,8 @@ extern "C" int molly_attn_paged(void* stream, const void* q, void* out, const vo
     p.n_pages = n_pages; p.page_shift = log2_exact(page_size); p.max_pages = max_pages; p.ld_table = ld_table;
     p.nh = n_heads; p.nkv = n_kv_heads; p.G = n_heads / n_kv_heads; p.ldq = ldq; p.ldo = ldo; p.scale_log2 = scale * LOG2E;
     Shape sh = pick_shape(n_tokens, B, n_kv_heads, p.G, head_dim, kscale_or_null != nullptr, (long)max_pages * page_size, max_q, max_kv);
-    if (!workspace || workspace_floats < sh.part_floats) sh.parts = 1;
-    p.part = workspace; p.tps = sh.tps; p.parts = sh.parts; p.class_bits = sh.class_bits;
+    if (!workspace || workspace_floats < sh.part_floats) sh.cut.parts = 1;
+    p.part = workspace; p.tps = sh.tps; p.cut = sh.cut; p.class_bits = sh.class_bits;
     hipStream_t st = (hipStream_t)stream;
     if (head_dim == 128) {
         if (kscale_or_null) launch<128, true>(st, p, sh);

@@ -445,7 +445,7 @@ int molly_attn_paged(void* stream, const void* q, void* out, const void* kpool, 
  * (out == logits allowed for fp32 with the same stride).  c = occurrences of the token among the first n_generated[row] (NULL: n_history)
  * entries of generated [rows][ld_generated] (ids outside 0 .. V - 1 are ignored):
  *   c > 0: s = (s < 0 ? s * repetition : s / repetition) - presence - frequency * c;  s += bias;  s = -inf where the token is not allowed
- * (HF:generation/logits_process.py RepetitionPenaltyLogitsProcessor, then the additive ones, then the hard ones).  The three penalties: scalars, or
+ * (the order of HF:generation/logits_process.py: repetition, then the additive ones, then the hard ones).  The three penalties: scalars, or
  * fp32 [rows] where *_rows is given.  bias fp32 [V] (ld_bias 0: one for all rows) or [rows][ld_bias]; allowed: bit v & 31 of word v >> 5 set =
  * token v allowed, [words] (ld_allowed 0) or [rows][ld_allowed].  V <= 2^30, rows <= 65535. */
 int molly_process_logits(void* stream, const void* logits, int logits_bf16, float* out, int rows, int V, long ld_logits, long ld_out,

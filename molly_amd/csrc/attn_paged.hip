@@ -25,8 +25,8 @@ constexpr int MAX_PARTS = 64;
 
 // The parts that a tile's key axis is cut into, at most `parts`, and a part's keys (whole ones of `align`).  A part has 2^shift keys or so at least (`round`: what
 // counts as the last one); an axis of which a cut would take fewer than min_cut keys out of a block's way stays whole.
-//   single steps: a round of the block's waves or more, min_cut 400: the join costs 4 us and a key 9 ns.  1 x 700 keys bf16 11.1 -> 10.0 us, 1 x 2,000 15.1 (parts of 512 and
-//     more) -> 11.3, 4 x 2,000 15.9 -> 12.5; cut all the same, 1 x 300 7.9 -> 9.8, 16 x 700 e4m3 12.7 -> 14.7
+//   single steps: a round of the block's waves or more, min_cut 400: the join costs 4 us and a key 9 ns.  1 x 700 keys bf16 11.1 -> 9.5 us, 1 x 2,000 15.1 (parts of 512 and
+//     more) -> 10.7, 4 x 2,000 15.9 -> 12.8; cut all the same, 1 x 300 7.9 -> 9.8, 16 x 700 e4m3 12.7 -> 14.7
 //   tiles: 512 keys or more, for their parts carry more rows (2 x 100 new tokens x 32 heads over 1,000 keys 19.7 us, parts of 128 21.8); 128 where that makes
 //     more parts, up to 16 and as long as they come to 10,240 rows (32 new tokens x 32 heads over 700 keys 15.3 -> 13.1 us, over 2,500 18.5 -> 15.5)
 struct CutRule { int parts, align, shift, round, min_cut; };

@@ -1,8 +1,8 @@
 // Logit processors in front of the draw: penalties for repeated tokens, a bias and a mask of allowed tokens, in one pass over the row.
 //   c    = how often the token occurs in the row's generated sequence
-//   c > 0:  s = (s < 0 ? s * repetition : s / repetition) - presence       (the first is HF's RepetitionPenaltyLogitsProcessor,
-//   s   -= frequency * c                                                    HF:generation/logits_process.py; the reference's generate passes
-//   s   += bias[token]                                                      repetition_penalty through, src/model/omics_one.py:220-232)
+//   c > 0:  s = (s < 0 ? s * repetition : s / repetition) - presence       (the first as in HF:generation/logits_process.py; the
+//   s   -= frequency * c                                                    reference's generate passes repetition_penalty through,
+//   s   += bias[token]                                                      src/model/omics_one.py:220-232)
 //   s    = -inf where the token's bit of the mask is 0                     (HF's prefix_allowed_tokens_fn / bad_words_ids)
 // One workgroup = one row x one slice of the vocabulary: it counts the row's history into LDS (integer atomics: the order changes
 // nothing), then makes the slice's pass.  Bound by HBM: the logits are read once and written once; the history comes from L2 once per slice.

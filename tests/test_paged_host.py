@@ -92,7 +92,7 @@ def test_entry_points_refuse_bad_arguments():
                      (dict(n=1 << 30), "more tiles"), (dict(ws=P + 4, wsf=100), "workspace")):
         rejects("molly_attn_paged", text, *attn(**kw))
     assert L.fn["molly_attn_paged"](None, *attn(n=0)) == 0 and L.fn["molly_attn_paged"](None, *attn(B=0)) == 0
-    assert ops.attn_paged_workspace(1, 1, 16, 8, 128, 64, 15, False) == 0 and ops.attn_paged_workspace(1, 1, 16, 8, 128, 64, 1000, False) > 0
+    assert ops.attn_paged_workspace(1, 1, 16, 8, 128, 64, 6, False) == 0 and ops.attn_paged_workspace(1, 1, 16, 8, 128, 64, 1000, False) > 0
     assert ops.attn_paged_workspace(-1, 1, 16, 8, 128, 64, 1000, False) == 0 and ops.attn_paged_workspace(1, 1, 15, 8, 128, 64, 1000, False) == 0
 
     def logits(x=P, out=P, rows=2, V=100, ldx=100, ldo=100, gen=None, n=0, ldg=0, rep=1.0, bias=None, ldb=0, allowed=None, ldm=0):

@@ -123,35 +123,50 @@ __device__ __forceinline__ void dma_rows_clamped(const char* base, unsigned lds,
 __device__ __forceinline__ void lds_read_done() { asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory"); }
 template <int N> __device__ __forceinline__ void wait_vm() { asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory"); }
 
-// R rows of a 16-key group as e4m3 codes through registers: NL loads of 16 codes a lane, K's units first, then V's.  Lanes go over the 4 rows of a block
-// first: the stores into the image are free of bank conflicts.
-template <int HD, int R> struct Codes {
-    static constexpr int UPM = R * HD / 16, NL = 2 * UPM / 64;       // units of 16 codes per matrix; loads a lane
+// A 16-key group as e4m3 codes through registers: NL loads of 16 codes a lane, K's units first, then V's.
+template <int HD> struct Codes {
+    static constexpr int UPM = HD, NL = 2 * UPM / 64;                // units of 16 codes per matrix; loads a lane
     u32x4 c[NL];
     uint8_t e[NL];
 };
-template <int HD, int R, bool NT>
-__device__ __forceinline__ void codes_load(Codes<HD, R>& c, const AttnPagedArgs& p, size_t at, int r0, int lim, int lane) {
-    constexpr int NCB = HD / 16, LRB = NCB * 4, UPM = Codes<HD, R>::UPM;
+// a lane's unit: row block (of 4), row in it, column block.  Eight neighbouring lanes take four rows and the four of the row block after the next, whose halves
+// lie the other way round in the image: their stores meet in no bank.  (Four rows of two column blocks: two lanes in every bank, 29 % of the LDS cycles of
+// a mixed batch; 6 x 301 new tokens over 2,500 keys 120 -> 113 us, 2,048 over 16,384 531 -> 519.)  But a load takes half of 128-byte rows then,
+// and the streaming ones (NT) fetch them twice: 32 x 4,000 keys 49.0 -> 64.9 us, so those take whole rows.
+template <int HD, bool NT> __device__ __forceinline__ void code_unit(int w, int& rb, int& r, int& cb) {
+    r = w & 3;
+    if constexpr (NT && HD == 128) {
+        cb = (w >> 2) & 7;
+        rb = w >> 5;
+    } else {
+        rb = ((w >> 2) & 1) * 2 + ((w >> 3) & 1);
+        cb = w >> 4;
+    }
+}
+template <int HD, bool NT>
+__device__ __forceinline__ void codes_load(Codes<HD>& c, const AttnPagedArgs& p, size_t at, int lim, int lane) {
 #pragma unroll
-    for (int j = 0; j < Codes<HD, R>::NL; ++j) {
-        const int u = j * 64 + lane, w = u % UPM;
-        const bool isv = u >= UPM;
-        const int row = min((r0 & 15) + w / LRB * 4 + (w & 3), lim), cb = (w >> 2) & (NCB - 1);
-        const size_t key = at + row;
+    for (int j = 0; j < Codes<HD>::NL; ++j) {
+        const int u = j * 64 + lane;
+        const bool isv = u >= Codes<HD>::UPM;
+        int rb, r, cb;
+        code_unit<HD, NT>(u % Codes<HD>::UPM, rb, r, cb);
+        const size_t key = at + min(rb * 4 + r, lim);
         const u32x4* src = reinterpret_cast<const u32x4*>((isv ? p.vpool : p.kpool) + key * HD + cb * 16);
         c.c[j] = NT ? __builtin_nontemporal_load(src) : *src;
         c.e[j] = (isv ? p.vscale : p.kscale)[key];
     }
 }
-template <int HD, int R>
-__device__ __forceinline__ void codes_store(const Codes<HD, R>& c, bf16_t* imgk, bf16_t* imgv, int r0, int lane) {      // the tile's images
-    constexpr int NCB = HD / 16, LRB = NCB * 4, UPM = Codes<HD, R>::UPM;
+template <int HD, bool NT>
+__device__ __forceinline__ void codes_store(const Codes<HD>& c, bf16_t* imgk, bf16_t* imgv, int r0, int lane) {      // rows r0 .. of the tile's images
+    constexpr int NCB = HD / 16;
 #pragma unroll
-    for (int j = 0; j < Codes<HD, R>::NL; ++j) {
-        const int u = j * 64 + lane, w = u % UPM;
-        const int rbl = (r0 >> 2) + w / LRB, cb = (w >> 2) & (NCB - 1), b0 = rbl & 1, b1 = (rbl >> 1) & 1;
-        bf16_t* d = (u >= UPM ? imgv : imgk) + (rbl * NCB + (cb ^ b0)) * 64 + (w & 3) * 16;
+    for (int j = 0; j < Codes<HD>::NL; ++j) {
+        const int u = j * 64 + lane;
+        int rb, r, cb;
+        code_unit<HD, NT>(u % Codes<HD>::UPM, rb, r, cb);
+        const int rbl = (r0 >> 2) + rb, b0 = rbl & 1, b1 = (rbl >> 1) & 1;
+        bf16_t* d = (u >= Codes<HD>::UPM ? imgv : imgk) + (rbl * NCB + (cb ^ b0)) * 64 + r * 16;
         const float scale = exp2i((int)c.e[j] - 127);
         *reinterpret_cast<u32x4*>(d + b1 * 8) = e4m3_to_bf8(u32x2{c.c[j][0], c.c[j][1]}, scale);
         *reinterpret_cast<u32x4*>(d + (b1 ^ 1) * 8) = e4m3_to_bf8(u32x2{c.c[j][2], c.c[j][3]}, scale);
@@ -420,20 +435,20 @@ __global__ __launch_bounds__(64 * rows_waves(HD, FP8), rows_waves(HD, FP8) / 4) 
         if constexpr (FP8) {
             // (one step's codes on their way in registers; three, at one block a CU, were slower: 52.8 us against 45.8 for 32 x 1,000..4,000 keys.  A lone wave
             // spends 1.3 us a step, 0.65 of it in attend32 and 0.37 in the conversion: it is a second wave on the SIMD that hides them)
-            Codes<HD, 16> c[2];
+            Codes<HD> c[2];
             auto load_step = [&](int key) {
                 const int i = look(key);
 #pragma unroll
                 for (int g = 0; g < 2; ++g) {
                     const int kb = key + 16 * g, kc = min(kb, last & ~15);
-                    codes_load<HD, 16, true>(c[g], p, src.group(kc, __builtin_amdgcn_readlane(pages, 2 * i + g)), 0, kb > last ? 0 : min(last - kc, 15), lane);
+                    codes_load<HD, true>(c[g], p, src.group(kc, __builtin_amdgcn_readlane(pages, 2 * i + g)), kb > last ? 0 : min(last - kc, 15), lane);
                 }
             };
             if (key0 < k1) load_step(key0);
 #pragma unroll 1
             for (int key = key0; key < k1; key += STRIDE) {
 #pragma unroll
-                for (int g = 0; g < 2; ++g) codes_store<HD, 16>(c[g], img, img + IMG, 16 * g, lane);
+                for (int g = 0; g < 2; ++g) codes_store<HD, true>(c[g], img, img + IMG, 16 * g, lane);
                 if (key + STRIDE < k1) load_step(key + STRIDE);
                 attend32<HD, true>(st, img, img + IMG, 0, key, p.scale_log2, lane);
             }
@@ -627,7 +642,7 @@ __global__ __launch_bounds__(256, 2) void attn_paged_tile_kernel(AttnPagedArgs p
     const unsigned smem_lds = __builtin_amdgcn_readfirstlane((unsigned)(uintptr_t)LDS_PTR(smem));
     const int tiles = k1 > k0 ? (k1 - k0 + 63) >> 6 : 0;
     int pages = 0;                                   // page ids of this wave's rows of the next 64 tiles (waited for once in 4,096 keys)
-    Codes<HD, R> c;
+    Codes<HD> c;
     auto issue = [&](int i) {                        // tile i
         if ((i & 63) == 0) {
             pages = src.row[min(k0 + 64 * (i + lane) + (r0 & ~15), last) >> p.page_shift];
@@ -636,7 +651,7 @@ __global__ __launch_bounds__(256, 2) void attn_paged_tile_kernel(AttnPagedArgs p
         const int kb = k0 + 64 * i + (r0 & ~15), kc = min(kb, last & ~15);
         const size_t at = src.group(kc, __builtin_amdgcn_readlane(pages, i & 63));
         if constexpr (FP8) {
-            codes_load<HD, R, false>(c, p, at, r0, kb > last ? 0 : min(last - kc, 15), lane);
+            codes_load<HD, false>(c, p, at, kb > last ? 0 : min(last - kc, 15), lane);
         } else {
             const unsigned dst = smem_lds + ((i & 1) * 2 * TILE + r0 * HD) * 2;
             if (kb + 15 <= last) {
@@ -652,7 +667,7 @@ __global__ __launch_bounds__(256, 2) void attn_paged_tile_kernel(AttnPagedArgs p
     auto land = [&](int i) {                         // this wave's rows of tile i are in LDS
         if constexpr (FP8) {
             bf16_t* img = smem + (i & 1) * 2 * TILE;
-            codes_store<HD, R>(c, img, img + TILE, r0, lane);
+            codes_store<HD, false>(c, img, img + TILE, r0, lane);
             if (i + 1 < tiles) issue(i + 1);         // (the codes go out a whole tile ahead)
         } else {
             dma_wait();

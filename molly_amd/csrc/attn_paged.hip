@@ -25,8 +25,9 @@ constexpr int MAX_PARTS = 64;
 
 // The parts that a tile's key axis is cut into, at most `parts`, and a part's keys (whole ones of `align`).  A part has 2^shift keys or so at least (`round`: what
 // counts as the last one); an axis of which a cut would take fewer than min_cut keys out of a block's way stays whole.
-//   single steps: a round of the block's waves or more, min_cut 400: the join costs 4 us and a key 9 ns.  1 x 700 keys bf16 11.1 -> 9.5 us, 1 x 2,000 15.1 (parts of 512 and
-//     more) -> 10.7, 4 x 2,000 15.9 -> 12.8; cut all the same, 1 x 300 7.9 -> 9.8, 16 x 700 e4m3 12.7 -> 14.7
+//   single steps: a round of the block's waves or more, min_cut 700.  On the GPU the join costs 4 us and a key 9 ns, and a cut pays from 400 keys on (1 x 700
+//     keys bf16 11.1 -> 9.5 us in a graph; 1 x 300 7.9 -> 9.8); called one by one the second launch and its scratch cost the host 4 us more, and it pays from 1,000
+//     on (1 x 700 11.5 -> 15.2).  1 x 2,000 in a graph 15.1 (parts of 512 and more) -> 10.7, 4 x 2,000 15.9 -> 12.8; 16 x 700 e4m3, cut in two, 12.7 -> 14.7
 //   tiles: 512 keys or more, for their parts carry more rows (2 x 100 new tokens x 32 heads over 1,000 keys 19.7 us, parts of 128 21.8); 128 where that makes
 //     more parts, up to 16 and as long as they come to 10,240 rows (32 new tokens x 32 heads over 700 keys 15.3 -> 13.1 us, over 2,500 18.5 -> 15.5)
 struct CutRule { int parts, align, shift, round, min_cut; };
@@ -844,7 +845,7 @@ Shape pick_shape(int n_tok, int B, int nkv, int G, int HD, bool fp8, long max_ke
     long few = 10240 / ((long)n_tok * G * nkv);
     few = few < 16 ? few : 16;                       // (the join takes 8 parts at a time)
     const long coarse = parts < keys / 512 ? parts : keys / 512;
-    if (!sh.ks) sh.cut = CutRule{(int)parts, round, round == 256 ? 8 : 7, round - 1, 400};
+    if (!sh.ks) sh.cut = CutRule{(int)parts, round, round == 256 ? 8 : 7, round - 1, 700};
     else if (few > coarse) sh.cut = CutRule{(int)(parts < few ? parts : few), 64, 7, 0, 400};
     else sh.cut = CutRule{(int)parts, 64, 9, 0, 0};
     sh.cut.parts = cut_keys(sh.cut, (int)(keys < 0x7ffffe00L ? keys : 0x7ffffe00L)).parts;

@@ -545,6 +545,7 @@ template <int TROWS> __device__ __forceinline__ Seq load_seq(const AttnPagedArgs
 template <int TROWS> __device__ __forceinline__ int find_tile(const AttnPagedArgs& p, Seq q, int rank, int lane, int* ti) {
     const float per_key = (float)p.G / TROWS;
     for (int b0 = 0;;) {
+        const Seq next = load_seq<TROWS>(p, b0 + 64 + lane);
         const int total = wave_total(q.n);
         if (rank < total) {
             if (p.B == 1) {
@@ -568,7 +569,7 @@ template <int TROWS> __device__ __forceinline__ int find_tile(const AttnPagedArg
         rank -= total;
         b0 += 64;
         if (b0 >= p.B) return -1;
-        q = load_seq<TROWS>(p, b0 + lane);
+        q = next;
     }
 }
 // The rank of an XCD's block `pos`, of N.  Blocks start in order, the first 32 on a compute unit each, the next 32 on the same ones in the same order, while there is
@@ -612,12 +613,13 @@ __global__ __launch_bounds__(256, 2) void attn_paged_tile_kernel(AttnPagedArgs p
         whole = false;
     }
     const Seq seq = load_seq<TROWS>(p, lane);
-    int total = wave_total(seq.n);
-    for (int b0 = 64; b0 < p.B; b0 += 64) total += wave_total(load_seq<TROWS>(p, b0 + lane).n);
-    total = min(total, p.tps);                       // (more only where cu_q does not ascend)
-    const int N = (total - x + X - 1) / X;
-    if (pos >= N) return;
-    const int f = (whole ? deal<HD == 128 || FP8 ? 2 : 4>(pos, N) : pos) * X + x;
+    int f = pos * X + x;
+    if (whole && p.B <= 64) {                        // (more sequences: more tiles than start at once)
+        const int total = min(wave_total(seq.n), p.tps), N = (total - x + X - 1) / X;
+        if (pos >= N) return;
+        f = deal<HD == 128 || FP8 ? 2 : 4>(pos, N) * X + x;
+    }
+    if (f >= p.tps) return;                          // (more tiles than that only where cu_q does not ascend)
     const int s = unit % p.cut.parts, kvh = unit / p.cut.parts;
     int ti = 0;
     const int b = __builtin_amdgcn_readfirstlane(find_tile<TROWS>(p, seq, f, lane, &ti));

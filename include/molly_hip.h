@@ -428,7 +428,7 @@ int molly_paged_kv_read(void* stream, const void* kpool, const void* vpool, cons
                         int ldk, int ldv);
 /* attention of ragged chunks of new tokens over the pages: sequence b has the q rows cu_q[b] .. cu_q[b + 1] - 1 (cu_q int [B + 1], ascending),
  * kv_len[b] keys in the cache, the new tokens' own among them (they are its last ones), and key j in page block_table[b][j / page_size] (row
- * stride ld_table).  Row i of the n new ones sees the keys 0 .. kv_len[b] - n + i; a row that sees none comes out as zeros; a row
+ * stride ld_table; max_pages * page_size < 2^31 - 2^15).  Row i of the n new ones sees the keys 0 .. kv_len[b] - n + i; a row that sees none comes out as zeros; a row
  * one of whose keys lies on a page outside 0 .. n_pages - 1, or behind max_pages, comes out as NaN (no memory outside the pools is read); rows
  * in front of cu_q[0] or behind cu_q[B] are left as they were.  One new token a sequence is the decode step.  scale > 0.
  * max_q / max_kv: the most new tokens / keys of any sequence, as far as the caller knows (0: no idea); they choose how the work is cut, never the

@@ -22,6 +22,9 @@ namespace {
 
 constexpr int RROWS = 32;                            // rows of a tile in the rows kernel; the tile kernel has 32 a wave
 constexpr int MAX_PARTS = 64;
+// Most keys a sequence's row of the table may hold.  Key numbers are ints, and some are taken beyond the last key: the lookup of the page ids asks 31 steps of 256
+// keys and 16 ahead (7,952), and the parts of a cut axis, each rounded up to 256 keys, end up to 64 * 256 = 16,384 behind it.
+constexpr long MAX_KEYS = 0x7fffffffL - 32768;
 
 // The parts that a tile's key axis is cut into, at most `parts`, and a part's keys (whole ones of `align`).  A part has 2^shift keys or so at least (`round`: what
 // counts as the last one); an axis of which a cut would take fewer than min_cut keys out of a block's way stays whole.
@@ -850,7 +853,7 @@ Shape pick_shape(int n_tok, int B, int nkv, int G, int HD, bool fp8, long max_ke
     if (!sh.ks) sh.cut = CutRule{(int)parts, round, round == 256 ? 8 : 7, round - 1, 700};
     else if (few > coarse) sh.cut = CutRule{(int)(parts < few ? parts : few), 64, 7, 0, 400};
     else sh.cut = CutRule{(int)parts, 64, 9, 0, 0};
-    sh.cut.parts = cut_keys(sh.cut, (int)(keys < 0x7ffffe00L ? keys : 0x7ffffe00L)).parts;
+    sh.cut.parts = cut_keys(sh.cut, (int)keys).parts;
     sh.part_floats = sh.cut.parts > 1 ? units * sh.cut.parts * rows * (HD + 2) : 0;
     return sh;
 }
@@ -886,7 +889,7 @@ void launch(hipStream_t st, const AttnPagedArgs& p, const Shape& sh) {
 int check_sizes(int n_tokens, int B, int n_heads, int n_kv_heads, int max_pages, int page_size) {
     MOLLY_CHECK(n_tokens >= 0 && B >= 0 && max_pages >= 0, "attn_paged: n_tokens=%d B=%d max_pages=%d", n_tokens, B, max_pages);
     MOLLY_CHECK(n_heads > 0 && n_kv_heads > 0 && n_heads % n_kv_heads == 0, "attn_paged: n_heads=%d not a multiple of n_kv_heads=%d", n_heads, n_kv_heads);
-    MOLLY_CHECK((long)max_pages * page_size <= 0x7ffffe00L, "attn_paged: %d pages of %d keys a sequence: keys are 32-bit", max_pages, page_size);
+    MOLLY_CHECK((long)max_pages * page_size <= MAX_KEYS, "attn_paged: %d pages of %d keys a sequence, more than 2^31 - 2^15 - 1: keys are 32-bit", max_pages, page_size);
     MOLLY_CHECK((long)n_tokens * n_heads / n_kv_heads <= 0x1fffffffL && ((long)n_tokens * n_heads / 32 + 2L * B * n_kv_heads) * MAX_PARTS <= 0x7fffffffL,
                 "attn_paged: n_tokens=%d x n_heads=%d, B=%d: more tiles than one call takes", n_tokens, n_heads, B);
     return 0;

@@ -101,3 +101,24 @@ def test_entry_points_refuse_bad_arguments():
                      (dict(rep=0.0), "must be > 0"), (dict(bias=P, ldb=50), "ld_bias=50"), (dict(allowed=P, ldm=3), "ld_allowed=3"), (dict(x=None), "required")):
         rejects("molly_process_logits", text, *logits(**kw))
     assert L.fn["molly_process_logits"](None, *logits(rows=0)) == 0
+
+
+def test_key_numbers_stay_in_32_bits():
+    """The kernels count keys in ints and run ahead of the last one: the page lookup by 31 steps of 256 keys and 16, the end of the last part by what the parts
+    were rounded up by.  At the largest table that is taken none of it passes 2^31 - 1; a larger one is refused."""
+    L, P, most = _lib.lib(), 1 << 20, 0x7fffffff - 32768
+
+    def call(page, pages):                                        # (no new tokens: nothing is launched, the sizes are checked)
+        return L.fn["molly_attn_paged"](None, P, P, P, P, None, None, P, P, P, 0, 5, 4, page, pages, pages, 1, 1, 64, 64, 64, 1.0, 0, 0, None, 0)
+    for page in (16, 32, 64, 128, 256):
+        pages = most // page
+        assert call(page, pages) == 0
+        for p in (pages + 1, (0x7fffffff - 8192) // page, 0x7ffffe00 // page):
+            assert call(page, p) != 0 and "32-bit" in L.last_error()
+            assert ops.attn_paged_workspace(5, 5, 1, 1, 64, page, p, False, 1, 0) == 0
+    keys = most // 16 * 16
+    for parts in range(1, 65):
+        for align, ahead in ((256, 31 * 256 + 16), (128, 31 * 128 + 16), (64, 63 * 64 + 48)):
+            assert keys - 1 + ahead <= 0x7fffffff and keys + align <= 0x7fffffff
+            part = ((keys - 1) // parts + align) // align * align                         # n / parts rounded up, to the next multiple
+            assert -(-keys // part) * part <= 0x7fffffff

@@ -250,7 +250,7 @@ __global__ __launch_bounds__(1024) void sample_kernel(float* __restrict__ logits
         const float u = (float)(rnd[0] >> 8) * (1.0f / 16777216.0f) * ksum;
         float acc = 0.f;
         int pick = n_keep - 1;
-        while (pick > 0 && s_val[pick] == 0.f) --pick;               // (u may round up to ksum: never a token without mass, such as a masked one)
+        while (pick > 0 && s_val[pick] == 0.f) --pick;               // (u may round up to ksum: never a token without mass, such as a masked one, beside one that has some)
         for (int j = 0; j < n_keep; ++j) {
             acc += s_val[j];
             if (u < acc) { pick = j; break; }

@@ -450,6 +450,18 @@ def allowed_bits(allowed, vocab: int, device) -> torch.Tensor:
     return torch.where(w >= 1 << 31, w - (1 << 32), w).to(torch.int32).to(device)
 
 
+def _require_a_token(logits, unfinished):
+    """-> logits [rows, V], with an error where an unfinished row has no token left (every score -inf).  A row that has ended says its pad token whatever
+    its scores are: without one they become zeros, for the draw that is not used."""
+    dead = logits.amax(1) == float("-inf")
+    if not bool(dead.any()):
+        return logits
+    if bool((dead & unfinished).any()):
+        raise ValueError(f"generate: no token is left in row {int((dead & unfinished).nonzero()[0])}: what is allowed is banned by min_new_tokens, "
+                         "no_repeat_ngram_size or logit_bias")
+    return logits.masked_fill(dead[:, None], 0.0)
+
+
 def _bias_row(logit_bias, vocab: int, device) -> torch.Tensor:
     """{token: bias} or a [vocab] tensor -> fp32 [vocab]"""
     if torch.is_tensor(logit_bias):
@@ -476,7 +488,8 @@ def generate(model, input_ids, attention_mask=None, omic_ids=None, omic_info_lis
     the processors, in front of the warpers).
     kv_cache / prefill_chunk: GenerationSession.  presence_penalty, frequency_penalty (subtracted once / once an occurrence for every token generated
     so far), logit_bias ({token: added} or [V]) and prefix_allowed_tokens_fn(row, generated ids) -> allowed tokens (HF's) go, with the repetition
-    penalty, through one kernel in front of the warpers (ops.process_logits)."""
+    penalty, through one kernel in front of the warpers (ops.process_logits).  A row that has not ended and of which they, the n-gram rule and
+    min_new_tokens leave no token is a ValueError."""
     extra = bool(presence_penalty or frequency_penalty or logit_bias is not None or prefix_allowed_tokens_fn is not None)
     if num_beams and num_beams > 1:
         if min_new_tokens:
@@ -492,6 +505,8 @@ def generate(model, input_ids, attention_mask=None, omic_ids=None, omic_info_lis
     B = input_ids.shape[0]
     dev = logits.device
     bias = None if logit_bias is None else _bias_row(logit_bias, logits.shape[1], dev)
+    # what can take a row's last token away (penalties and finite biases cannot)
+    bans = prefix_allowed_tokens_fn is not None or (bias is not None and bool((bias == float("-inf")).any()))
     eos = None if eos_token_id is None else torch.as_tensor(eos_token_id, device=dev).reshape(-1)
     pad = pad_token_id if pad_token_id is not None else (int(eos[0]) if eos is not None else 0)
     out = torch.empty(B, 0, dtype=torch.int64, device=dev)
@@ -524,6 +539,8 @@ def generate(model, input_ids, attention_mask=None, omic_ids=None, omic_info_lis
             logits = ops.process_logits(logits, generated=out if out.shape[1] else None, repetition_penalty=float(repetition_penalty or 1.0),
                                         presence_penalty=float(presence_penalty), frequency_penalty=float(frequency_penalty), bias=bias, allowed=allowed)
             penalty = None                                  # (done)
+            if bans:
+                logits = _require_a_token(logits, unfinished)
         if fused:
             nxt = ops.sample_logits(logits, out if out.shape[1] else None, penalty, temperature, top_k, top_p,
                                     seed, it)

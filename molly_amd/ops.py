@@ -578,7 +578,8 @@ def argmax(logits: torch.Tensor, out: Optional[torch.Tensor] = None) -> torch.Te
 
 def sample_logits(logits, generated, repetition_penalty, temperature, top_k, top_p, seed, step, out=None, debug_cap=0):
     """HF's sampling processors + one draw per row on the device (molly_sample_logits).  logits fp32 [rows, V] (modified in
-    place by the repetition penalty); generated int64 [rows, n] or None.  -> next tokens int64 [rows]
+    place by the repetition penalty); generated int64 [rows, n] or None.  A row whose scores are all -inf has no draw: it gives some id of the
+    vocabulary.  -> next tokens int64 [rows]
     (+ (probs, ids, n_kept) of the surviving tokens when debug_cap > 0)."""
     assert logits.dtype == torch.float32 and logits.stride(1) == 1
     rows, V = logits.shape

@@ -162,3 +162,24 @@ def test_refusals(tiny_meta):
             m.generate(ids, mask, omic, info, do_sample=False, max_new_tokens=4, prefix_allowed_tokens_fn=bad)
     with pytest.raises(ValueError):
         m.generate(ids, mask, omic, info, do_sample=False, max_new_tokens=4, molly_logit_bias={5000: 1.0})
+
+
+@pytest.mark.parametrize("how", [dict(do_sample=False), dict(do_sample=True, top_k=20, temperature=0.8, top_p=0.95), dict(do_sample=True, temperature=0.8, top_p=1.0)])
+def test_a_row_without_a_token_is_an_error(tiny_meta, how):
+    """What is allowed is banned by another rule: the same error for greedy, fused and plain draws; no error for a row that has ended."""
+    m = build_tiny(tiny_meta)
+    ids, mask, omic, info = _left_padded_batch(tiny_meta)
+    gen = lambda **kw: m.generate(ids, mask, omic, info, generator=torch.Generator(device="cuda").manual_seed(0), **how, **kw)  # noqa: E731
+    m.text_config.eos_token_id = 9
+    with pytest.raises(ValueError, match="no token is left in row 1"):
+        gen(max_new_tokens=4, min_new_tokens=2, prefix_allowed_tokens_fn=lambda r, x: [9] if r else range(50, 90))
+    with pytest.raises(ValueError, match="no token is left"):     # 1, 2, 1, then 2 would make a pair that was there
+        gen(max_new_tokens=4, no_repeat_ngram_size=2, prefix_allowed_tokens_fn=lambda r, x: [1 + len(x) % 2])
+    b = torch.full((m.text_config.vocab_size,), -float("inf"))
+    with pytest.raises(ValueError, match="no token is left in row 0"):
+        gen(max_new_tokens=4, molly_logit_bias=b)
+    b[70] = 0.0
+    assert (gen(max_new_tokens=3, molly_logit_bias=b) == 70).all()
+    # row 0 ends with its first token; that it may then say nothing but what is banned is nobody's business
+    out = gen(max_new_tokens=3, no_repeat_ngram_size=1, prefix_allowed_tokens_fn=lambda r, x: [60 + len(x)] if r else [9])
+    assert out[0].tolist() == [9, m.text_config.pad_token_id, m.text_config.pad_token_id] and out[1].tolist() == [60, 61, 62]

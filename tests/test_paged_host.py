@@ -3,7 +3,7 @@ import pytest
 import torch
 
 from molly_amd import _lib, ops
-from molly_amd.generate import _bias_row, allowed_bits
+from molly_amd.generate import _bias_row, _require_a_token, allowed_bits
 from molly_amd.paged import PagedKVCache
 
 
@@ -52,6 +52,20 @@ def test_allowed_bits_and_bias():
     for bad in ({V: 1.0}, {-1: 1.0}, torch.zeros(V + 1)):
         with pytest.raises(ValueError):
             _bias_row(bad, V, "cpu")
+
+
+def test_rows_without_a_token_are_refused():
+    inf = float("inf")
+    x = torch.zeros(3, 7)
+    x[0, 1:], x[2, :] = -inf, -inf
+    on = torch.ones(3, dtype=torch.bool)
+    with pytest.raises(ValueError, match="row 2"):
+        _require_a_token(x, on)
+    assert torch.equal(_require_a_token(x[:2], on[:2]), x[:2])
+    y = _require_a_token(x, torch.tensor([True, True, False]))    # a row that has ended needs none
+    assert torch.equal(y[:2], x[:2]) and not y[2].any()
+    x[2, 3] = float("nan")                                        # (not finite for another reason: not this refusal's)
+    _require_a_token(x, on)
 
 
 def test_wrappers_refuse_host_tensors():

@@ -196,7 +196,9 @@ extern "C" int molly_paged_kv_append(void* stream, const void* k, const void* v,
     MOLLY_ENTER();
     if (int rc = check_pool("paged_kv_append", kpool, vpool, kscale_or_null, vscale_or_null, n_pages, page_size, n_kv_heads, head_dim)) return rc;
     const int nq = q_or_null ? n_heads : 0;
-    MOLLY_CHECK(n_rows >= 0 && nq >= 0 && k && v && slot, "paged_kv_append: n_rows=%d n_heads=%d; k, v, slot required", n_rows, n_heads);
+    MOLLY_CHECK(n_rows >= 0, "paged_kv_append: n_rows=%d", n_rows);
+    if (n_rows == 0) return 0;                       // (no rows have no address: nothing else is asked of them)
+    MOLLY_CHECK(nq >= 0 && k && v && slot, "paged_kv_append: n_heads=%d; k, v, slot required", n_heads);
     MOLLY_CHECK((q_or_null == nullptr) == (q_out_or_null == nullptr), "paged_kv_append: q and q_out go together");
     MOLLY_CHECK((cos == nullptr) == (sin == nullptr) && (cos == nullptr || (positions != nullptr && n_pos > 0)),
                 "paged_kv_append: cos, sin and positions go together (n_pos=%d)", n_pos);
@@ -208,7 +210,6 @@ extern "C" int molly_paged_kv_append(void* stream, const void* k, const void* v,
                             ldqo >= nq * head_dim), "paged_kv_append: q rows must be 16-byte aligned and hold n_heads * head_dim values (ldq=%d ldqo=%d)",
                 ldq, ldqo);
     MOLLY_CHECK(aligned16(q_norm_w) && aligned16(k_norm_w) && aligned16(cos) && aligned16(sin), "paged_kv_append: gains / tables must be 16-byte aligned");
-    if (n_rows == 0) return 0;
     AppendArgs p{};
     p.q = (const bf16_t*)q_or_null; p.k = (const bf16_t*)k; p.v = (const bf16_t*)v; p.q_out = (bf16_t*)q_out_or_null;
     p.kpool = kpool; p.vpool = vpool; p.kscale = (uint8_t*)kscale_or_null; p.vscale = (uint8_t*)vscale_or_null;
@@ -233,10 +234,11 @@ extern "C" int molly_paged_kv_read(void* stream, const void* kpool, const void* 
                                    void* v_out, int ldk, int ldv) {
     MOLLY_ENTER();
     if (int rc = check_pool("paged_kv_read", kpool, vpool, kscale_or_null, vscale_or_null, n_pages, page_size, n_kv_heads, head_dim)) return rc;
-    MOLLY_CHECK(n_rows >= 0 && slot && k_out && v_out && 2L * n_kv_heads <= 65535, "paged_kv_read: n_rows=%d; slot, k_out, v_out required", n_rows);
+    MOLLY_CHECK(n_rows >= 0, "paged_kv_read: n_rows=%d", n_rows);
+    if (n_rows == 0) return 0;
+    MOLLY_CHECK(slot && k_out && v_out && 2L * n_kv_heads <= 65535, "paged_kv_read: slot, k_out, v_out required (n_kv_heads=%d)", n_kv_heads);
     MOLLY_CHECK(aligned16(k_out) && aligned16(v_out) && ldk % 8 == 0 && ldv % 8 == 0 && ldk >= n_kv_heads * head_dim && ldv >= n_kv_heads * head_dim,
                 "paged_kv_read: output rows must be 16-byte aligned and hold n_kv_heads * head_dim values (ldk=%d ldv=%d)", ldk, ldv);
-    if (n_rows == 0) return 0;
     ReadArgs p{};
     p.kpool = kpool; p.vpool = vpool; p.kscale = (const uint8_t*)kscale_or_null; p.vscale = (const uint8_t*)vscale_or_null;
     p.slot = slot; p.k_out = (bf16_t*)k_out; p.v_out = (bf16_t*)v_out;

@@ -122,6 +122,18 @@ def test_append_without_queries_takes_their_gain_too():
     assert all(torch.equal(a.view(torch.int16), b.view(torch.int16)) for a, b in ((kp, kp2), (vp, vp2)))
 
 
+@pytest.mark.parametrize("fp8", [False, True])
+def test_append_and_read_of_no_rows(fp8):
+    q, k, v, qw, kw, cos, sin, pos = store_inputs(3, 4, 2, 64, 3)
+    kp, vp, ks, vs = empty_pools(1, 2, 16, 64, fp8)
+    slot = torch.zeros(0, dtype=torch.int32, device=DEV)
+    before = [p.view(torch.uint8).clone() for p in (kp, vp)]
+    qo = ops().paged_kv_append(k[:0], v[:0], kp, vp, slot, kscale=ks, vscale=vs, q=q[:0], qw=qw, kw=kw, cos=cos, sin=sin, positions=pos[:0])
+    kr, vr = ops().paged_kv_read(kp, vp, slot, kscale=ks, vscale=vs)
+    assert qo.shape == (0, 256) and kr.shape == vr.shape == (0, 128)
+    assert all(torch.equal(p.view(torch.uint8), b) for p, b in zip((kp, vp), before))
+
+
 def test_append_in_place_strided_and_bad_positions():
     n, nq, nkv, hd = 9, 4, 2, 64
     q, k, v, qw, kw, cos, sin, pos = store_inputs(n, nq, nkv, hd, 3)

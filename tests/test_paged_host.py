@@ -136,3 +136,13 @@ def test_key_numbers_stay_in_32_bits():
             assert keys - 1 + ahead <= 0x7fffffff and keys + align <= 0x7fffffff
             part = ((keys - 1) // parts + align) // align * align                         # n / parts rounded up, to the next multiple
             assert -(-keys // part) * part <= 0x7fffffff
+
+
+def test_no_rows_are_no_error():
+    """An empty tensor has no address."""
+    L, P = _lib.lib(), 1 << 20
+    for q in (None, P):
+        assert L.fn["molly_paged_kv_append"](None, None, None, q, q, P, P, None, None, None, 0, 4, 16, 2, 2, 64, 128, 128, 128, 128, P, P, P, P, None, 9, 1e-6) == 0
+    assert L.fn["molly_paged_kv_read"](None, P, P, P, P, None, 0, 4, 16, 2, 64, None, None, 128, 128) == 0
+    for page in (8, 48):                                          # (the pools are still looked at)
+        assert L.fn["molly_paged_kv_read"](None, P, P, P, P, None, 0, 4, page, 2, 64, None, None, 128, 128) != 0

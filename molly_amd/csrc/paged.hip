@@ -200,7 +200,7 @@ extern "C" int molly_paged_kv_append(void* stream, const void* k, const void* v,
     if (n_rows == 0) return 0;                       // (no rows have no address: nothing else is asked of them)
     MOLLY_CHECK(nq >= 0 && k && v && slot, "paged_kv_append: n_heads=%d; k, v, slot required", n_heads);
     MOLLY_CHECK((q_or_null == nullptr) == (q_out_or_null == nullptr), "paged_kv_append: q and q_out go together");
-    MOLLY_CHECK((cos == nullptr) == (sin == nullptr) && (cos == nullptr || (positions != nullptr && n_pos > 0)),
+    MOLLY_CHECK((cos == nullptr) == (sin == nullptr) && (cos == nullptr) == (positions == nullptr) && (cos == nullptr || n_pos > 0),
                 "paged_kv_append: cos, sin and positions go together (n_pos=%d)", n_pos);
     MOLLY_CHECK((nq + 2L * n_kv_heads) * ((long)n_rows / 32 + 1) <= 0x7fffffffL, "paged_kv_append: %d rows of %d + 2 * %d heads: more than one call takes",
                 n_rows, nq, n_kv_heads);

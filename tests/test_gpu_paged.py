@@ -134,6 +134,14 @@ def test_append_and_read_of_no_rows(fp8):
     assert all(torch.equal(p.view(torch.uint8), b) for p, b in zip((kp, vp), before))
 
 
+def test_tables_without_rows_are_refused():
+    _, k, v, _, _, cos, sin, pos = store_inputs(3, 4, 2, 64, 3)
+    kp, vp, _, _ = empty_pools(1, 2, 16, 64, False)
+    with pytest.raises(RuntimeError, match="go together"):
+        ops().paged_kv_append(k, v, kp, vp, torch.arange(3, device=DEV, dtype=torch.int32), cos=cos[:0], sin=sin[:0], positions=pos)
+    assert torch.isnan(kp).all() and torch.isnan(vp).all()
+
+
 def test_append_in_place_strided_and_bad_positions():
     n, nq, nkv, hd = 9, 4, 2, 64
     q, k, v, qw, kw, cos, sin, pos = store_inputs(n, nq, nkv, hd, 3)

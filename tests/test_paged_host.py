@@ -146,3 +146,11 @@ def test_no_rows_are_no_error():
     assert L.fn["molly_paged_kv_read"](None, P, P, P, P, None, 0, 4, 16, 2, 64, None, None, 128, 128) == 0
     for page in (8, 48):                                          # (the pools are still looked at)
         assert L.fn["molly_paged_kv_read"](None, P, P, P, P, None, 0, 4, page, 2, 64, None, None, 128, 128) != 0
+
+
+def test_positions_without_tables_are_refused():
+    """Tables without rows have no address: they are not the same as none, the rows would go in unturned."""
+    L, P = _lib.lib(), 1 << 20
+    for cos, sin, pos, n_pos in ((None, None, P, 0), (None, None, P, 9), (P, P, P, 0), (P, None, P, 9), (None, P, None, 9)):
+        assert L.fn["molly_paged_kv_append"](None, P, P, None, None, P, P, None, None, P, 4, 4, 16, 0, 2, 64, 0, 128, 128, 0, None, None, cos, sin, pos, n_pos, 1e-6) != 0
+        assert "go together" in L.last_error()

@@ -26,7 +26,7 @@ class GenerationSession:
     def __init__(self, model, max_new_tokens: int, use_graph: bool = None, kv_cache: str = "dense", prefill_chunk: Optional[int] = None,
                  page_size: int = 64):
         """kv_cache: 'dense' (one [B, T + max_new] rectangle a layer), 'paged' or 'paged_e4m3'; prefill_chunk: most prompt tokens of a sequence taken at a
-        time (paged caches; None: the whole prompt)."""
+        time (paged caches; None: the whole prompt): the prefill's activations are those of that many."""
         import os
         if kv_cache not in ("dense", "paged", "paged_e4m3"):
             raise ValueError(f"GenerationSession: kv_cache must be 'dense', 'paged' or 'paged_e4m3', got {kv_cache!r}")
@@ -61,10 +61,13 @@ class GenerationSession:
         # the session's GEMM scratch is sized BEFORE its first GEMM (the launcher's split-K choices look at how much there is: a
         # workspace that grew between the prefill and a later one of the same shape could cut the second differently)
         ops.ensure_gemm_workspace(32 * 4 * max(B, 8) * max(2 * e.ff, e.nqkv), dev)
-        hs, _ = m._embed_and_inject(m._stage(input_ids, None, None, omic_ids, omic_info_list, want_sort=False), False)
-        e.reserve(B * T, B, T, training=False)
+        st = m._stage(input_ids, None, None, omic_ids, omic_info_list, want_sort=False)
         if self.kv_cache != "dense":
+            hs = torch.empty(B * T, e.h, dtype=BF16, device=dev)               # (the layers' rows are the chunks', not the rectangle's)
+            m._embed_and_inject(st, False, out=hs)
             return self._prefill_paged(hs, mask, pos)
+        hs, _ = m._embed_and_inject(st, False)
+        e.reserve(B * T, B, T, training=False)
         # rope tables must cover prompt + generated positions
         from .qwen3 import rope_tables
         self.cos, self.sin = rope_tables(self.Tmax, e.hd, e.cfg.rope_theta, dev, e.rope_table_dtype)
@@ -117,7 +120,8 @@ class GenerationSession:
         self._lora(i, "down_proj", a["act"], out)
 
     def _prefill_paged(self, hs, mask, pos) -> torch.Tensor:
-        """The prompts' tokens without their padding, `prefill_chunk` of every sequence at a time, through the layers and into the pages."""
+        """The prompts' tokens without their padding, `prefill_chunk` of every sequence at a time, through the layers and into the pages.  The layers' activations
+        are those of the largest chunk: only the embeddings (hs) have a row for every place of the prompts' rectangle."""
         from .paged import PagedKVCache
         from .qwen3 import rope_tables
         e, dev = self.eng, self.rt.dev
@@ -139,8 +143,13 @@ class GenerationSession:
         self.places = places.to(dev)
         cols = [mask[b].nonzero().flatten() for b in range(B)]                # the columns that hold tokens
         chunk = self.prefill_chunk or max(n_valid)
+        most_rows = sum(min(chunk, n) for n in n_valid)                       # (the first chunk's: no later one has more)
         if e.lora is not None:
-            self.lt = torch.empty(max(sum(min(chunk, n) for n in n_valid), B), e.lora.rp, dtype=BF16, device=dev)
+            self.lt = torch.empty(max(most_rows, B), e.lora.rp, dtype=BF16, device=dev)
+        rows_of = lambda width: torch.empty(most_rows, width, dtype=BF16, device=dev)      # noqa: E731
+        scratch = dict(xn=rows_of(e.h), qkv=rows_of(e.nqkv), qk=rows_of(e.nqk), attn=rows_of(nq), x2=rows_of(e.h), xn2=rows_of(e.h), gu=rows_of(2 * e.ff),
+                       act=rows_of(e.ff))
+        x_all, out_all = rows_of(e.h), rows_of(e.h)
         last = torch.empty(B, e.h, dtype=BF16, device=dev)
         i32 = lambda x: torch.tensor(x, dtype=torch.int32, device=dev)        # noqa: E731
         for c0 in range(0, max(n_valid), chunk):
@@ -153,8 +162,8 @@ class GenerationSession:
             for k in new:
                 cu.append(cu[-1] + k)
             cu_q, kv_len = i32(cu), i32([min(c0 + chunk, m) for m in n_valid])
-            a = {k: v[:n] for k, v in e.A[0].items() if k in ("xn", "qkv", "qk", "attn", "x2", "xn2", "gu", "act")}
-            x, out = (torch.empty(n, e.h, dtype=BF16, device=dev) for _ in range(2))
+            a = {k: v[:n] for k, v in scratch.items()}
+            x, out = x_all[:n], out_all[:n]
             ops.copy_rows(hs, x, n, src_idx32=rows)
             for i in range(L):
                 w = e.W[i]

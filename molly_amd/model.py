@@ -451,19 +451,22 @@ class OmicsOne(_MetaSafe):
                                     want_sort=want_sort)
 
     @_in_gemm_ctx
-    def _embed_and_inject(self, st, keep_for_backward, wait_embed=None, wait_proj=None):
+    def _embed_and_inject(self, st, keep_for_backward, wait_embed=None, wait_proj=None, out=None):
         """reference: src/model/omics_one.py:164-172 — token embeddings, then encoder -> projector -> overwrite.  `st` is the
         staged batch (device-side ids, encoder ids, scatter indices).
         Launch order: the FROZEN encoders run first — they read no trainable parameter, so their ≈8 ms cover the head of the
         previous step's side-stream AdamW / all-gather (embedding, gains, projectors), which `wait_embed` / `wait_proj` then
-        find finished; the values written are those of the reference's order (lookup, then overwrite)."""
+        find finished; the values written are those of the reference's order (lookup, then overwrite).
+        out: [B * T, hidden] for the embeddings, where the decoder's own buffers of all B * T rows are not wanted (None: those are reserved)."""
         rt = self._rt
         B, T = st.B, st.T
         M = B * T
         if not keep_for_backward and getattr(rt, "opt", None) is not None:
             rt.opt.wait_all_params()              # inference entry points: every parameter must have been published
-        rt.llm.reserve(M, B, T, training=keep_for_backward)
-        hs = rt.llm.A[0]["x"] if keep_for_backward else rt.llm.x_out
+        if out is None:
+            rt.llm.reserve(M, B, T, training=keep_for_backward)
+            out = rt.llm.A[0]["x"] if keep_for_backward else rt.llm.x_out
+        hs = out
         saved = {}
         encoded = []
         if rt.train_bio or os.environ.get("MOLLY_ENC_FIRST", "1") == "0":   # trained encoders read parameters the optimizer is publishing

@@ -183,3 +183,28 @@ def test_a_row_without_a_token_is_an_error(tiny_meta, how):
     # row 0 ends with its first token; that it may then say nothing but what is banned is nobody's business
     out = gen(max_new_tokens=3, no_repeat_ngram_size=1, prefix_allowed_tokens_fn=lambda r, x: [60 + len(x)] if r else [9])
     assert out[0].tolist() == [9, m.text_config.pad_token_id, m.text_config.pad_token_id] and out[1].tolist() == [60, 61, 62]
+
+
+def test_prefill_chunk_bounds_the_activations(tiny_meta):
+    """A layer's rows are those of the chunk: xn, x2, xn2, x, out | qkv | qk | attn | gate and up, act.  (The rest is the same for both: weights, pages, embeddings; a chunk's
+    attention may take a few MB of scratch: a fifth of the difference is left for it.)"""
+    from molly_amd.synth import synth_batch
+    m = build_tiny(tiny_meta)
+    c = tiny_meta["config"]
+    B, T, chunk = 2, 4000, 96
+    b = synth_batch(B, T, [("protein", 64)], seed=3, text_vocab=1000, special_ids={k: tuple(v) for k, v in c["special_ids"].items()}, pad_id=1000)
+    batch = (b["input_ids"], None, b["omic_ids"], b["omic_info_list"])
+    t = c["text"]
+    hd, nh, nkv = t["head_dim"], t["num_attention_heads"], t["num_key_value_heads"]
+    row = 2 * (5 * t["hidden_size"] + (nh + 2 * nkv) * hd + (nh + nkv) * hd + nh * hd + 3 * t["intermediate_size"])
+
+    def run(k):
+        torch.cuda.synchronize()
+        torch.cuda.reset_peak_memory_stats()
+        s, logits = _session(m, batch, kv_cache="paged", prefill_chunk=k)
+        return torch.cuda.max_memory_allocated(), logits
+    run(chunk)                                                    # (what the encoders and the GEMMs keep)
+    (whole, lw), (cut, lc) = run(None), run(chunk)
+    assert whole - cut >= 0.8 * row * B * (T - chunk), (whole, cut, row)
+    assert m._runtime().llm.cap == 0                              # the decoder's own buffers for the whole rectangle were not asked for
+    assert (lw - lc).abs().max() <= 3e-2 * lw.abs().max()

@@ -68,7 +68,7 @@ __device__ __forceinline__ Tile make_tile(const AttnPagedArgs& p, int b, int ti)
     t.tok0 = s; t.n = e - s;
     t.row0 = ti * ROWS;
     t.rows = min(ROWS, t.n * p.G - t.row0);
-    t.first = p.kv_len[b] - t.n;
+    t.first = max(p.kv_len[b], 0) - t.n;             // (less than no keys: no row sees one either way, and the difference stays in 32 bits)
     t.n_vis = t.rows > 0 ? t.first + (t.row0 + t.rows - 1) / p.G + 1 : 0;
     return t;
 }

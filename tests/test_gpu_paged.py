@@ -308,6 +308,18 @@ def test_attn_paged_rows_that_see_nothing(fp8):
     assert (keep == 3.0).all()
 
 
+@pytest.mark.parametrize("fp8", [False, True])
+@pytest.mark.parametrize("new", [[1, 1, 2], [5, 3, 70], [1, 90, 200]])
+def test_attn_paged_any_negative_number_of_keys_is_none(new, fp8):
+    """kv_len - n of the smallest int is no small number."""
+    q, kp, vp, ks, vs, table, cu, keys, cu_t, len_t = case(new, [40, 300, 200], 4, 2, 64, 16, fp8)
+    good = ops().attn_paged(q, kp, vp, table, cu_t, len_t, 4, kscale=ks, vscale=vs, max_q=max(new))
+    for few in (0, -1, -2 ** 31, -2 ** 31 + 1, -2 ** 31 + 60):
+        len_t[0], len_t[2] = few, few
+        out = ops().attn_paged(q, kp, vp, table, cu_t, len_t, 4, kscale=ks, vscale=vs, max_q=max(new))
+        assert not out[: cu[1]].any() and not out[cu[2]:].any() and torch.equal(out[cu[1]:cu[2]], good[cu[1]:cu[2]])
+
+
 def test_attn_paged_rows_outside_the_sequences_stay():
     q, kp, vp, ks, vs, table, cu, keys, cu_t, len_t = case([4, 30], [50, 30], 4, 2, 128, 16, False)
     pad = torch.cat([q[:3], q, q[:20]])

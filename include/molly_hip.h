@@ -411,14 +411,16 @@ int molly_attn_decode_qkv(void* stream, const float* qkv_slabs, int n_slabs, con
  * A layer's cache is two pools, K and V, [n_pages][n_kv_heads][page_size][head_dim] contiguous, 16-byte aligned; a place (slot) is
  * page * page_size + offset.  page_size: a power of two in 16..256; head_dim 64 | 128; n_pages * page_size < 2^31.
  * kscale / vscale NULL: bf16 pools.  Given: e4m3 pools (1 byte a value) and their exponent bytes [n_pages][n_kv_heads][page_size]: a head of a
- * token holds code * 2^(e - 127), e the smallest with which its largest finite magnitude is at most 448 * 2^(e - 127); infinities and NaN are NaN.
+ * token holds code * 2^(e - 127), e the smallest from 1 on with which its largest finite magnitude is at most 448 * 2^(e - 127); infinities and NaN
+ * are NaN.  A held value is read (here and by the attention) as the nearest bf16: itself for e in 3 .. 246; magnitudes up to 448 * 2^-125 (e 1, 2) may fall on bf16's
+ * subnormals, and a code of 2^128 (e 247) is infinite.
  *
  * append: rows of k and v (row strides ldk / ldv) go to slot[row]; a slot outside the pool (-1) skips the row.  With gains (nullable, each by
  * itself) the heads of q and k get RMSNorm, with cos / sin [n_pos][head_dim / 2] rotary at positions[row] (HF:models/qwen3/
  * modeling_qwen3.py:225-236); a position outside the tables makes the row's heads NaN.  q rows (nullable) go to q_out (q_out == q allowed).
- * fp32 throughout, one rounding where a value is stored.  Slots of one call are distinct (two rows with one slot: the pool keeps
- * values of either).
- * read: the rows of slot[] back as bf16 (exact for either kind of pool); a slot outside the pool gives a row of zeros. */
+ * fp32 throughout, one rounding where a value is stored.  Slots of one call are distinct (two rows with one slot: the
+ * place then holds parts of both, in an e4m3 pool perhaps the codes of one with the exponent of the other).
+ * read: the rows of slot[] back as bf16 (bf16 pools: the very bits); a slot outside the pool gives a row of zeros. */
 int molly_paged_kv_append(void* stream, const void* k, const void* v, const void* q_or_null, void* q_out_or_null, void* kpool, void* vpool,
                           void* kscale_or_null, void* vscale_or_null, const int* slot, int n_rows, int n_pages, int page_size, int n_heads,
                           int n_kv_heads, int head_dim, int ldq, int ldk, int ldv, int ldqo, const void* q_norm_w, const void* k_norm_w,

@@ -12,7 +12,7 @@
 //                            keys, double-buffered.  Bound by the matrix pipes where the chunk is long.
 // Either cuts the key axis over blocks where there are too few tiles to fill the chip; attn_paged_join_kernel joins the parts.
 // A bf16 step's rows go straight to LDS by DMA (16 keys lie within one page, so one page id serves a wave's piece); e4m3 codes pass through registers,
-// are turned into bf16 there (exact) and stored into the same image: one set of fragment reads serves both.
+// are turned into bf16 there (exactly, but for paged.h's two ends) and stored into the same image: one set of fragment reads serves both.
 #include "attn_frag.h"
 #include "common.h"
 #include "molly_hip.h"

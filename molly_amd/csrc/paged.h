@@ -4,10 +4,12 @@
 // row of page ids.  Head-major: the keys of one (page, head) are contiguous, so what one workgroup of the attention reads are
 // whole lines, page_size * head_dim values at a time.
 //
-// e4m3 pools: a head of a token is held as codes and ONE exponent byte e: value = code * 2^(e - 127).  e is the smallest power of two that
-// brings the head's largest magnitude to 448 (the format's largest value) or less.  With a power of two the division and the product
+// e4m3 pools: a head of a token is held as codes and ONE exponent byte e in 1 .. 247: value = code * 2^(e - 127).  e - 127 is the smallest power of two (from
+// -126 on) that brings the head's largest finite magnitude to 448 (the format's largest value) or less.  With a power of two the division and the product
 // are exact: the only rounding is the code's own (round to nearest even, half a step: 2^-4 of the value), the value read back is
-// a bf16 without rounding, and one conversion instruction (v_cvt_scalef32_pk_bf16_fp8) makes two of them.  What a
+// a bf16 without another rounding for e in 3 .. 246, and one conversion instruction (v_cvt_scalef32_pk_bf16_fp8) makes two of them.  Beyond that bf16 ends before the format
+// does: with e 1 and 2 (a head of magnitudes up to 448 * 2^-125 = 1.1e-35) the smallest codes, multiples of 2^-135 and 2^-134, are rounded to nearest even to bf16's subnormals of 2^-133;
+// with e 247 (a magnitude above 1.75 * 2^127 = 3.0e38) the code that stands for 2^128 is read back as infinity.  What a
 // free scale would gain is nothing above the format's subnormals: a code keeps its 4 significant bits wherever it sits in the 15 octaves.
 #pragma once
 #include "common.h"

@@ -833,7 +833,7 @@ def _ints(t, dev, what, name, shape):
 
 def paged_kv_append(k, v, kpool, vpool, slot, kscale=None, vscale=None, q=None, q_out=None, qw=None, kw=None, cos=None, sin=None,
                     positions=None, eps=1e-6):
-    """Rows of k and v [n, kv heads * dim] into the places slot (int32 [n], page * page_size + offset; -1: the row is padding) of the pools, with
+    """Rows of k and v [n, kv heads * dim] into the places slot (int32 [n], page * page_size + offset, each place once; -1: the row is padding) of the pools, with
     q/k-norm (gains qw / kw [dim]) and rotary (cos / sin fp32 [n_pos, dim / 2], positions int32 [n]) of k, and of q [n, heads * dim], in the same
     pass where they are given (molly_paged_kv_append; qw without q is not used).  Row strides are free.
     -> q's rows after both (q_out; q_out may be q), or None."""

@@ -112,6 +112,23 @@ def test_append_codes_match_the_format():
     assert torch.equal(kr.double().nan_to_num(7.0), val.bfloat16().double().nan_to_num(7.0)) and torch.equal(torch.isnan(kr), torch.isnan(vr))
 
 
+@pytest.mark.parametrize("e", [1, 2, 3, 4, 100, 127, 246, 247])
+def test_every_code_is_read_as_the_nearest_bf16(e):
+    """Exactly what it stands for with exponent bytes of 3 .. 246; below, bf16's subnormals are coarser than the smallest codes; above, 2^128 is no bf16."""
+    codes = torch.arange(256, dtype=torch.int32, device=DEV).to(torch.uint8)
+    kp = torch.zeros(1, 1, 16, 128, dtype=torch.uint8, device=DEV)
+    kp.view(-1)[:256] = codes
+    kp, ks = kp.view(torch.float8_e4m3fn), torch.full((1, 1, 16), e, dtype=torch.uint8, device=DEV)
+    kr, vr = ops().paged_kv_read(kp, kp, torch.arange(2, dtype=torch.int32, device=DEV), kscale=ks, vscale=ks)
+    held = C.held(kp, ks).view(-1)[:256]
+    want = held.cpu().float().bfloat16()                          # (float32 holds them all; one rounding)
+    for got in (kr, vr):
+        got = got.view(-1).cpu()
+        assert torch.equal(torch.isnan(got), torch.isnan(want)) and torch.equal(got[~torch.isnan(want)], want[~torch.isnan(want)])
+    fin = torch.isfinite(held.cpu())
+    assert bool((want.double() == held.cpu())[fin].all()) == (3 <= e <= 246)
+
+
 def test_append_without_queries_takes_their_gain_too():
     _, k, v, qw, kw, *_ = store_inputs(9, 4, 2, 64, 3)
     slot = torch.arange(9, device=DEV, dtype=torch.int32)

@@ -1,4 +1,4 @@
-// What the attention kernels (attention.hip, paged.hip) share: the LDS tile image that serves row reads and transposed reads, the fragments of the
+// What the attention kernels (attention.hip, attn_paged.hip) share: the LDS tile image that serves row reads and transposed reads, the fragments of the
 // 32x32x16 bf16 MFMA taken from it, and the softmax's small parts.  Orientation: S^T = K Q^T, so a lane owns ONE query column
 // (lane & 31) with its keys in registers, and P^T in bf16 is directly the B operand of O^T = V^T P^T.
 #pragma once

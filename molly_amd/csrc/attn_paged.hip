@@ -8,8 +8,8 @@
 // domain in fp32, P in bf16 for the second product (one bf16 in the tiles, the sum of two in the rows: attend32).  Two kernels:
 //   attn_paged_rows_kernel : up to 32 rows a tile (decode, short chunks).  The 4 | 8 waves of a block take turns at steps of 32 keys, each with
 //                            K / V images of its own in LDS: no workgroup barrier in the loop, the waves meet at the end.  Bound by HBM.
-//   attn_paged_tile_kernel : 128 rows a tile (prompt chunks, mixed batches).  The waves own 32 rows each and share K / V tiles of 64
-//                            keys, double-buffered.  Bound by the matrix pipes where the chunk is long.
+//   attn_paged_tile_kernel : 128 rows a tile (prompt chunks, mixed batches), 64 where there are few tiles (KS 2: two waves a row, half of the keys each).  The waves
+//                            own 32 rows each and share K / V tiles of 64 keys, double-buffered.  Bound by the matrix pipes where the chunk is long.
 // Either cuts the key axis over blocks where there are too few tiles to fill the chip; attn_paged_join_kernel joins the parts.
 // A bf16 step's rows go straight to LDS by DMA (16 keys lie within one page, so one page id serves a wave's piece); e4m3 codes pass through registers,
 // are turned into bf16 there (exactly, but for paged.h's two ends) and stored into the same image: one set of fragment reads serves both.
@@ -28,9 +28,10 @@ constexpr long MAX_KEYS = 0x7fffffffL - 32768;
 
 // The parts that a tile's key axis is cut into, at most `parts`, and a part's keys (whole ones of `align`).  A part has 2^shift keys or so at least (`round`: what
 // counts as the last one); an axis of which a cut would take fewer than min_cut keys out of a block's way stays whole.
-//   single steps: a round of the block's waves or more, min_cut 700.  On the GPU the join costs 4 us and a key 9 ns, and a cut pays from 400 keys on (1 x 700
-//     keys bf16 11.1 -> 9.5 us in a graph; 1 x 300 7.9 -> 9.8); called one by one the second launch and its scratch cost the host 4 us more, and it pays from 1,000
-//     on (1 x 700 11.5 -> 15.2).  1 x 2,000 in a graph 15.1 (parts of 512 and more) -> 10.7, 4 x 2,000 15.9 -> 12.8; 16 x 700 e4m3, cut in two, 12.7 -> 14.7
+//   single steps: a round of the block's waves or more, min_cut 700: 828 keys and more are cut where a round is 128 keys, 956 where it is 256.  On the GPU the join costs 4 us
+//     and a key 9 ns, and a cut pays from 400 keys saved on (in a graph, bf16: 1 x 700 11.1 -> 9.5 us, 1 x 300 7.9 -> 9.8, 1 x 828 11.8 -> 9.2, 1 x 2,000 20.9 -> 10.0, 4 x 2,000
+//     23.7 -> 12.0).  Called one by one the second launch and its scratch are host time, and it pays from some 1,100 keys on (1 x 700 11.5 -> 15.2, 1 x 828 11.9 -> 14.2,
+//     1 x 1,000 13.0 -> 14.1, 1 x 1,200 15.2 -> 14.1; with a scratch of the caller's 12.2 each): 700 lies between.  16 x 700 e4m3, cut in two in a graph, 12.7 -> 14.7
 //   tiles: 512 keys or more, for their parts carry more rows (2 x 100 new tokens x 32 heads over 1,000 keys 19.7 us, parts of 128 21.8); 128 where that makes
 //     more parts, up to 16 and as long as they come to 10,240 rows (32 new tokens x 32 heads over 700 keys 15.3 -> 13.1 us, over 2,500 18.5 -> 15.5)
 struct CutRule { int parts, align, shift, round, min_cut; };

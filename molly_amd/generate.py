@@ -63,7 +63,7 @@ class GenerationSession:
         ops.ensure_gemm_workspace(32 * 4 * max(B, 8) * max(2 * e.ff, e.nqkv), dev)
         st = m._stage(input_ids, None, None, omic_ids, omic_info_list, want_sort=False)
         if self.kv_cache != "dense":
-            hs = torch.empty(B * T, e.h, dtype=BF16, device=dev)               # (the layers' rows are the chunks', not the rectangle's)
+            hs = e.prompt_rows(B * T)                                          # (the layers' rows are the chunks', not the rectangle's)
             m._embed_and_inject(st, False, out=hs)
             return self._prefill_paged(hs, mask, pos)
         hs, _ = m._embed_and_inject(st, False)
@@ -146,10 +146,7 @@ class GenerationSession:
         most_rows = sum(min(chunk, n) for n in n_valid)                       # (the first chunk's: no later one has more)
         if e.lora is not None:
             self.lt = torch.empty(max(most_rows, B), e.lora.rp, dtype=BF16, device=dev)
-        rows_of = lambda width: torch.empty(most_rows, width, dtype=BF16, device=dev)      # noqa: E731
-        scratch = dict(xn=rows_of(e.h), qkv=rows_of(e.nqkv), qk=rows_of(e.nqk), attn=rows_of(nq), x2=rows_of(e.h), xn2=rows_of(e.h), gu=rows_of(2 * e.ff),
-                       act=rows_of(e.ff))
-        x_all, out_all = rows_of(e.h), rows_of(e.h)
+        scratch = e.prefill_rows(most_rows, None if self.prefill_chunk is None else B * chunk)
         last = torch.empty(B, e.h, dtype=BF16, device=dev)
         i32 = lambda x: torch.tensor(x, dtype=torch.int32, device=dev)        # noqa: E731
         for c0 in range(0, max(n_valid), chunk):
@@ -162,8 +159,8 @@ class GenerationSession:
             for k in new:
                 cu.append(cu[-1] + k)
             cu_q, kv_len = i32(cu), i32([min(c0 + chunk, m) for m in n_valid])
-            a = {k: v[:n] for k, v in scratch.items()}
-            x, out = x_all[:n], out_all[:n]
+            a = {k: scratch[k][:n] for k in ("xn", "qkv", "qk", "attn", "x2", "xn2", "gu", "act")}
+            x, out = scratch["x"][:n], scratch["out"][:n]
             ops.copy_rows(hs, x, n, src_idx32=rows)
             for i in range(L):
                 w = e.W[i]

@@ -72,6 +72,7 @@ class Qwen3Engine:
         # (the down_proj adapter adds to d(act)); MOLLY_FUSED_SWIGLU_BWD=0 restores dgrad + swiglu_bwd
         self.fused_swiglu_bwd = lora is None and os.environ.get("MOLLY_FUSED_SWIGLU_BWD", "1") != "0"
         self.cap = 0
+        self.chunk_rows, self.chunk, self.prompt = 0, None, None      # a paged prefill's buffers
         self.tT = None
         self.tTg, self._pend = None, []   # grouped per-layer weight gradients (reserve)
         self.grads_final_hook = None      # callable(lo, hi): flat-offset range of gradients that became final (ZeRO overlap)
@@ -105,6 +106,28 @@ class Qwen3Engine:
             self.d_norm_w = self.G.views[self.pre + "model.norm.weight"]
 
     # ---- activation slabs -----------------------------------------------------------------------------------
+    def prefill_rows(self, rows: int, most: int = None) -> dict:
+        """One layer's activations for `rows` tokens of a paged prefill (the first of as many rows as there are): the buffers of `reserve` where they hold as many, else
+        a set that is kept for the next prefill (what is given back between two generations goes to the driver with a graph's capture, and each would allocate it anew),
+        unless it has more than `most` rows."""
+        if self.cap >= rows:
+            return dict(self.A[0], out=self.hn)
+        if self.chunk_rows < rows or (most is not None and self.chunk_rows > most):
+            self.chunk_rows, self.chunk = rows, None              # (the old ones go before the new ones come)
+            e = lambda w: torch.empty(rows, w, dtype=BF16, device=self.dev)
+            self.chunk = dict(x=e(self.h), out=e(self.h), xn=e(self.h), qkv=e(self.nqkv), qk=e(self.nqk), attn=e(self.nh * self.hd), x2=e(self.h), xn2=e(self.h),
+                              gu=e(2 * self.ff), act=e(self.ff))
+        return self.chunk
+
+    def prompt_rows(self, rows: int) -> torch.Tensor:
+        """[rows, hidden] for the embeddings of a paged prefill's prompts, kept likewise."""
+        if self.cap >= rows:
+            return self.x_out[:rows]
+        if self.prompt is None or self.prompt.shape[0] < rows:
+            self.prompt = None
+            self.prompt = torch.empty(rows, self.h, dtype=BF16, device=self.dev)
+        return self.prompt[:rows]
+
     def reserve(self, M: int, B: int, T: int, training: bool):
         """Allocate (once) every buffer a forward/backward over M = B*T tokens needs."""
         if self.cap >= M and getattr(self, "_train_alloc", False) >= training and self.BT == (B, T):
@@ -112,6 +135,7 @@ class Qwen3Engine:
         dev, h, ff = self.dev, self.h, self.ff
         e = lambda *s, dt=BF16: torch.empty(*s, dtype=dt, device=dev)
         self.cap, self.BT, self._train_alloc = M, (B, T), training
+        self.chunk_rows, self.chunk, self.prompt = 0, None, None
         nl = self.L if training else 1                    # inference keeps one layer's worth of scratch
         self.A = []
         for _ in range(nl):

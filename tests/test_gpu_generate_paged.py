@@ -204,7 +204,38 @@ def test_prefill_chunk_bounds_the_activations(tiny_meta):
         s, logits = _session(m, batch, kv_cache="paged", prefill_chunk=k)
         return torch.cuda.max_memory_allocated(), logits
     run(chunk)                                                    # (what the encoders and the GEMMs keep)
-    (whole, lw), (cut, lc) = run(None), run(chunk)
+    cut, lc = run(chunk)
+    whole, lw = run(None)
     assert whole - cut >= 0.8 * row * B * (T - chunk), (whole, cut, row)
     assert m._runtime().llm.cap == 0                              # the decoder's own buffers for the whole rectangle were not asked for
     assert (lw - lc).abs().max() <= 3e-2 * lw.abs().max()
+    # the rows are kept for the next prefill, and a chunk's replace a whole prompt's
+    e = m._runtime().llm
+    kept = {k: v.data_ptr() for k, v in e.chunk.items()}
+    run(None)
+    assert {k: v.data_ptr() for k, v in e.chunk.items()} == kept and e.chunk_rows == B * T
+    run(chunk)
+    assert e.chunk_rows == B * chunk == e.chunk["x"].shape[0]
+    run(chunk // 2)
+    assert e.chunk_rows == B * (chunk // 2)
+
+
+@pytest.mark.parametrize("chunk", [None, 50])
+def test_paged_prefill_in_the_decoder_s_own_rows(tiny_meta, chunk):
+    """Behind a dense session (or a training step) the rows are there already: none are allocated beside them, and the logits are the same bits; a larger batch gets rows
+    of its own, and the decoder's next allocation gives them up."""
+    batch = _left_padded_batch(tiny_meta)
+    m = build_tiny(tiny_meta)
+    own, want = _session(m, batch, kv_cache="paged", prefill_chunk=chunk)
+    e = m._runtime().llm
+    assert e.cap == 0 and e.chunk_rows > 0 and e.prompt is not None
+    _session(m, batch)                                            # dense
+    assert e.cap == batch[0].numel() and e.chunk_rows == 0 and e.chunk is None and e.prompt is None
+    shared, got = _session(m, batch, kv_cache="paged", prefill_chunk=chunk)
+    assert e.chunk is None and e.prompt is None and torch.equal(got, want)
+    tok = want.argmax(-1)
+    assert torch.equal(shared.step(tok), own.step(tok))
+    twice = tuple(torch.cat([t, t]) for t in batch[:3]) + (batch[3] * 2,)
+    _, both = _session(m, twice, kv_cache="paged")
+    assert e.chunk_rows == 2 * int(batch[1].sum()) and e.prompt.shape[0] == twice[0].numel() and e.cap == batch[0].numel()
+    assert (both[:2] - want).abs().max() <= 3e-2 * want.abs().max() and (both[2:] - want).abs().max() <= 3e-2 * want.abs().max()

@@ -113,10 +113,11 @@ class Qwen3Engine:
         if self.cap >= rows:
             return dict(self.A[0], out=self.hn)
         if self.chunk_rows < rows or (most is not None and self.chunk_rows > most):
-            self.chunk_rows, self.chunk = rows, None              # (the old ones go before the new ones come)
+            self.chunk_rows, self.chunk = 0, None                 # (the old ones go before the new ones come)
             e = lambda w: torch.empty(rows, w, dtype=BF16, device=self.dev)
             self.chunk = dict(x=e(self.h), out=e(self.h), xn=e(self.h), qkv=e(self.nqkv), qk=e(self.nqk), attn=e(self.nh * self.hd), x2=e(self.h), xn2=e(self.h),
                               gu=e(2 * self.ff), act=e(self.ff))
+            self.chunk_rows = rows
         return self.chunk
 
     def prompt_rows(self, rows: int) -> torch.Tensor:

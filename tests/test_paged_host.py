@@ -154,3 +154,23 @@ def test_positions_without_tables_are_refused():
     for cos, sin, pos, n_pos in ((None, None, P, 0), (None, None, P, 9), (P, P, P, 0), (P, None, P, 9), (None, P, None, 9)):
         assert L.fn["molly_paged_kv_append"](None, P, P, None, None, P, P, None, None, P, 4, 4, 16, 0, 2, 64, 0, 128, 128, 0, None, None, cos, sin, pos, n_pos, 1e-6) != 0
         assert "go together" in L.last_error()
+
+
+def test_prefill_rows_behind_a_failed_allocation(monkeypatch):
+    """Rows that could not be had are not taken for rows that are there; smaller ones are had afterwards."""
+    from molly_amd.qwen3 import Qwen3Engine
+    e = Qwen3Engine.__new__(Qwen3Engine)
+    e.h, e.hd, e.nh, e.nkv, e.ff, e.nqkv, e.nqk, e.dev = 8, 4, 2, 1, 16, 16, 12, "cpu"
+    e.cap, e.chunk_rows, e.chunk, e.prompt = 0, 0, None, None
+    assert e.prefill_rows(8)["gu"].shape == (8, 32) and e.chunk_rows == 8 and e.prefill_rows(5) is e.chunk
+    real = torch.empty
+
+    def empty(rows, width, **kw):
+        if rows > 100 and width > 16:
+            raise torch.OutOfMemoryError("no")
+        return real(rows, width, **kw)
+    monkeypatch.setattr(torch, "empty", empty)
+    with pytest.raises(torch.OutOfMemoryError):
+        e.prefill_rows(1000)
+    assert e.prefill_rows(20)["gu"].shape == (20, 32) and e.chunk_rows == 20
+    assert e.prefill_rows(4, most=6)["act"].shape == (4, 16) and e.chunk_rows == 4
